@@ -183,6 +183,99 @@ typedef struct PthAttnWriteArgs {
   int32_t num_blocks;
 } PthAttnWriteArgs;
 
+/* Arguments of pth_attn_paged16: attention over a paged cache in the model's
+ * own 16-bit type. No counterpart in the reference. Request r has kv_lens[r]
+ * keys and, with query_start_loc NULL, the one query token r (num_tokens ==
+ * num_reqs); otherwise the tokens [query_start_loc[r], query_start_loc[r + 1]),
+ * each of which sees all of the request's keys. window > 0 (one query token
+ * per request only): the last `window` keys. A row that sees no key is 0; rows
+ * of tokens that belong to no request are not written. kv_lens are brought
+ * into [0, max_kv_len] and to the block table's reach, query_start_loc into
+ * [0, num_tokens], and a page number outside the cache is read as page 0:
+ * nothing out of bounds is touched whatever these tensors hold. */
+typedef struct PthAttnP16Args {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnP16Args) */
+
+  const void* q; /* [num_tokens, num_q_heads, head_size], 16-byte aligned rows */
+  int64_t q_stride_token; /* bytes */
+  int64_t q_stride_head;
+  void* out; /* as q */
+  int64_t out_stride_token;
+  int64_t out_stride_head;
+  int32_t dtype; /* of q, out and the cache: PTH_ATTN_F16 or PTH_ATTN_BF16 */
+
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_size;      /* 64, 128 or 256 */
+  PthAttnStream k_cache;  /* [num_blocks, block_size, num_kv_heads, head_size] */
+  PthAttnStream v_cache;
+  const int32_t* block_table; /* [>= num_reqs, block_table_width] */
+  int64_t block_table_row_stride; /* ELEMENTS between rows */
+  int32_t block_table_width;
+  int32_t max_kv_len; /* no request has more keys */
+  const int32_t* kv_lens;         /* [num_reqs] */
+  const int32_t* query_start_loc; /* [num_reqs + 1] or NULL */
+
+  int32_t num_reqs;
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t max_query_len; /* of a request (a choice of kernel only) */
+  int32_t window;        /* 0 = none */
+  float softmax_scale;
+  float* ws; /* pth_attn_paged16_workspace_floats(head_size) floats */
+  int64_t ws_floats;
+} PthAttnP16Args;
+
+/* Arguments of the 16-bit cache writer (pth_attn_write_kv16): as
+ * PthAttnWriteArgs, without scales. No counterpart in the reference. */
+typedef struct PthAttnWrite16Args {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnWrite16Args) */
+
+  const void* key;   /* [num_tokens, num_kv_heads, head_size] */
+  const void* value; /* [num_tokens, num_kv_heads, head_size] */
+  int64_t key_stride_token; /* bytes */
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  int32_t kv_dtype;    /* cache_dtype, or PTH_ATTN_F32 */
+  int32_t cache_dtype; /* PTH_ATTN_F16 or PTH_ATTN_BF16 */
+  int32_t num_tokens;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t block_size;
+  int32_t num_blocks;
+  const int64_t* slot_mapping; /* [num_tokens]; outside the cache: skipped */
+  PthAttnStream k_cache; /* [num_blocks, block_size, num_kv_heads, head_size] */
+  PthAttnStream v_cache;
+} PthAttnWrite16Args;
+
+/* Arguments of pth_attn_step_tables: a step's block tables and slot map from
+ * its request lengths. No counterpart in the reference. */
+typedef struct PthAttnTablesArgs {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnTablesArgs) */
+
+  int32_t* block_table; /* [>= num_reqs, block_table_width], in and out */
+  int64_t block_table_row_stride; /* ELEMENTS between rows */
+  int32_t block_table_width;
+  int32_t block_size;
+  int64_t* slot_mapping; /* [num_slots] out */
+  int64_t num_slots;
+  int32_t* seq_lens;        /* [num_reqs] out */
+  int32_t* query_start_loc; /* [num_reqs + 1] out */
+  int32_t* pool_out;        /* [2] out: pages taken so far, requests refused */
+  const int32_t* context_lens; /* [num_reqs] tokens in the cache */
+  const int32_t* query_lens;   /* [num_reqs] new tokens */
+  const int32_t* free_pages;   /* [num_free] */
+  int64_t num_free;
+  const int32_t* pool_in; /* [2]: pages taken before, ignored */
+  int32_t num_reqs;
+  int32_t reserved;
+} PthAttnTablesArgs;
+
 /* Loader choice of pth_attn_attention_ex. Reference: attn_capi.h:32-39.
  * loader: 0 = default, 1 = separate streams (the only loader of this
  * library; 0 and 1 are the same), 2 = whole cell (not built: EINVAL). */
@@ -271,6 +364,39 @@ int32_t pth_attn_attention_lse_noalloc(const PthAttnArgs* args, float* lse,
  * mirror: python/pth_testing/reference.py:76-103), into the cache cells.
  * Enqueued on `stream`, no sync. No counterpart in the reference's ABI. */
 int32_t pth_attn_write_kv(const PthAttnWriteArgs* args, void* stream);
+
+/* Attention of one new token per request, or of an encoder's states (cross
+ * attention), over a paged 16-bit cache: see PthAttnP16Args. At most two
+ * kernels on `stream`, no allocation, no sync. The workspace holds nothing
+ * between calls; calls that overlap in time need one each. */
+int32_t pth_attn_paged16(const PthAttnP16Args* args, void* stream);
+int32_t pth_attn_paged16_args_bytes(void);
+/* Floats of workspace of pth_attn_paged16 at this head size on the current
+ * device, whatever the batch; 0 if there is no device. */
+int64_t pth_attn_paged16_workspace_floats(int32_t head_size);
+
+/* Keys and values into a paged 16-bit cache: a copy, or (fp32) one rounding
+ * to nearest even. Slots are distinct; a slot outside the cache is skipped. */
+int32_t pth_attn_write_kv16(const PthAttnWrite16Args* args, void* stream);
+int32_t pth_attn_write16_args_bytes(void);
+
+/* A step's tables. With c = max(context_lens[r], 0), n = max(query_lens[r], 0),
+ * have = ceil(c / block_size), need = ceil((c + n) / block_size), request r
+ * takes need - have pages from free_pages, in request order from
+ * max(pool_in[0], 0) on. A request that needs more than block_table_width
+ * pages, or pages behind the end of free_pages, is refused: it takes none and
+ * its lengths stay (once the pages are short, every later request that needs
+ * one is refused too).
+ *   block_table[r, have .. need) = the pages taken; nothing else is written
+ *   seq_lens[r] = c + n, or c if refused
+ *   query_start_loc[r] = min(sum of n before r, num_slots)
+ *   slot_mapping[t] = page * block_size + position % block_size for the new
+ *     token t, -1 for one of a refused request, behind a negative page number,
+ *     or behind the last request
+ *   pool_out = {pool_in[0] + pages taken, requests refused}
+ * No output may overlap an input (block_table is both). */
+int32_t pth_attn_step_tables(const PthAttnTablesArgs* args, void* stream);
+int32_t pth_attn_tables_args_bytes(void);
 
 #ifdef __cplusplus
 } /* extern "C" */

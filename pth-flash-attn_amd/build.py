@@ -3,9 +3,8 @@
 Outputs (next to the Python package, so they travel with the source tree):
   python/pth_flash_attn/libpth_attn.so  HIP kernels + launcher + C ABI
                                         (include/pth_attn.h); no torch.
-  python/pth_flash_attn/_C.so           the torch op pth_flash_attn::pth_flash_attn_fwd
-                                        (CUDA = HIP key and CPU key), linked
-                                        against libpth_attn.so.
+  python/pth_flash_attn/_C.so           the torch ops pth_flash_attn::* (CUDA = HIP key
+                                        and CPU key), linked against libpth_attn.so.
 
 Usage: python pth-flash-attn_amd/build.py [--lib-only] [-v]
 Compiles every time it is called (no staleness check); needs hipcc only, no GPU.
@@ -29,7 +28,9 @@ ARCH = "gfx950"
 
 HIP_SOURCES = ("attn_fwd.hip", "attn_staged.hip", "attn_rows.hip", "attn_wide.hip",
                "attn_paged64.hip", "attn_generic.hip", "attn_combine.hip", "attn_launch.hip",
-               "attn_writer.hip")
+               "attn_writer.hip", "p16_rows.hip", "p16_wide.hip", "p16_writer.hip",
+               "p16_launch.hip", "step_tables.hip")
+OP_SOURCES = ("torch_op.cpp", "torch_op_p16.cpp")
 # Packed fp32 VALU ops are disabled for all device code (they have given wrong
 # results on this pool); the host pass warns that it does not know the
 # feature, which is harmless.
@@ -90,7 +91,7 @@ def build_op(verbose: bool = False) -> Path:
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         f"-I{INCLUDE}", f"-I{CSRC}", *inc, "-I/opt/rocm/include",
-        str(CSRC / "torch_op.cpp"),
+        *[str(CSRC / s) for s in OP_SOURCES],
         "-o", str(tmp),
         f"-L{PY_PKG}", "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN",
         *[f"-L{d}" for d in libdirs],

@@ -1,0 +1,147 @@
+// p16_launch.hip -- host side of attention over a paged 16-bit cache: checks,
+// the choice of kernel, the partition's size, and the C entry points.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "p16.h"
+
+namespace pa {
+namespace {
+
+bool rows_aligned(const void* p, int64_t a, int64_t b) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
+}
+bool stream_ok(const PthAttnStream& s) {
+  return rows_aligned(s.data, s.stride_block, s.stride_slot) && s.stride_head % 16 == 0 &&
+         s.stride_block >= 0 && s.stride_head >= 0 && s.stride_slot >= 0 &&
+         s.stride_slot < (1 << 24);
+}
+CacheStream stream_of(const PthAttnStream& s) {
+  return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
+                     s.stride_head};
+}
+
+}  // namespace
+
+int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
+  clear_error();
+  PA_REQUIRE(a.abi_version == PTH_ATTN_ABI_VERSION,
+             "abi_version " + std::to_string(a.abi_version) + " != library ABI " +
+                 std::to_string(PTH_ATTN_ABI_VERSION));
+  PA_REQUIRE(a.struct_bytes == static_cast<int32_t>(sizeof(PthAttnP16Args)),
+             "struct_bytes " + std::to_string(a.struct_bytes) + " != sizeof(PthAttnP16Args) " +
+                 std::to_string(sizeof(PthAttnP16Args)));
+  PA_REQUIRE(a.head_size == 64 || a.head_size == 128 || a.head_size == 256,
+             "head_size must be 64, 128 or 256");
+  PA_REQUIRE(a.dtype == PTH_ATTN_F16 || a.dtype == PTH_ATTN_BF16,
+             "dtype must be PTH_ATTN_F16 or PTH_ATTN_BF16");
+  PA_REQUIRE(a.num_reqs >= 0 && a.num_tokens >= 0 && a.num_blocks >= 1 && a.block_size >= 1,
+             "num_reqs, num_tokens >= 0, num_blocks and block_size >= 1");
+  PA_REQUIRE(a.num_kv_heads >= 1 && a.num_q_heads >= 1 && a.num_q_heads % a.num_kv_heads == 0,
+             "num_q_heads must be a positive multiple of num_kv_heads");
+  PA_REQUIRE(a.num_q_heads / a.num_kv_heads <= 64, "at most 64 query heads per KV head");
+  PA_REQUIRE(a.query_start_loc != nullptr || a.num_tokens == a.num_reqs,
+             "without query_start_loc, num_tokens must equal num_reqs");
+  PA_REQUIRE(a.query_start_loc == nullptr || a.window == 0,
+             "a window needs one query token per request");
+  PA_REQUIRE(a.window >= 0, "window must be >= 0");
+  PA_REQUIRE(a.max_kv_len >= 0 && a.block_table_width >= 0,
+             "max_kv_len and block_table_width must be >= 0");
+  PA_REQUIRE(std::isfinite(a.softmax_scale) && a.softmax_scale > 0.0f,
+             "softmax_scale must be finite and > 0");
+  if (a.num_reqs == 0 || a.num_tokens == 0) return PTH_ATTN_OK;
+  PA_REQUIRE(a.q && a.out && a.k_cache.data && a.v_cache.data && a.kv_lens,
+             "q, out, k_cache, v_cache and kv_lens must be non-NULL");
+  PA_REQUIRE(a.block_table || a.block_table_width == 0, "block_table must be non-NULL");
+  PA_REQUIRE(rows_aligned(a.q, a.q_stride_token, a.q_stride_head) &&
+                 rows_aligned(a.out, a.out_stride_token, a.out_stride_head),
+             "q and out must have 16-byte aligned rows");
+  PA_REQUIRE(stream_ok(a.k_cache) && stream_ok(a.v_cache),
+             "k_cache and v_cache must have 16-byte aligned rows, strides >= 0 and less than "
+             "2^24 bytes between slots");
+  const int32_t cus = resident_workgroups();
+  PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
+  const int64_t need = p16_workspace_floats(a.head_size, cus);
+  PA_REQUIRE(a.ws && reinterpret_cast<uintptr_t>(a.ws) % 16 == 0 && a.ws_floats >= need,
+             "ws must be 16-byte aligned and hold " + std::to_string(need) + " floats, holds " +
+                 std::to_string(a.ws_floats));
+
+  P16Params p{};
+  p.q = static_cast<const char*>(a.q);
+  p.s_q_tok = a.q_stride_token;
+  p.s_q_head = a.q_stride_head;
+  p.out = static_cast<char*>(a.out);
+  p.s_out_tok = a.out_stride_token;
+  p.s_out_head = a.out_stride_head;
+  p.k = stream_of(a.k_cache);
+  p.v = stream_of(a.v_cache);
+  p.block_table = a.block_table;
+  p.bt_stride = a.block_table_row_stride;
+  p.kv_lens = a.kv_lens;
+  p.qsl = a.query_start_loc;
+  p.ws = a.ws;
+  p.group = a.num_q_heads / a.num_kv_heads;
+  p.bs_div = Div32::make(static_cast<uint32_t>(a.block_size));
+  p.g_div = Div32::make(static_cast<uint32_t>(p.group));
+  p.num_blocks = a.num_blocks;
+  const int64_t reach = static_cast<int64_t>(a.block_table_width) * a.block_size;
+  // Key positions stay below 2^31 with a tile to spare.
+  const int64_t most = INT32_MAX - 1024;
+  p.max_keys = static_cast<int32_t>(std::min({static_cast<int64_t>(a.max_kv_len), reach, most}));
+  p.num_reqs = a.num_reqs;
+  p.num_tokens = a.num_tokens;
+  p.num_kv_heads = a.num_kv_heads;
+  p.window = a.window;
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+
+  const bool wide = a.query_start_loc != nullptr &&
+                    static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
+  const int64_t bm = wide ? kP16WideRows : kP16RowsRows, kt = wide ? kP16WideKeys : kP16RowsKeys;
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
+  PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
+  // Bounds of the partition: row tiles of all requests, key tiles of one.
+  const int64_t row_tiles = a.query_start_loc == nullptr
+                                ? a.num_reqs * ((p.group + bm - 1) / bm)
+                                : rows / bm + a.num_reqs;
+  const int64_t span = p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + 15)
+                                    : p.max_keys;
+  const int64_t key_tiles = std::max<int64_t>((span + kt - 1) / kt, 1);
+  PA_REQUIRE(row_tiles * a.num_kv_heads < INT32_MAX / key_tiles,
+             "the launch exceeds 2^31 tiles");
+  const int64_t tiles = row_tiles * a.num_kv_heads * key_tiles;
+  const int64_t fill = static_cast<int64_t>(cus) * (wide ? (a.head_size == 256 ? 1 : 2)
+                                                         : (a.head_size == 64 ? 4 : a.head_size == 128 ? 3 : 1));
+  p.num_wg = static_cast<int32_t>(std::min(tiles, fill));
+  const bool f16 = a.dtype == PTH_ATTN_F16, page16 = a.block_size % 16 == 0;
+  hipError_t err = wide ? launch_p16_wide_kernel(p, f16, page16, a.head_size, stream)
+                        : launch_p16_rows_kernel(p, f16, page16, a.head_size, stream);
+  // A unit of one tile is never cut.
+  if (err == hipSuccess && key_tiles > 1)
+    err = launch_p16_combine_kernel(p, f16, wide, a.head_size, stream);
+  if (err != hipSuccess)
+    return fail(PTH_ATTN_ECUDA, std::string("paged16 launch: ") + hipGetErrorString(err));
+  return PTH_ATTN_OK;
+}
+
+}  // namespace pa
+
+extern "C" {
+
+int32_t pth_attn_paged16_args_bytes(void) { return static_cast<int32_t>(sizeof(PthAttnP16Args)); }
+
+int64_t pth_attn_paged16_workspace_floats(int32_t head_size) {
+  const int32_t cus = pa::resident_workgroups();
+  return cus > 0 ? pa::p16_workspace_floats(head_size, cus) : 0;
+}
+
+int32_t pth_attn_paged16(const PthAttnP16Args* args, void* stream) {
+  if (args == nullptr) return pa::fail(PTH_ATTN_EINVAL, "args is NULL");
+  return pa::launch_p16(*args, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

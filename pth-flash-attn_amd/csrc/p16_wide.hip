@@ -1,0 +1,301 @@
+// p16_wide.hip -- cross attention of many query rows over a paged 16-bit
+// cache: every row of a request sees all of the request's keys. A unit is 128
+// rows of one KV head (p16.h), 32 for each of four waves, which share the key
+// tiles of 64 in LDS; two work-groups per compute unit (one at D = 256).
+//
+// Layout. v_mfma_f32_32x32x16 with the keys (or the output columns) on M and
+// the wave's query rows on N: lane l holds row l % 32, and of a 32-key score
+// tile the keys 8 b + 4 (l / 32) + i (b, i < 4), which are the B operand of the
+// PV product as they are if V takes the keys in the same order.
+// ds_read_b64_tr_b16 gives a lane one column of four consecutive keys of a
+// row-major V, so K and V lie in LDS as in the cache, and come there directly
+// (global_load_lds, 16 bytes a lane, a wave 16 keys). A row's 16-byte pieces
+// are permuted by the row's number, K's so that 16 consecutive rows' same
+// piece, V's so that four consecutive rows' same four pieces lie on different
+// banks.
+//
+// Numerics. Scores, m, l and o are 32 bits; the running maximum moves only when
+// a score passes it by 2^kSlack, so most tiles rescale nothing. P is rounded
+// once to the inputs' type, as the output is: both errors are independent, and
+// together sqrt(2) of the output's own. In fp16, whose range is short, P is
+// scaled by 2^14: weights down to 2^-28 of a row's largest keep all 11 bits.
+
+#include "attn_device.h"
+#include "p16.h"
+
+namespace pa {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
+
+template <int D>
+struct WideOf {
+  static constexpr int kPerSimd = D == 256 ? 1 : 2;
+  static constexpr int kQ = D / 16;      // QK products per 32 keys
+  static constexpr int kO = D / 32;      // output tiles
+  static constexpr int kRow = 2 * D;     // bytes of a key row
+  static constexpr int kPieces = D / 8;  // 16-byte pieces of a row
+  static constexpr int kBuf = kP16WideKeys * kRow;
+  static constexpr int kLoads = 16 * kPieces / 64;  // loads of a wave per tile and stream
+  // The place of piece c of row t.
+  static __device__ __forceinline__ int k_piece(int t, int c) {
+    return c ^ (D == 64 ? (t >> 1) & 7 : t & 15);
+  }
+  static __device__ __forceinline__ int v_piece(int t, int c) {
+    return c ^ (D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2);
+  }
+};
+
+template <bool kF16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (kF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  else
+    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
+}
+
+// Column l % 16 of four rows of a row-major 16-bit matrix in LDS: lane i of
+// each 16 gives the address of row i / 4, columns 4 (i % 4).
+__device__ __forceinline__ u32x2 column4(const char* a) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (i16x4 __attribute__((address_space(3)))*)(
+                                           const_cast<char*>(a))));
+}
+
+template <int D, bool kF16, bool kPage16>
+__global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
+    const P16Params p) {
+  using W = WideOf<D>;
+  constexpr int kBM = kP16WideRows, kKT = kP16WideKeys;
+  constexpr float kSlack = kF16 ? 1.0f : 8.0f;
+  constexpr float kBias = kF16 ? 14.0f : 0.0f;
+  __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  // The work-groups of an XCD (every eighth) take neighbouring shares, so
+  // that the row tiles of one KV head read its keys from one L2.
+  const int per = p.num_wg >> 3;
+  const int wg = per * 8 == p.num_wg
+                     ? static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3)
+                     : static_cast<int>(blockIdx.x);
+  P16Cursor cur;
+  const int64_t tiles = p16_begin<kBM, kKT>(p, cur, lane);
+  const int takers = p16_takers(p, tiles);
+  if (wg >= takers) return;
+  int64_t at = p16_share(tiles, wg, takers);
+  const int64_t end = p16_share(tiles, wg + 1, takers);
+
+  while (at < end) {
+    const P16Unit u = p16_locate<kBM, kKT>(p, cur, at, lane);
+    const int take = static_cast<int>(min(static_cast<int64_t>(u.req.n_kt - u.kt), end - at));
+    const bool whole = take == u.req.n_kt;
+    const int slot = 2 * wg + (u.kt == 0 ? 1 : 0);
+    at += take;
+    const int rows = min(kBM, u.req.rows - u.rt * kBM);
+    const int row = 32 * wave + r32;
+    const bool live = row < rows;
+    int64_t token, head;
+    p16_row<kBM>(p, u, min(row, rows - 1), token, head);
+
+    u32x4 q[W::kQ];
+    {
+      const char* src = p.q + token * p.s_q_tok + head * p.s_q_head + 16 * h;
+#pragma unroll
+      for (int j = 0; j < W::kQ; ++j) {
+        q[j] = *reinterpret_cast<const u32x4*>(src + 32 * j);
+        if (!live) q[j] = (u32x4){0u, 0u, 0u, 0u};
+      }
+    }
+    float m = kNegInf, l = 0.0f;
+    f32x16 o[W::kO];
+#pragma unroll
+    for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
+
+    const int32_t* table = p.block_table + static_cast<int64_t>(u.r) * p.bt_stride;
+    const int len = u.req.len;
+    // The wave's 16 keys of tile t into buffer `buf`; keys past the last
+    // one repeat it.
+    auto load = [&](int t, int buf) {
+      int kb = kKT * t + 16 * wave;
+      kb = min(kb, (len - 1) & ~15);
+      const char *kb_base = nullptr, *vb_base = nullptr;
+      if constexpr (kPage16) {
+        const uint32_t pg = p.bs_div.div(static_cast<uint32_t>(kb));
+        int32_t id = ld_ro(table, pg);
+        id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
+        const int64_t first = kb - static_cast<int64_t>(pg) * p.bs_div.d;
+        kb_base = p.k.base + static_cast<int64_t>(id) * p.k.s_block + first * p.k.s_slot +
+                  static_cast<int64_t>(u.head) * p.k.s_head;
+        vb_base = p.v.base + static_cast<int64_t>(id) * p.v.s_block + first * p.v.s_slot +
+                  static_cast<int64_t>(u.head) * p.v.s_head;
+      }
+      char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
+      char* vd = kd + 2 * W::kBuf;
+#pragma unroll
+      for (int i = 0; i < W::kLoads; ++i) {
+        const int t16 = (64 * i + lane) / W::kPieces;  // row within the 16
+        const int c = (64 * i + lane) % W::kPieces;
+        const int from = min(t16, len - 1 - kb);
+        const char *ks, *vs;
+        if constexpr (kPage16) {
+          ks = kb_base + __umul24(static_cast<uint32_t>(from), static_cast<uint32_t>(p.k.s_slot));
+          vs = vb_base + __umul24(static_cast<uint32_t>(from), static_cast<uint32_t>(p.v.s_slot));
+        } else {
+          const uint32_t key = static_cast<uint32_t>(kb + from);
+          const uint32_t pg = p.bs_div.div(key);
+          int32_t id = table[pg];
+          id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
+          const int64_t in = static_cast<int64_t>(key - pg * p.bs_div.d);
+          ks = p.k.base + static_cast<int64_t>(id) * p.k.s_block + in * p.k.s_slot +
+               static_cast<int64_t>(u.head) * p.k.s_head;
+          vs = p.v.base + static_cast<int64_t>(id) * p.v.s_block + in * p.v.s_slot +
+               static_cast<int64_t>(u.head) * p.v.s_head;
+        }
+        dma16(ks + 16 * W::k_piece(t16, c), kd + 1024 * i);
+        dma16(vs + 16 * W::v_piece(t16, c), vd + 1024 * i);
+      }
+    };
+
+    const int t_end = len > 0 ? u.kt + take : u.kt;
+    int buf = 0;
+    // The last unit's reads of both buffers are done.
+    __syncthreads();
+    if (u.kt < t_end) load(u.kt, 0);
+    for (int t = u.kt; t < t_end; ++t, buf ^= 1) {
+      wait_vmcnt<0>();
+      __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
+      if (t + 1 < t_end) load(t + 1, buf ^ 1);
+      const char* kt = lds + buf * W::kBuf;
+      const char* vt = kt + 2 * W::kBuf;
+
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+        const char* krow = kt + (32 * b + r32) * W::kRow;
+#pragma unroll
+        for (int j = 0; j < W::kQ; ++j)
+          s[b] = mfma32<kF16>(
+              *reinterpret_cast<const u32x4*>(krow + 16 * W::k_piece(r32, 2 * j + h)), q[j], s[b]);
+      }
+      if (kKT * t + kKT > len) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = kKT * t + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+            s[b][i] = key < len ? s[b][i] : kNegInf;
+          }
+      }
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+      {
+        const SwapPair sw = swap_halves(top);
+        top = fmaxf(sw.a, sw.b) * p.scale_log2;
+      }
+      if (__ballot(top > m + kSlack || (m == kNegInf && top > m)) != 0) {
+        const float next = fmaxf(m, top);
+        const float ref = next == kNegInf ? 0.0f : next;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = next;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < W::kO; ++j) o[j] *= alpha;
+      }
+      const float shift = (m == kNegInf ? 0.0f : m) - kBias;
+      u32x4 pf[4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const float x0 = __builtin_amdgcn_exp2f(s[b][i] * p.scale_log2 - shift);
+          const float x1 = __builtin_amdgcn_exp2f(s[b][i + 1] * p.scale_log2 - shift);
+          l += x0 + x1;
+          pf[2 * b + (i >> 3)][(i & 7) >> 1] = pack16<kF16>(x0, x1);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < W::kO; ++j) {
+          // Rows 16 i + 4 h + 0..3 and 8 further on, columns 32 j + l % 32.
+          const int t0 = 4 * h + ((lane & 15) >> 2);
+          const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+          const char* a = vt + (16 * i + t0) * W::kRow + 16 * W::v_piece(t0, byte >> 4) + (byte & 15);
+          const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
+          o[j] = mfma32<kF16>((u32x4){x[0], x[1], y[0], y[1]}, pf[i], o[j]);
+        }
+      }
+    }
+
+    const SwapPair ls = swap_halves(l);
+    const float sum = ls.a + ls.b;
+    if (live && !whole) {
+      float* dst = p16_slot_o<kBM, D>(p, slot) + row * D + 4 * h;
+#pragma unroll
+      for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<f32x4*>(dst + 32 * j + 8 * b) =
+              (f32x4){o[j][4 * b], o[j][4 * b + 1], o[j][4 * b + 2], o[j][4 * b + 3]};
+      if (h == 0) {
+        float* ml = p16_slot_ml<kBM, D>(p, slot) + 2 * row;
+        ml[0] = m;
+        ml[1] = sum;
+      }
+    } else if (live) {
+      // A row without keys is 0; one whose scores are all -inf is 0 / 0, NaN.
+      const float inv = 1.0f / sum;
+      char* dst = p.out + token * p.s_out_tok + head * p.s_out_head + 8 * h;
+#pragma unroll
+      for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const u32x2 y = {pack16<kF16>(o[j][4 * b] * inv, o[j][4 * b + 1] * inv),
+                           pack16<kF16>(o[j][4 * b + 2] * inv, o[j][4 * b + 3] * inv)};
+          *reinterpret_cast<u32x2*>(dst + 64 * j + 16 * b) = len == 0 ? (u32x2){0u, 0u} : y;
+        }
+    }
+  }
+}
+
+template <int D>
+hipError_t wide_kernel(const P16Params& p, bool f16, bool page16, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.num_wg)), block(64 * kP16Waves);
+  if (f16 && page16) hipLaunchKernelGGL((p16_wide<D, true, true>), grid, block, 0, stream, p);
+  else if (f16) hipLaunchKernelGGL((p16_wide<D, true, false>), grid, block, 0, stream, p);
+  else if (page16) hipLaunchKernelGGL((p16_wide<D, false, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((p16_wide<D, false, false>), grid, block, 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_p16_wide_kernel(const P16Params& p, bool f16, bool page16, int head_size,
+                                  hipStream_t stream) {
+  note_kernel("p16_wide");
+  switch (head_size) {
+    case 64: return wide_kernel<64>(p, f16, page16, stream);
+    case 256: return wide_kernel<256>(p, f16, page16, stream);
+    default: return wide_kernel<128>(p, f16, page16, stream);
+  }
+}
+
+}  // namespace pa

@@ -128,6 +128,23 @@ def vllm_packed_views(
     return k, v, ks, vs
 
 
+def paged16_views(kv: torch.Tensor, *, layout: str = "NHD") -> tuple[torch.Tensor, torch.Tensor]:
+    """The (k_cache, v_cache) views ``[num_blocks, block_size, Hkv, D]`` of a
+    paged cache in a 16-bit type, for the ops of ``ops16``.
+
+    ``kv`` is ``[num_blocks, 2, block_size, Hkv, D]`` (layout NHD) or
+    ``[num_blocks, 2, Hkv, block_size, D]`` (HND), keys first; nothing is copied.
+    """
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}")
+    if kv.dim() != 5 or kv.shape[1] != 2 or kv.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("kv must be a bfloat16 or float16 tensor [num_blocks, 2, ., ., D]")
+    if kv.stride(4) != 1:
+        raise ValueError("kv must have stride 1 in its last dimension")
+    nhd = kv if layout == "NHD" else kv.transpose(2, 3)
+    return nhd[:, 0], nhd[:, 1]
+
+
 @dataclass
 class PagedCache:
     """A filled cache plus the per-request metadata the op needs."""

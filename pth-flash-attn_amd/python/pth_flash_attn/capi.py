@@ -40,6 +40,13 @@ EXPORTED_SYMBOLS = (
     "pth_attn_combine_kernel",
     "pth_attn_write_args_bytes",
     "pth_attn_write_kv",
+    "pth_attn_paged16",
+    "pth_attn_paged16_args_bytes",
+    "pth_attn_paged16_workspace_floats",
+    "pth_attn_write_kv16",
+    "pth_attn_write16_args_bytes",
+    "pth_attn_step_tables",
+    "pth_attn_tables_args_bytes",
 )
 
 
@@ -153,6 +160,86 @@ class PthAttnOptions(ctypes.Structure):
     ]
 
 
+class PthAttnP16Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("block_table_width", ctypes.c_int32),
+        ("max_kv_len", ctypes.c_int32),
+        ("kv_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("max_query_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("ws", ctypes.c_void_p),
+        ("ws_floats", ctypes.c_int64),
+    ]
+
+
+class PthAttnWrite16Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("kv_dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("slot_mapping", ctypes.c_void_p),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+    ]
+
+
+class PthAttnTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("block_table_width", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("slot_mapping", ctypes.c_void_p),
+        ("num_slots", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("pool_out", ctypes.c_void_p),
+        ("context_lens", ctypes.c_void_p),
+        ("query_lens", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("num_free", ctypes.c_int64),
+        ("pool_in", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class AttnLib:
     """The loaded libpth_attn.so with typed entry points."""
 
@@ -172,6 +259,9 @@ class AttnLib:
             "pth_attn_options_bytes",
             "pth_attn_has_cuda",
             "pth_attn_write_args_bytes",
+            "pth_attn_paged16_args_bytes",
+            "pth_attn_write16_args_bytes",
+            "pth_attn_tables_args_bytes",
         ):
             getattr(lib, name).restype = i32
             getattr(lib, name).argtypes = []
@@ -201,7 +291,26 @@ class AttnLib:
             ctypes.POINTER(PthAttnArgs), vp, ctypes.c_int64, ctypes.c_int64, vp]
         lib.pth_attn_write_kv.restype = i32
         lib.pth_attn_write_kv.argtypes = [ctypes.POINTER(PthAttnWriteArgs), vp]
+        for name, args in (("pth_attn_paged16", PthAttnP16Args),
+                           ("pth_attn_write_kv16", PthAttnWrite16Args),
+                           ("pth_attn_step_tables", PthAttnTablesArgs)):
+            getattr(lib, name).restype = i32
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), vp]
+        lib.pth_attn_paged16_workspace_floats.restype = ctypes.c_int64
+        lib.pth_attn_paged16_workspace_floats.argtypes = [i32]
         self.lib = lib
+
+    def paged16(self, args: PthAttnP16Args, stream: int | None = None) -> int:
+        """Attention over a paged 16-bit cache (see the header)."""
+        return self.lib.pth_attn_paged16(ctypes.byref(args), stream)
+
+    def write_kv16(self, args: PthAttnWrite16Args, stream: int | None = None) -> int:
+        """The 16-bit cache writer (see the header)."""
+        return self.lib.pth_attn_write_kv16(ctypes.byref(args), stream)
+
+    def step_tables(self, args: PthAttnTablesArgs, stream: int | None = None) -> int:
+        """A step's block tables and slot map (see the header)."""
+        return self.lib.pth_attn_step_tables(ctypes.byref(args), stream)
 
     def write_kv(self, args: PthAttnWriteArgs, stream: int | None = None) -> int:
         """The int8 cache writer (see include/pth_attn.h)."""
@@ -368,4 +477,69 @@ def write_args(*, key: Any, value: Any, k_cache: Any, v_cache: Any, k_scale: Any
     a.k_cache, a.v_cache = _stream(k_cache), _stream(v_cache)
     a.k_scale, a.v_scale = _stream(k_scale), _stream(v_scale)
     a.num_blocks, a.block_size = int(k_cache.shape[0]), int(k_cache.shape[1])
+    return a
+
+
+def paged16_args(*, q: Any, out: Any, k_cache: Any, v_cache: Any, block_table: Any, kv_lens: Any,
+                 max_kv_len: int, softmax_scale: float, ws: Any, query_start_loc: Any = None,
+                 max_query_len: int = 1, window: int = 0) -> PthAttnP16Args:
+    """PthAttnP16Args of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnP16Args()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(PthAttnP16Args)
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.q_stride_token, a.q_stride_head = _bstride(q, 0), _bstride(q, 1)
+    a.out_stride_token, a.out_stride_head = _bstride(out, 0), _bstride(out, 1)
+    a.dtype = _dtype_code(q.dtype)
+    a.num_blocks, a.block_size, a.num_kv_heads, a.head_size = (int(x) for x in k_cache.shape)
+    a.k_cache, a.v_cache = _stream(k_cache), _stream(v_cache)
+    a.block_table = block_table.data_ptr()
+    a.block_table_row_stride = int(block_table.stride(0))
+    a.block_table_width = int(block_table.shape[1])
+    a.max_kv_len = max_kv_len
+    a.kv_lens = kv_lens.data_ptr()
+    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
+    a.num_reqs = int(kv_lens.shape[0])
+    a.num_tokens, a.num_q_heads = int(q.shape[0]), int(q.shape[1])
+    a.max_query_len = max_query_len
+    a.window = window
+    a.softmax_scale = softmax_scale
+    a.ws, a.ws_floats = ws.data_ptr(), int(ws.numel())
+    return a
+
+
+def write16_args(*, key: Any, value: Any, k_cache: Any, v_cache: Any,
+                 slot_mapping: Any) -> PthAttnWrite16Args:
+    """PthAttnWrite16Args of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnWrite16Args()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(PthAttnWrite16Args)
+    a.key, a.value = key.data_ptr(), value.data_ptr()
+    a.key_stride_token, a.key_stride_head = _bstride(key, 0), _bstride(key, 1)
+    a.value_stride_token, a.value_stride_head = _bstride(value, 0), _bstride(value, 1)
+    a.kv_dtype, a.cache_dtype = _dtype_code(key.dtype), _dtype_code(k_cache.dtype)
+    a.num_tokens, a.num_kv_heads, a.head_size = (int(x) for x in key.shape)
+    a.num_blocks, a.block_size = int(k_cache.shape[0]), int(k_cache.shape[1])
+    a.slot_mapping = slot_mapping.data_ptr()
+    a.k_cache, a.v_cache = _stream(k_cache), _stream(v_cache)
+    return a
+
+
+def tables_args(*, block_table: Any, slot_mapping: Any, seq_lens: Any, query_start_loc: Any,
+                pool_out: Any, context_lens: Any, query_lens: Any, free_pages: Any, pool_in: Any,
+                block_size: int) -> PthAttnTablesArgs:
+    """PthAttnTablesArgs of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnTablesArgs()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(PthAttnTablesArgs)
+    a.block_table = block_table.data_ptr()
+    a.block_table_row_stride = int(block_table.stride(0))
+    a.block_table_width = int(block_table.shape[1])
+    a.block_size = block_size
+    a.slot_mapping, a.num_slots = slot_mapping.data_ptr(), int(slot_mapping.numel())
+    a.seq_lens, a.query_start_loc = seq_lens.data_ptr(), query_start_loc.data_ptr()
+    a.pool_out, a.pool_in = pool_out.data_ptr(), pool_in.data_ptr()
+    a.context_lens, a.query_lens = context_lens.data_ptr(), query_lens.data_ptr()
+    a.free_pages, a.num_free = free_pages.data_ptr(), int(free_pages.numel())
+    a.num_reqs = int(context_lens.shape[0])
     return a

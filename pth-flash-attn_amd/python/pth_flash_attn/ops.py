@@ -21,6 +21,13 @@ from pathlib import Path
 
 import torch
 
+from pth_flash_attn import ops16
+from pth_flash_attn.ops16 import (  # noqa: F401  (the ops of a 16-bit cache)
+    build_step_tables,
+    cross_attn_fwd,
+    paged_decode_fwd,
+    reshape_and_cache_16bit,
+)
 from pth_flash_attn.planner import (
     MAX_ROWS_PER_CTA,
     MMA_ROWS_PER_WARP,
@@ -277,6 +284,8 @@ def _load_library() -> bool:
     torch.ops.load_library(str(LIBRARY_PATH))
     torch.library.register_fake(OP_QUALNAME)(pth_flash_attn_fwd_fake)
     torch.library.register_fake(WRITER_QUALNAME)(reshape_and_cache_int8_fake)
+    for name, fake in ops16.FAKES.items():
+        torch.library.register_fake(f"{OP_NAMESPACE}::{name}")(fake)
     return True
 
 

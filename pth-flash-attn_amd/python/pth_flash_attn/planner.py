@@ -294,3 +294,15 @@ def workspace_bytes(*, ws_token_splits: int, Hq: int, D: int) -> int:
     """W_ts * Hq * (D + 1) * 4: bytes of both fp32 partial buffers."""
     (w_ts, hq, d), _ = workspace_shapes(ws_token_splits=ws_token_splits, Hq=Hq, D=D)
     return w_ts * hq * (d + 1) * PARTIAL_BYTES_PER_ELEMENT
+
+
+# Rows of partial sums per compute unit that the 16-bit cache's kernels can have
+# in flight (two slots of each resident work-group).
+PAGED16_ROWS_PER_CU = 512
+
+
+def paged16_workspace_floats(*, D: int, num_sms: int) -> int:
+    """fp32 elements of the workspace of ``paged_decode_fwd`` / ``cross_attn_fwd``:
+    512 rows of D sums, a maximum and a sum per compute unit, whatever the
+    batch, its heads and its lengths (no counterpart in the reference)."""
+    return _host_int("num_sms", num_sms, 1) * PAGED16_ROWS_PER_CU * (_head_size(D) + 2)
