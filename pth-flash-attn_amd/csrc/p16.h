@@ -5,15 +5,19 @@
 //
 // The work of a launch is a stream of key tiles. A unit is a row tile (kRows
 // consecutive rows, a row being a (query token, query head of the KV head)
-// pair) of one request and one KV head; it has ceil(keys / kKeys) tiles, one
-// if it sees no key. Units lie end to end, requests first, then KV heads,
-// then row tiles. Work-group w of W takes tiles [w N / W, (w + 1) N / W) of
-// the N (W at most N, so that none between two of a unit's is without tiles):
-// equal shares whatever the lengths, and at most two units of a work-group are
-// cut, its first and its last. A cut unit leaves unnormalised
-// partial sums in the workspace, two slots per work-group whatever the batch:
-// slot 2 w for a range that begins inside a unit, 2 w + 1 for one that begins
-// with it. The combine's work-group w joins the unit whose beginning w holds.
+// pair) of one request and one KV head; units lie requests first, then KV
+// heads, then row tiles. A group is `team` consecutive units of a request that
+// a work-group computes side by side; it has ceil(keys / key_tile) tiles, one
+// if it sees no key. Groups lie end to end, and work-group w of W takes tiles
+// [w N / W, (w + 1) N / W) of the N (W at most N, so that none between two of a
+// group's is without tiles): equal shares whatever the lengths, and at most
+// two groups of a work-group are cut, its first and its last. A cut group
+// leaves unnormalised partial sums in the workspace, two slots per work-group
+// whatever the batch: slot 2 w for a range that begins inside a group, 2 w + 1
+// for one that begins with it. The work-group that holds a group's beginning
+// notes how it was cut (P16Cut), for the combine, which joins it: the note's
+// place is the group's number where that is known (one query token per request)
+// and there are few, the work-group's otherwise.
 //
 // Everything is a function of the device's lengths and of launch constants,
 // so a captured graph replays as the lengths change.
@@ -45,19 +49,34 @@ struct P16Params {
   int32_t group;
   int32_t window;
   int32_t num_wg;
-  float scale_log2;  // softmax_scale * log2(e)
+  int32_t team;           // units of a group: 1, 2 or 4
+  int32_t key_tile_log2;  // keys of a tile
+  int32_t slot_rows;      // rows of a unit that a slot holds: no unit has more
+  int32_t notes;          // notes by group number: how many; 0: by work-group
+  float scale_log2;       // softmax_scale * log2(e)
 };
 
-// Key tile and row tile of the two kernels.
+// Row tiles of the two kernels, and the wide one's key tile (the other's is 32
+// for each wave of a unit).
 constexpr int kP16Waves = 4;
-constexpr int kP16RowsRows = 16, kP16RowsKeys = 32 * kP16Waves;
+constexpr int kP16RowsRows = 16;
 constexpr int kP16WideRows = 32 * kP16Waves, kP16WideKeys = 64;
 
-// Floats of workspace per compute unit: the most that a kernel's resident
-// work-groups need, two slots of kRows * (D + 2) each.
-constexpr int kP16WsRowsPerCu = 512;
+// A cut group: the slots that hold it (0: none is cut) and, above kP16CutShift,
+// the work-group that begins it; its request's first query token and rows, its
+// place among the request's groups.
+struct P16Cut {
+  uint32_t slots_wg;
+  int32_t q0, rows, group;
+};
+constexpr int kP16CutShift = 16;
+
+// Workspace: rows of D sums with a maximum and a sum each, as many as the
+// work-groups of a compute unit (at most kP16WgPerCu) have in their slots, and
+// a P16Cut for each work-group.
+constexpr int kP16WsRowsPerCu = 512, kP16WgPerCu = 8;
 inline int64_t p16_workspace_floats(int32_t head_size, int32_t cus) {
-  return static_cast<int64_t>(cus) * kP16WsRowsPerCu * (head_size + 2);
+  return static_cast<int64_t>(cus) * (kP16WsRowsPerCu * (head_size + 2) + 4 * kP16WgPerCu);
 }
 
 #if defined(__HIPCC__)
@@ -72,10 +91,11 @@ struct P16Req {
   int32_t base;  // lo rounded down to a 16-key block
   int32_t len;   // one past the last
   int32_t n_rt;  // row tiles
+  int32_t n_gr;  // groups of units
   int32_t n_kt;  // key tiles, >= 1
 };
 
-template <int kRows, int kKeys>
+template <int kRows>
 __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int q0, int q1,
                                                  int len) {
   P16Req x;
@@ -89,17 +109,13 @@ __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int 
   x.lo = p.window > 0 ? max(x.len - p.window, 0) : 0;
   x.base = x.lo & ~15;
   x.n_rt = (x.rows + kRows - 1) / kRows;
-  x.n_kt = max((x.len - x.base + kKeys - 1) / kKeys, 1);
+  x.n_gr = (p.num_kv_heads * x.n_rt + p.team - 1) >> (p.team >> 1);  // / team
+  x.n_kt = max((x.len - x.base + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
   return x;
 }
 
-template <int kRows, int kKeys>
-__device__ __forceinline__ int64_t p16_tiles(const P16Params& p, const P16Req& x) {
-  return static_cast<int64_t>(p.num_kv_heads) * x.n_rt * x.n_kt;
-}
-
 // Tiles of request `r` by vector loads (r differs from lane to lane).
-template <int kRows, int kKeys>
+template <int kRows>
 __device__ __forceinline__ int64_t p16_lane_tiles(const P16Params& p, int r) {
   if (r >= p.num_reqs) return 0;
   int len = p.kv_lens[r], q0 = 0, q1 = 0;
@@ -107,7 +123,8 @@ __device__ __forceinline__ int64_t p16_lane_tiles(const P16Params& p, int r) {
     q0 = p.qsl[r];
     q1 = p.qsl[r + 1];
   }
-  return p16_tiles<kRows, kKeys>(p, p16_request_of<kRows, kKeys>(p, r, q0, q1, len));
+  const P16Req x = p16_request_of<kRows>(p, r, q0, q1, len);
+  return static_cast<int64_t>(x.n_gr) * x.n_kt;
 }
 
 // Forward-only walk over the requests, 64 at a time (every lane the same but
@@ -119,56 +136,51 @@ struct P16Cursor {
 };
 
 // All tiles of the launch; the cursor at its first 64 requests.
-template <int kRows, int kKeys>
+template <int kRows>
 __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, int lane) {
   c.r0 = 0;
   c.base = 0;
-  c.incl = wave_scan64(p16_lane_tiles<kRows, kKeys>(p, lane), lane);
+  c.incl = wave_scan64(p16_lane_tiles<kRows>(p, lane), lane);
   c.end = readlane64(c.incl, 63);
-  int64_t more = 0;
-  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) more += p16_lane_tiles<kRows, kKeys>(p, r0 + lane);
   if (p.num_reqs <= 64) return c.end;
+  int64_t more = 0;
+  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) more += p16_lane_tiles<kRows>(p, r0 + lane);
   return c.end + readlane64(wave_scan64(more, lane), 63);
 }
 
-// A unit, and the tile of it that a position falls on.
-struct P16Unit {
+// A group, and the tile of it that a position falls on.
+struct P16Group {
   P16Req req;
-  int32_t r, head, rt, kt;
+  int32_t r, group, kt;
 };
 
-// The unit of tile `at` (not before the cursor, and less than all tiles).
-template <int kRows, int kKeys>
-__device__ __forceinline__ P16Unit p16_locate(const P16Params& p, P16Cursor& c, int64_t at,
-                                              int lane) {
+// The group of tile `at` (not before the cursor, and less than all tiles).
+template <int kRows>
+__device__ __forceinline__ P16Group p16_locate(const P16Params& p, P16Cursor& c, int64_t at,
+                                               int lane) {
   while (at >= c.end && c.r0 + 64 < p.num_reqs) {
     c.r0 += 64;
     c.base = c.end;
-    c.incl = wave_scan64(p16_lane_tiles<kRows, kKeys>(p, c.r0 + lane), lane);
+    c.incl = wave_scan64(p16_lane_tiles<kRows>(p, c.r0 + lane), lane);
     c.end = c.base + readlane64(c.incl, 63);
   }
   const int64_t local = at - c.base;
   const int j = min(static_cast<int>(__popcll(__ballot(c.incl <= local))), 63);
   const int64_t before = j > 0 ? readlane64(c.incl, j - 1) : 0;
-  P16Unit u;
+  P16Group u;
   u.r = __builtin_amdgcn_readfirstlane(min(c.r0 + j, p.num_reqs - 1));
   int len = ld_ro(p.kv_lens, u.r), q0 = 0, q1 = 0;
   if (p.qsl != nullptr) {
     q0 = ld_ro(p.qsl, u.r);
     q1 = ld_ro(p.qsl, u.r + 1);
   }
-  u.req = p16_request_of<kRows, kKeys>(p, u.r, q0, q1, len);
+  u.req = p16_request_of<kRows>(p, u.r, q0, q1, len);
   // Within a request: less than 2^31 tiles, by the launcher's check.
   const uint32_t in_req = static_cast<uint32_t>(local - before);
-  const uint32_t unit = in_req / static_cast<uint32_t>(u.req.n_kt);
-  u.kt = static_cast<int32_t>(in_req - unit * static_cast<uint32_t>(u.req.n_kt));
-  const uint32_t n_rt = static_cast<uint32_t>(max(u.req.n_rt, 1));
-  u.head = static_cast<int32_t>(unit / n_rt);
-  u.rt = static_cast<int32_t>(unit - static_cast<uint32_t>(u.head) * n_rt);
-  u.r = __builtin_amdgcn_readfirstlane(u.r);
-  u.head = __builtin_amdgcn_readfirstlane(u.head);
-  u.rt = __builtin_amdgcn_readfirstlane(u.rt);
-  u.kt = __builtin_amdgcn_readfirstlane(u.kt);
+  const uint32_t n_kt = static_cast<uint32_t>(u.req.n_kt);
+  u.group = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(in_req / n_kt));
+  u.kt = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(in_req)) -
+         u.group * static_cast<int32_t>(n_kt);
   return u;
 }
 
@@ -178,30 +190,68 @@ __device__ __forceinline__ int p16_takers(const P16Params& p, int64_t tiles) {
 }
 // The first tile of work-group w (w at most num_wg, num_wg > 0).
 __device__ __forceinline__ int64_t p16_share(int64_t tiles, int w, int num_wg) {
-  return tiles * w / num_wg;
+  const uint64_t x = static_cast<uint64_t>(tiles) * static_cast<uint32_t>(w);
+  if (x >> 32 == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(num_wg);
+  return static_cast<int64_t>(x / static_cast<uint32_t>(num_wg));
 }
 // The work-group that holds tile `at`.
 __device__ __forceinline__ int p16_holder(int64_t tiles, int64_t at, int num_wg) {
-  return static_cast<int>(((at + 1) * num_wg + tiles - 1) / tiles) - 1;
+  const uint64_t x = static_cast<uint64_t>(at + 1) * static_cast<uint32_t>(num_wg) +
+                     static_cast<uint64_t>(tiles) - 1;
+  if (x >> 32 == 0) return static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(tiles)) - 1;
+  return static_cast<int>(x / static_cast<uint64_t>(tiles)) - 1;
 }
 
-// Slot `i`'s partial sums and its (maximum, sum) pairs.
-template <int kRows, int D>
-__device__ __forceinline__ float* p16_slot_o(const P16Params& p, int i) {
-  return p.ws + static_cast<int64_t>(i) * kRows * D;
-}
-template <int kRows, int D>
-__device__ __forceinline__ float* p16_slot_ml(const P16Params& p, int i) {
-  return p.ws + static_cast<int64_t>(2) * p.num_wg * kRows * D + static_cast<int64_t>(i) * kRows * 2;
+// A unit: KV head and row tile.
+struct P16Unit {
+  int32_t head, rt;
+};
+__device__ __forceinline__ P16Unit p16_unit(const P16Req& x, int32_t index) {
+  const uint32_t n = static_cast<uint32_t>(max(x.n_rt, 1));
+  P16Unit u;
+  u.head = n == 1 ? index : static_cast<int32_t>(static_cast<uint32_t>(index) / n);
+  u.rt = n == 1 ? 0 : index - u.head * static_cast<int32_t>(n);
+  return u;
 }
 
-// The address of row `row` (within its unit's row tile): query token and head.
+// Row `row` of a slot's unit `sub`: D sums, and their maximum and weight sum.
+// A slot holds slot_rows rows of each unit: one long request's many slots are
+// read together, and lie as close as they can.
+template <int D>
+__device__ __forceinline__ float* p16_slot_o(const P16Params& p, int slot, int sub, int row) {
+  return p.ws + (static_cast<int64_t>(slot * p.team + sub) * p.slot_rows + row) * D;
+}
+template <int D>
+__device__ __forceinline__ float* p16_slot_ml(const P16Params& p, int slot, int sub, int row) {
+  const int64_t rows = static_cast<int64_t>(2) * p.num_wg * p.team * p.slot_rows;
+  return p.ws + rows * D + (static_cast<int64_t>(slot * p.team + sub) * p.slot_rows + row) * 2;
+}
+template <int D>
+__device__ __forceinline__ P16Cut* p16_cut(const P16Params& p, int i) {
+  return reinterpret_cast<P16Cut*>(p16_slot_ml<D>(p, 2 * p.num_wg, 0, 0)) + i;
+}
+// Notes that work-group wg begins the group `gr`, cut or (`cut` false) whole.
+template <int D>
+__device__ __forceinline__ void p16_note(const P16Params& p, const P16Group& gr, int wg,
+                                         int64_t tiles, int64_t first, int takers, bool cut) {
+  P16Cut c = {0u, gr.req.q0, gr.req.rows, gr.group};
+  if (cut)
+    c.slots_wg = static_cast<uint32_t>(p16_holder(tiles, first + gr.req.n_kt - 1, takers) - wg + 1) |
+                 static_cast<uint32_t>(wg) << kP16CutShift;
+  *p16_cut<D>(p, p.notes ? gr.r * gr.req.n_gr + gr.group : wg) = c;
+}
+template <int D>
+__device__ __forceinline__ void p16_note_none(const P16Params& p, int wg) {
+  if (!p.notes) p16_cut<D>(p, wg)->slots_wg = 0u;
+}
+
+// Query token and head of row `row` of a unit.
 template <int kRows>
-__device__ __forceinline__ void p16_row(const P16Params& p, const P16Unit& u, int row,
+__device__ __forceinline__ void p16_row(const P16Params& p, int32_t q0, const P16Unit& u, int row,
                                         int64_t& token, int64_t& head) {
   const uint32_t i = static_cast<uint32_t>(u.rt * kRows + row);
   const uint32_t t = p.g_div.div(i);
-  token = u.req.q0 + static_cast<int64_t>(t);
+  token = q0 + static_cast<int64_t>(t);
   head = static_cast<int64_t>(u.head) * p.group + (i - t * static_cast<uint32_t>(p.group));
 }
 
@@ -214,7 +264,7 @@ hipError_t launch_p16_rows_kernel(const P16Params& p, bool f16, bool page16, int
 hipError_t launch_p16_wide_kernel(const P16Params& p, bool f16, bool page16, int head_size,
                                   hipStream_t stream);
 hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
-                                     hipStream_t stream);
+                                     int y, hipStream_t stream);
 int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream);
 int32_t launch_step_tables(const PthAttnTablesArgs& a, hipStream_t stream);
 

@@ -13,6 +13,9 @@
 namespace pa {
 namespace {
 
+// Slots per group up to which the combine is cheap.
+constexpr int64_t kMostSlots = 128;
+
 bool rows_aligned(const void* p, int64_t a, int64_t b) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
 }
@@ -24,6 +27,27 @@ bool stream_ok(const PthAttnStream& s) {
 CacheStream stream_of(const PthAttnStream& s) {
   return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
                      s.stride_head};
+}
+
+// Units that a work-group of the 16-row kernel computes side by side, one for
+// each wave or pair of waves: neighbours in the cache (the KV heads of NHD
+// pages), or row tiles of the same keys, as long as enough groups remain.
+int32_t team_of(const P16Params& p, int32_t cus) {
+  const int64_t n_rt = p.qsl ? 1 : (p.group + kP16RowsRows - 1) / kP16RowsRows;
+  const bool heads_adjacent = p.k.s_head < p.k.s_slot && p.v.s_head < p.v.s_slot;
+  const int64_t beside = heads_adjacent ? p.num_kv_heads * n_rt : n_rt;
+  int32_t team = beside % 4 == 0 ? 4 : beside % 2 == 0 ? 2 : 1;
+  while (team > 1 && p.num_reqs * p.num_kv_heads * n_rt / team * kMostSlots < cus) team /= 2;
+  return team;
+}
+
+// Work-groups per compute unit of the 16-row kernel. One, four waves, reads
+// the cache fastest (more streams at once cost the memory more than they
+// hide); where a work-group takes several groups, others fill the gaps between
+// them, as many as fit.
+int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
+  const int64_t fit = head_size == 64 ? 3 : head_size == 128 ? 2 : 1;
+  return std::min(fit, std::max<int64_t>(1, groups / cus));
 }
 
 }  // namespace
@@ -101,28 +125,36 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
 
   const bool wide = a.query_start_loc != nullptr &&
                     static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
-  const int64_t bm = wide ? kP16WideRows : kP16RowsRows, kt = wide ? kP16WideKeys : kP16RowsKeys;
+  const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
   PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
-  // Bounds of the partition: row tiles of all requests, key tiles of one.
+  p.team = wide ? 1 : team_of(p, cus);
+  p.key_tile_log2 = wide ? 6 : 7 - (p.team >> 1);
+  p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
+  // Bounds of the partition: groups of all requests, key tiles of one.
   const int64_t row_tiles = a.query_start_loc == nullptr
                                 ? a.num_reqs * ((p.group + bm - 1) / bm)
                                 : rows / bm + a.num_reqs;
   const int64_t span = p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + 15)
                                     : p.max_keys;
-  const int64_t key_tiles = std::max<int64_t>((span + kt - 1) / kt, 1);
+  const int64_t key_tiles = std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
+  const int64_t groups_exact = a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team);
+  const int64_t groups = a.query_start_loc == nullptr
+                             ? groups_exact
+                             : (row_tiles * a.num_kv_heads + p.team - 1) / p.team + (p.team > 1 ? a.num_reqs : 0);
   PA_REQUIRE(row_tiles * a.num_kv_heads < INT32_MAX / key_tiles,
              "the launch exceeds 2^31 tiles");
-  const int64_t tiles = row_tiles * a.num_kv_heads * key_tiles;
-  const int64_t fill = static_cast<int64_t>(cus) * (wide ? (a.head_size == 256 ? 1 : 2)
-                                                         : (a.head_size == 64 ? 4 : a.head_size == 128 ? 3 : 1));
-  p.num_wg = static_cast<int32_t>(std::min(tiles, fill));
+  const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : 2) : rows_per_cu(a.head_size, groups, cus));
+  p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
+  if (a.query_start_loc == nullptr && groups_exact <= p.num_wg) p.notes = static_cast<int32_t>(groups_exact);
   const bool f16 = a.dtype == PTH_ATTN_F16, page16 = a.block_size % 16 == 0;
   hipError_t err = wide ? launch_p16_wide_kernel(p, f16, page16, a.head_size, stream)
                         : launch_p16_rows_kernel(p, f16, page16, a.head_size, stream);
-  // A unit of one tile is never cut.
+  const int32_t items = p.team * p.slot_rows;
+  const int32_t y = wide ? 4 : p.notes ? std::min(items, std::max(1, 2 * cus / p.notes)) : 1;
+  // A group of one tile is never cut.
   if (err == hipSuccess && key_tiles > 1)
-    err = launch_p16_combine_kernel(p, f16, wide, a.head_size, stream);
+    err = launch_p16_combine_kernel(p, f16, wide, a.head_size, y, stream);
   if (err != hipSuccess)
     return fail(PTH_ATTN_ECUDA, std::string("paged16 launch: ") + hipGetErrorString(err));
   return PTH_ATTN_OK;

@@ -93,23 +93,32 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
                      ? static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3)
                      : static_cast<int>(blockIdx.x);
   P16Cursor cur;
-  const int64_t tiles = p16_begin<kBM, kKT>(p, cur, lane);
+  const int64_t tiles = p16_begin<kBM>(p, cur, lane);
   const int takers = p16_takers(p, tiles);
-  if (wg >= takers) return;
+  if (wg >= takers) {
+    if (threadIdx.x == 0) p16_note_none<D>(p, wg);
+    return;
+  }
   int64_t at = p16_share(tiles, wg, takers);
   const int64_t end = p16_share(tiles, wg + 1, takers);
+  bool noted = false;
 
   while (at < end) {
-    const P16Unit u = p16_locate<kBM, kKT>(p, cur, at, lane);
-    const int take = static_cast<int>(min(static_cast<int64_t>(u.req.n_kt - u.kt), end - at));
-    const bool whole = take == u.req.n_kt;
-    const int slot = 2 * wg + (u.kt == 0 ? 1 : 0);
+    const P16Group gr = p16_locate<kBM>(p, cur, at, lane);
+    const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
+    const bool whole = take == gr.req.n_kt;
+    const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
+    if (gr.kt == 0 && (!whole || p.notes)) {
+      noted |= !whole;
+      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
+    }
     at += take;
-    const int rows = min(kBM, u.req.rows - u.rt * kBM);
+    const P16Unit u = p16_unit(gr.req, gr.group);
+    const int rows = min(kBM, gr.req.rows - u.rt * kBM);
     const int row = 32 * wave + r32;
     const bool live = row < rows;
     int64_t token, head;
-    p16_row<kBM>(p, u, min(row, rows - 1), token, head);
+    p16_row<kBM>(p, gr.req.q0, u, min(row, rows - 1), token, head);
 
     u32x4 q[W::kQ];
     {
@@ -127,8 +136,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
 
-    const int32_t* table = p.block_table + static_cast<int64_t>(u.r) * p.bt_stride;
-    const int len = u.req.len;
+    const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
+    const int len = gr.req.len;
     // The wave's 16 keys of tile t into buffer `buf`; keys past the last
     // one repeat it.
     auto load = [&](int t, int buf) {
@@ -172,12 +181,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       }
     };
 
-    const int t_end = len > 0 ? u.kt + take : u.kt;
+    const int t_end = len > 0 ? gr.kt + take : gr.kt;
     int buf = 0;
     // The last unit's reads of both buffers are done.
     __syncthreads();
-    if (u.kt < t_end) load(u.kt, 0);
-    for (int t = u.kt; t < t_end; ++t, buf ^= 1) {
+    if (gr.kt < t_end) load(gr.kt, 0);
+    for (int t = gr.kt; t < t_end; ++t, buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
       if (t + 1 < t_end) load(t + 1, buf ^ 1);
@@ -248,18 +257,14 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     const SwapPair ls = swap_halves(l);
     const float sum = ls.a + ls.b;
     if (live && !whole) {
-      float* dst = p16_slot_o<kBM, D>(p, slot) + row * D + 4 * h;
+      float* dst = p16_slot_o<D>(p, slot, 0, row) + 4 * h;
 #pragma unroll
       for (int j = 0; j < W::kO; ++j)
 #pragma unroll
         for (int b = 0; b < 4; ++b)
           *reinterpret_cast<f32x4*>(dst + 32 * j + 8 * b) =
               (f32x4){o[j][4 * b], o[j][4 * b + 1], o[j][4 * b + 2], o[j][4 * b + 3]};
-      if (h == 0) {
-        float* ml = p16_slot_ml<kBM, D>(p, slot) + 2 * row;
-        ml[0] = m;
-        ml[1] = sum;
-      }
+      if (h == 0) *reinterpret_cast<f32x2*>(p16_slot_ml<D>(p, slot, 0, row)) = (f32x2){m, sum};
     } else if (live) {
       // A row without keys is 0; one whose scores are all -inf is 0 / 0, NaN.
       const float inv = 1.0f / sum;
@@ -274,6 +279,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
         }
     }
   }
+  if (!noted && threadIdx.x == 0) p16_note_none<D>(p, wg);
 }
 
 template <int D>

@@ -44,7 +44,7 @@ def test_sizes():
 
 
 def test_workspace_size():
-    assert planner.paged16_workspace_floats(D=128, num_sms=256) == 256 * 512 * 130
+    assert planner.paged16_workspace_floats(D=128, num_sms=256) == 256 * (512 * 130 + 32)
     with pytest.raises(ValueError, match="D must be one of"):
         planner.paged16_workspace_floats(D=96, num_sms=256)
     with pytest.raises(TypeError, match="num_sms must be a host int"):
