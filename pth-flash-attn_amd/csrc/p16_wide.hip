@@ -66,6 +66,18 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
 }
 
+// sum + the two values of a pair.
+template <bool kF16>
+__device__ __forceinline__ float add_pair(uint32_t w, float sum) {
+  if constexpr (kF16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w),
+                                  (f16x2){static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)},
+                                  sum, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
+                                           __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+}
+
 // Column l % 16 of four rows of a row-major 16-bit matrix in LDS: lane i of
 // each 16 gives the address of row i / 4, columns 4 (i % 4).
 __device__ __forceinline__ u32x2 column4(const char* a) {
@@ -138,46 +150,63 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
 
     const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
     const int len = gr.req.len;
+    // The lane's bytes within 16 keys, for each load.
+    uint32_t k_off[W::kLoads], v_off[W::kLoads];
+#pragma unroll
+    for (int i = 0; i < W::kLoads; ++i) {
+      const int t16 = (64 * i + lane) / W::kPieces, c = (64 * i + lane) % W::kPieces;
+      k_off[i] = __umul24(t16, static_cast<uint32_t>(p.k.s_slot)) + 16 * W::k_piece(t16, c);
+      v_off[i] = __umul24(t16, static_cast<uint32_t>(p.v.s_slot)) + 16 * W::v_piece(t16, c);
+    }
     // The wave's 16 keys of tile t into buffer `buf`; keys past the last
     // one repeat it.
     auto load = [&](int t, int buf) {
       int kb = kKT * t + 16 * wave;
       kb = min(kb, (len - 1) & ~15);
-      const char *kb_base = nullptr, *vb_base = nullptr;
-      if constexpr (kPage16) {
-        const uint32_t pg = p.bs_div.div(static_cast<uint32_t>(kb));
-        int32_t id = ld_ro(table, pg);
-        id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
-        const int64_t first = kb - static_cast<int64_t>(pg) * p.bs_div.d;
-        kb_base = p.k.base + static_cast<int64_t>(id) * p.k.s_block + first * p.k.s_slot +
-                  static_cast<int64_t>(u.head) * p.k.s_head;
-        vb_base = p.v.base + static_cast<int64_t>(id) * p.v.s_block + first * p.v.s_slot +
-                  static_cast<int64_t>(u.head) * p.v.s_head;
-      }
       char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
       char* vd = kd + 2 * W::kBuf;
+      if constexpr (kPage16) {
+        const uint32_t pg = mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
+        int32_t id = ld_ro(table, pg);
+        id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
+        const int64_t first = kb - static_cast<int32_t>(pg * p.bs_div.d);
+        const char* ks = p.k.base + static_cast<int64_t>(id) * p.k.s_block + first * p.k.s_slot +
+                         static_cast<int64_t>(u.head) * p.k.s_head;
+        const char* vs = p.v.base + static_cast<int64_t>(id) * p.v.s_block + first * p.v.s_slot +
+                         static_cast<int64_t>(u.head) * p.v.s_head;
+        if (kb + 16 <= len) {
 #pragma unroll
-      for (int i = 0; i < W::kLoads; ++i) {
-        const int t16 = (64 * i + lane) / W::kPieces;  // row within the 16
-        const int c = (64 * i + lane) % W::kPieces;
-        const int from = min(t16, len - 1 - kb);
-        const char *ks, *vs;
-        if constexpr (kPage16) {
-          ks = kb_base + __umul24(static_cast<uint32_t>(from), static_cast<uint32_t>(p.k.s_slot));
-          vs = vb_base + __umul24(static_cast<uint32_t>(from), static_cast<uint32_t>(p.v.s_slot));
+          for (int i = 0; i < W::kLoads; ++i) {
+            dma16(ks + k_off[i], kd + 1024 * i);
+            dma16(vs + v_off[i], vd + 1024 * i);
+          }
         } else {
-          const uint32_t key = static_cast<uint32_t>(kb + from);
+#pragma unroll
+          for (int i = 0; i < W::kLoads; ++i) {
+            const int t16 = (64 * i + lane) / W::kPieces, c = (64 * i + lane) % W::kPieces;
+            const uint32_t from = min(t16, len - 1 - kb);
+            dma16(ks + (__umul24(from, static_cast<uint32_t>(p.k.s_slot)) + 16 * W::k_piece(t16, c)),
+                  kd + 1024 * i);
+            dma16(vs + (__umul24(from, static_cast<uint32_t>(p.v.s_slot)) + 16 * W::v_piece(t16, c)),
+                  vd + 1024 * i);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W::kLoads; ++i) {
+          const int t16 = (64 * i + lane) / W::kPieces, c = (64 * i + lane) % W::kPieces;
+          const uint32_t key = static_cast<uint32_t>(kb + min(t16, len - 1 - kb));
           const uint32_t pg = p.bs_div.div(key);
           int32_t id = table[pg];
           id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
           const int64_t in = static_cast<int64_t>(key - pg * p.bs_div.d);
-          ks = p.k.base + static_cast<int64_t>(id) * p.k.s_block + in * p.k.s_slot +
-               static_cast<int64_t>(u.head) * p.k.s_head;
-          vs = p.v.base + static_cast<int64_t>(id) * p.v.s_block + in * p.v.s_slot +
-               static_cast<int64_t>(u.head) * p.v.s_head;
+          const char* ks = p.k.base + static_cast<int64_t>(id) * p.k.s_block + in * p.k.s_slot +
+                           static_cast<int64_t>(u.head) * p.k.s_head;
+          const char* vs = p.v.base + static_cast<int64_t>(id) * p.v.s_block + in * p.v.s_slot +
+                           static_cast<int64_t>(u.head) * p.v.s_head;
+          dma16(ks + 16 * W::k_piece(t16, c), kd + 1024 * i);
+          dma16(vs + 16 * W::v_piece(t16, c), vd + 1024 * i);
         }
-        dma16(ks + 16 * W::k_piece(t16, c), kd + 1024 * i);
-        dma16(vs + 16 * W::v_piece(t16, c), vd + 1024 * i);
       }
     };
 
@@ -193,17 +222,46 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       const char* kt = lds + buf * W::kBuf;
       const char* vt = kt + 2 * W::kBuf;
 
+      // Scores: K operands four products ahead.
       f32x16 s[2];
+      u32x4 kf[2][4];
+      auto read_k = [&](int n) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+        for (int e = 0; e < 4; ++e) {
+          const int b = (4 * n + e) / W::kQ, j = (4 * n + e) % W::kQ;
+          kf[n & 1][e] = *reinterpret_cast<const u32x4*>(kt + (32 * b + r32) * W::kRow +
+                                                         16 * W::k_piece(r32, 2 * j + h));
+        }
+      };
+      read_k(0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-        const char* krow = kt + (32 * b + r32) * W::kRow;
+      for (int n = 0; n < W::kQ / 2; ++n) {
+        if (n + 1 < W::kQ / 2) read_k(n + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < W::kQ; ++j)
-          s[b] = mfma32<kF16>(
-              *reinterpret_cast<const u32x4*>(krow + 16 * W::k_piece(r32, 2 * j + h)), q[j], s[b]);
+        for (int e = 0; e < 4; ++e) {
+          const int b = (4 * n + e) / W::kQ, j = (4 * n + e) % W::kQ;
+          if (j == 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+          s[b] = mfma32<kF16>(kf[n & 1][e], q[j], s[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      // V operands of 16 keys: rows 16 i + 4 h + 0..3 and 8 further on, columns
+      // 32 j + l % 32.
+      u32x4 vf[2][W::kO];
+      auto read_v = [&](int i) {
+        const int t0 = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+        for (int j = 0; j < W::kO; ++j) {
+          const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+          const char* a = vt + (16 * i + t0) * W::kRow + 16 * W::v_piece(t0, byte >> 4) + (byte & 15);
+          const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
+          vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
+        }
+      };
+      read_v(0);
       if (kKT * t + kKT > len) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -213,21 +271,33 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
             s[b][i] = key < len ? s[b][i] : kNegInf;
           }
       }
-      float top = fmaxf(s[0][0], s[1][0]);
+      // The first maximum is the compiler's, which waits for the last product
+      // (and so for all before it); it does not wait for an asm operand.
+      float top = fmaxf(s[1][15], s[0][15]);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+      for (int i = 0; i < 15; ++i) top = max3_raw(top, s[0][i], s[1][i]);
       {
         const SwapPair sw = swap_halves(top);
-        top = fmaxf(sw.a, sw.b) * p.scale_log2;
+        top = max_raw(sw.a, sw.b) * p.scale_log2;
       }
-      if (__ballot(top > m + kSlack || (m == kNegInf && top > m)) != 0) {
+      if (__ballot(top > m + kSlack) != 0) {
         const float next = fmaxf(m, top);
         const float ref = next == kNegInf ? 0.0f : next;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        float alpha = __builtin_amdgcn_exp2f(m - ref);
         m = next;
+        // In place: otherwise the branch costs a copy of O in every tile. The
+        // compiler does not see that the first product needs a wait after the
+        // exp2; O's own products were issued before the scores'.
+        asm volatile("s_nop 3" : "+v"(alpha));
         l *= alpha;
 #pragma unroll
-        for (int j = 0; j < W::kO; ++j) o[j] *= alpha;
+        for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float x = o[j][i];
+            asm volatile("v_mul_f32 %0, %0, %1" : "+v"(x) : "v"(alpha));
+            o[j][i] = x;
+          }
       }
       const float shift = (m == kNegInf ? 0.0f : m) - kBias;
       u32x4 pf[4];
@@ -237,20 +307,17 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
         for (int i = 0; i < 16; i += 2) {
           const float x0 = __builtin_amdgcn_exp2f(s[b][i] * p.scale_log2 - shift);
           const float x1 = __builtin_amdgcn_exp2f(s[b][i + 1] * p.scale_log2 - shift);
-          l += x0 + x1;
-          pf[2 * b + (i >> 3)][(i & 7) >> 1] = pack16<kF16>(x0, x1);
+          const uint32_t w = pack16<kF16>(x0, x1);
+          l = add_pair<kF16>(w, l);
+          pf[2 * b + (i >> 3)][(i & 7) >> 1] = w;
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < 3) read_v(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < W::kO; ++j) {
-          // Rows 16 i + 4 h + 0..3 and 8 further on, columns 32 j + l % 32.
-          const int t0 = 4 * h + ((lane & 15) >> 2);
-          const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-          const char* a = vt + (16 * i + t0) * W::kRow + 16 * W::v_piece(t0, byte >> 4) + (byte & 15);
-          const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
-          o[j] = mfma32<kF16>((u32x4){x[0], x[1], y[0], y[1]}, pf[i], o[j]);
-        }
+        for (int j = 0; j < W::kO; ++j) o[j] = mfma32<kF16>(vf[i & 1][j], pf[i], o[j]);
       }
     }
 
