@@ -15,9 +15,9 @@
 // leaves unnormalised partial sums in the workspace, two slots per work-group
 // whatever the batch: slot 2 w for a range that begins inside a group, 2 w + 1
 // for one that begins with it. The work-group that holds a group's beginning
-// notes how it was cut (P16Cut), for the combine, which joins it: the note's
-// place is the group's number where that is known (one query token per request)
-// and there are few, the work-group's otherwise.
+// notes how it was cut (P16Cut), for the combine, which joins it. The note's
+// place is the group's number where the launch has few groups, so that the
+// combine needs no work-groups for nothing, and the work-group's otherwise.
 //
 // Everything is a function of the device's lengths and of launch constants,
 // so a captured graph replays as the lengths change.
@@ -52,7 +52,7 @@ struct P16Params {
   int32_t team;           // units of a group: 1, 2 or 4
   int32_t key_tile_log2;  // keys of a tile
   int32_t slot_rows;      // rows of a unit that a slot holds: no unit has more
-  int32_t notes;          // notes by group number: how many; 0: by work-group
+  int32_t notes;          // notes by group number: at most so many; 0: by work-group
   float scale_log2;       // softmax_scale * log2(e)
 };
 
@@ -73,7 +73,7 @@ constexpr int kP16CutShift = 16;
 
 // Workspace: rows of D sums with a maximum and a sum each, as many as the
 // work-groups of a compute unit (at most kP16WgPerCu) have in their slots, and
-// a P16Cut for each work-group.
+// a P16Cut for each work-group and one before them.
 constexpr int kP16WsRowsPerCu = 512, kP16WgPerCu = 8;
 inline int64_t p16_workspace_floats(int32_t head_size, int32_t cus) {
   return static_cast<int64_t>(cus) * (kP16WsRowsPerCu * (head_size + 2) + 4 * kP16WgPerCu);
@@ -114,17 +114,21 @@ __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int 
   return x;
 }
 
-// Tiles of request `r` by vector loads (r differs from lane to lane).
+// Tiles and groups of request `r` by vector loads (r differs from lane to lane).
+struct P16Count {
+  int64_t tiles;
+  int32_t groups;
+};
 template <int kRows>
-__device__ __forceinline__ int64_t p16_lane_tiles(const P16Params& p, int r) {
-  if (r >= p.num_reqs) return 0;
+__device__ __forceinline__ P16Count p16_lane_count(const P16Params& p, int r) {
+  if (r >= p.num_reqs) return {0, 0};
   int len = p.kv_lens[r], q0 = 0, q1 = 0;
   if (p.qsl != nullptr) {
     q0 = p.qsl[r];
     q1 = p.qsl[r + 1];
   }
   const P16Req x = p16_request_of<kRows>(p, r, q0, q1, len);
-  return static_cast<int64_t>(x.n_gr) * x.n_kt;
+  return {static_cast<int64_t>(x.n_gr) * x.n_kt, x.n_gr};
 }
 
 // Forward-only walk over the requests, 64 at a time (every lane the same but
@@ -133,18 +137,35 @@ struct P16Cursor {
   int r0;
   int64_t base, end;  // tiles before request r0, and through r0 + 63
   int64_t incl;       // the lane's inclusive prefix within the 64
+  int32_t groups, group_incl;  // groups before request r0; prefix (p16_counted)
 };
+
+// Groups are counted beside the tiles where their number is the note's place
+// and the requests have different ones.
+__device__ __forceinline__ bool p16_counted(const P16Params& p) {
+  return p.notes != 0 && p.qsl != nullptr;
+}
+
+// The cursor at the 64 requests from r0 on.
+template <int kRows>
+__device__ __forceinline__ void p16_window(const P16Params& p, P16Cursor& c, int lane) {
+  const P16Count n = p16_lane_count<kRows>(p, c.r0 + lane);
+  c.incl = wave_scan64(n.tiles, lane);
+  c.end = c.base + readlane64(c.incl, 63);
+  if (p16_counted(p)) c.group_incl = wave_scan32(n.groups);
+}
 
 // All tiles of the launch; the cursor at its first 64 requests.
 template <int kRows>
 __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, int lane) {
   c.r0 = 0;
   c.base = 0;
-  c.incl = wave_scan64(p16_lane_tiles<kRows>(p, lane), lane);
-  c.end = readlane64(c.incl, 63);
+  c.groups = 0;
+  c.group_incl = 0;
+  p16_window<kRows>(p, c, lane);
   if (p.num_reqs <= 64) return c.end;
   int64_t more = 0;
-  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) more += p16_lane_tiles<kRows>(p, r0 + lane);
+  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) more += p16_lane_count<kRows>(p, r0 + lane).tiles;
   return c.end + readlane64(wave_scan64(more, lane), 63);
 }
 
@@ -152,6 +173,7 @@ __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, i
 struct P16Group {
   P16Req req;
   int32_t r, group, kt;
+  int32_t number;  // of the request's first group, where it counts (p16_counted)
 };
 
 // The group of tile `at` (not before the cursor, and less than all tiles).
@@ -161,13 +183,14 @@ __device__ __forceinline__ P16Group p16_locate(const P16Params& p, P16Cursor& c,
   while (at >= c.end && c.r0 + 64 < p.num_reqs) {
     c.r0 += 64;
     c.base = c.end;
-    c.incl = wave_scan64(p16_lane_tiles<kRows>(p, c.r0 + lane), lane);
-    c.end = c.base + readlane64(c.incl, 63);
+    c.groups += __builtin_amdgcn_readlane(c.group_incl, 63);
+    p16_window<kRows>(p, c, lane);
   }
   const int64_t local = at - c.base;
   const int j = min(static_cast<int>(__popcll(__ballot(c.incl <= local))), 63);
   const int64_t before = j > 0 ? readlane64(c.incl, j - 1) : 0;
   P16Group u;
+  u.number = c.groups + (j > 0 ? __builtin_amdgcn_readlane(c.group_incl, j - 1) : 0);
   u.r = __builtin_amdgcn_readfirstlane(min(c.r0 + j, p.num_reqs - 1));
   int len = ld_ro(p.kv_lens, u.r), q0 = 0, q1 = 0;
   if (p.qsl != nullptr) {
@@ -238,11 +261,24 @@ __device__ __forceinline__ void p16_note(const P16Params& p, const P16Group& gr,
   if (cut)
     c.slots_wg = static_cast<uint32_t>(p16_holder(tiles, first + gr.req.n_kt - 1, takers) - wg + 1) |
                  static_cast<uint32_t>(wg) << kP16CutShift;
-  *p16_cut<D>(p, p.notes ? gr.r * gr.req.n_gr + gr.group : wg) = c;
+  // Starts that run backwards can make more groups than there are notes.
+  const int number = (p16_counted(p) ? gr.number : gr.r * gr.req.n_gr) + gr.group;
+  if (p.notes == 0 || static_cast<uint32_t>(number) < static_cast<uint32_t>(p.notes))
+    *p16_cut<D>(p, p.notes ? 1 + number : wg) = c;
 }
 template <int D>
 __device__ __forceinline__ void p16_note_none(const P16Params& p, int wg) {
   if (!p.notes) p16_cut<D>(p, wg)->slots_wg = 0u;
+}
+// The note before the first group's: how many groups there are. By the first
+// work-group, in any case.
+template <int kRows, int D>
+__device__ __forceinline__ void p16_note_groups(const P16Params& p, const P16Cursor& c, int lane) {
+  if (!p16_counted(p)) return;
+  int32_t n = __builtin_amdgcn_readlane(c.group_incl, 63);
+  for (int r0 = 64; r0 < p.num_reqs; r0 += 64)
+    n += __builtin_amdgcn_readlane(wave_scan32(p16_lane_count<kRows>(p, r0 + lane).groups), 63);
+  if (threadIdx.x == 0) p16_cut<D>(p, 0)->slots_wg = static_cast<uint32_t>(n);
 }
 
 // Query token and head of row `row` of a unit.

@@ -28,7 +28,8 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
   __shared__ f32x4 s_o[kCrews][kVec];
   __shared__ float s_m[kCrews], s_l[kCrews];
   const int col = threadIdx.x % kVec, crew = threadIdx.x / kVec;
-  const P16Cut cut = *p16_cut<D>(p, blockIdx.x);
+  if (p16_counted(p) && blockIdx.x >= p16_cut<D>(p, 0)->slots_wg) return;
+  const P16Cut cut = *p16_cut<D>(p, p.notes ? 1 + blockIdx.x : blockIdx.x);
   const int slots = cut.slots_wg & ((1u << kP16CutShift) - 1);
   const int wg = cut.slots_wg >> kP16CutShift;
   if (slots == 0) return;

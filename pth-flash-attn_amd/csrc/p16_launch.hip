@@ -138,20 +138,19 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   const int64_t span = p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + 15)
                                     : p.max_keys;
   const int64_t key_tiles = std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
-  const int64_t groups_exact = a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team);
   const int64_t groups = a.query_start_loc == nullptr
-                             ? groups_exact
-                             : (row_tiles * a.num_kv_heads + p.team - 1) / p.team + (p.team > 1 ? a.num_reqs : 0);
+                             ? a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team)
+                             : row_tiles * a.num_kv_heads / p.team + (p.team > 1 ? a.num_reqs : 0);
   PA_REQUIRE(row_tiles * a.num_kv_heads < INT32_MAX / key_tiles,
              "the launch exceeds 2^31 tiles");
   const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : 2) : rows_per_cu(a.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
-  if (a.query_start_loc == nullptr && groups_exact <= p.num_wg) p.notes = static_cast<int32_t>(groups_exact);
+  if (groups <= p.num_wg) p.notes = static_cast<int32_t>(groups);
   const bool f16 = a.dtype == PTH_ATTN_F16, page16 = a.block_size % 16 == 0;
   hipError_t err = wide ? launch_p16_wide_kernel(p, f16, page16, a.head_size, stream)
                         : launch_p16_rows_kernel(p, f16, page16, a.head_size, stream);
   const int32_t items = p.team * p.slot_rows;
-  const int32_t y = wide ? 4 : p.notes ? std::min(items, std::max(1, 2 * cus / p.notes)) : 1;
+  const int32_t y = p.notes ? std::min(items, std::max(wide ? 4 : 1, (wide ? 8 : 2) * cus / p.notes)) : wide ? 4 : 1;
   // A group of one tile is never cut.
   if (err == hipSuccess && key_tiles > 1)
     err = launch_p16_combine_kernel(p, f16, wide, a.head_size, y, stream);

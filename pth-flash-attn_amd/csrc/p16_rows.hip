@@ -161,6 +161,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
   const int sub = wave & (p.team - 1), part = wave >> (p.team >> 1), parts = kP16Waves >> (p.team >> 1);
   P16Cursor cur;
   const int64_t tiles = p16_begin<kBM>(p, cur, lane);
+  if (wg == 0) p16_note_groups<kBM, D>(p, cur, lane);
   const int takers = p16_takers(p, tiles);
   if (wg >= takers) {
     if (threadIdx.x == 0) p16_note_none<D>(p, wg);
