@@ -74,9 +74,10 @@ constexpr int kP16CutShift = 16;
 // Workspace: rows of D sums with a maximum and a sum each, as many as the
 // work-groups of a compute unit (at most kP16WgPerCu) have in their slots, and
 // a P16Cut for each work-group and one before them.
-constexpr int kP16WsRowsPerCu = 512, kP16WgPerCu = 8;
+constexpr int kP16WgPerCu = 8;
 inline int64_t p16_workspace_floats(int32_t head_size, int32_t cus) {
-  return static_cast<int64_t>(cus) * (kP16WsRowsPerCu * (head_size + 2) + 4 * kP16WgPerCu);
+  const int64_t rows = head_size == 64 ? 768 : 512;
+  return cus * (rows * (head_size + 2) + 4 * kP16WgPerCu);
 }
 
 #if defined(__HIPCC__)

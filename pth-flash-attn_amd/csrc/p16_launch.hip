@@ -143,7 +143,7 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
                              : row_tiles * a.num_kv_heads / p.team + (p.team > 1 ? a.num_reqs : 0);
   PA_REQUIRE(row_tiles * a.num_kv_heads < INT32_MAX / key_tiles,
              "the launch exceeds 2^31 tiles");
-  const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : 2) : rows_per_cu(a.head_size, groups, cus));
+  const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : a.head_size == 64 ? 3 : 2) : rows_per_cu(a.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
   if (groups <= p.num_wg) p.notes = static_cast<int32_t>(groups);
   const bool f16 = a.dtype == PTH_ATTN_F16, page16 = a.block_size % 16 == 0;

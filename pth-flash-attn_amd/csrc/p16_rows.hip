@@ -176,10 +176,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
     const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
     const bool whole = take == gr.req.n_kt;
     const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
-    if (gr.kt == 0 && (!whole || p.notes)) {
-      noted |= !whole;
-      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
-    }
+    const int64_t begin = at;
     at += take;
     // A group's last units may be missing: their waves repeat the last one
     // and drop it.
@@ -189,6 +186,23 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
     int64_t token, head;
     p16_row<kBM>(p, gr.req.q0, u, min(r16, max(rows - 1, 0)), token, head);
 
+    float m = kNegInf, l = 0.0f;
+    f32x4 o[R::kO];
+#pragma unroll
+    for (int j = 0; j < R::kO; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+    Walker<kPage16> w{p, p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride, gr.req.lo,
+                      gr.req.len, u.head};
+    const int step = 1 << p.key_tile_log2;  // 32 x parts
+    const int k_end = min(gr.req.base + (gr.kt + take) * step, gr.req.len);
+    int k0 = gr.req.base + gr.kt * step + 32 * part;
+
+    // The page numbers are on their way while Q is read.
+    int32_t first_entry[2] = {0, 0};
+    if (k0 < k_end) {
+      first_entry[0] = w.entry(k0);
+      first_entry[1] = w.entry(k0 + 16);
+    }
     // Q: 16 bytes per product, zeros in rows that the unit lacks.
     if (!first && parts > 1) __syncthreads();  // the last group's sums have been read
     first = false;
@@ -202,17 +216,6 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
         if constexpr (R::kQInLds) s_x[wave][j][lane] = __builtin_bit_cast(f32x4, q[j]);
       }
     }
-
-    float m = kNegInf, l = 0.0f;
-    f32x4 o[R::kO];
-#pragma unroll
-    for (int j = 0; j < R::kO; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-
-    Walker<kPage16> w{p, p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride, gr.req.lo,
-                      gr.req.len, u.head};
-    const int step = 1 << p.key_tile_log2;  // 32 x parts
-    const int k_end = min(gr.req.base + (gr.kt + take) * step, gr.req.len);
-    int k0 = gr.req.base + gr.kt * step + 32 * part;
 
     u32x4 kf[2][R::kQ];
     V vf[8][R::kPieces];
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
     if (k0 < k_end) {
       typename Walker<kPage16>::Block blk[2];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) blk[b] = w.block(k0 + 16 * b, w.entry(k0 + 16 * b));
+      for (int b = 0; b < 2; ++b) blk[b] = w.block(k0 + 16 * b, first_entry[b]);
 #pragma unroll
       for (int b = 0; b < 2; ++b) load_k(blk[b], b);
 #pragma unroll
@@ -318,6 +321,10 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
       chunk(std::false_type{});
     }
 
+    if (gr.kt == 0 && (!whole || p.notes)) {
+      noted |= !whole;
+      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, begin, takers, !whole);
+    }
     // The unit's first wave joins the others' sums to its own.
     l = xor_sum(l);
     if (parts > 1) {

@@ -33,7 +33,7 @@ typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
 struct WideOf {
-  static constexpr int kPerSimd = D == 256 ? 1 : 2;
+  static constexpr int kPerSimd = D == 256 ? 1 : D == 64 ? 3 : 2;
   static constexpr int kQ = D / 16;      // QK products per 32 keys
   static constexpr int kO = D / 32;      // output tiles
   static constexpr int kRow = 2 * D;     // bytes of a key row
@@ -79,6 +79,13 @@ __device__ __forceinline__ float add_pair(uint32_t w, float sum) {
                                            __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
 }
 
+// A barrier for LDS alone: __syncthreads also waits for stores to memory.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Column l % 16 of four rows of a row-major 16-bit matrix in LDS: lane i of
 // each 16 gives the address of row i / 4, columns 4 (i % 4).
 __device__ __forceinline__ u32x2 column4(const char* a) {
@@ -122,11 +129,6 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
     const bool whole = take == gr.req.n_kt;
     const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
-    if (gr.kt == 0 && (!whole || p.notes)) {
-      noted |= !whole;
-      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
-    }
-    at += take;
     const P16Unit u = p16_unit(gr.req, gr.group);
     const int rows = min(kBM, gr.req.rows - u.rt * kBM);
     const int row = 32 * wave + r32;
@@ -134,15 +136,6 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     int64_t token, head;
     p16_row<kBM>(p, gr.req.q0, u, min(row, rows - 1), token, head);
 
-    u32x4 q[W::kQ];
-    {
-      const char* src = p.q + token * p.s_q_tok + head * p.s_q_head + 16 * h;
-#pragma unroll
-      for (int j = 0; j < W::kQ; ++j) {
-        q[j] = *reinterpret_cast<const u32x4*>(src + 32 * j);
-        if (!live) q[j] = (u32x4){0u, 0u, 0u, 0u};
-      }
-    }
     float m = kNegInf, l = 0.0f;
     f32x16 o[W::kO];
 #pragma unroll
@@ -214,9 +207,24 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
 
     const int t_end = len > 0 ? gr.kt + take : gr.kt;
     int buf = 0;
-    // The last unit's reads of both buffers are done.
-    __syncthreads();
+    // The last unit's reads of both buffers are done (its stores may be on
+    // their way).
+    lds_barrier();
     if (gr.kt < t_end) load(gr.kt, 0);
+    u32x4 q[W::kQ];
+    {
+      const char* src = p.q + token * p.s_q_tok + head * p.s_q_head + 16 * h;
+#pragma unroll
+      for (int j = 0; j < W::kQ; ++j) {
+        q[j] = *reinterpret_cast<const u32x4*>(src + 32 * j);
+        if (!live) q[j] = (u32x4){0u, 0u, 0u, 0u};
+      }
+    }
+    if (gr.kt == 0 && (!whole || p.notes)) {
+      noted |= !whole;
+      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
+    }
+    at += take;
     for (int t = gr.kt; t < t_end; ++t, buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       auto read_k = [&](int n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int b = (4 * n + e) / W::kQ, j = (4 * n + e) % W::kQ;
+          const int b = e & 1, j = 2 * n + (e >> 1);
           kf[n & 1][e] = *reinterpret_cast<const u32x4*>(kt + (32 * b + r32) * W::kRow +
                                                          16 * W::k_piece(r32, 2 * j + h));
         }
@@ -242,7 +250,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int b = (4 * n + e) / W::kQ, j = (4 * n + e) % W::kQ;
+          const int b = e & 1, j = 2 * n + (e >> 1);
           if (j == 0)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
