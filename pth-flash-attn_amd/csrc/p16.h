@@ -115,20 +115,31 @@ __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int 
   return x;
 }
 
-// Tiles and groups of request `r` by vector loads (r differs from lane to lane).
+// Length and first and last query token of request `r` (r differs from lane to
+// lane; none behind the last request).
+struct P16Lane {
+  int32_t len, q0, q1;
+};
+__device__ __forceinline__ P16Lane p16_lane(const P16Params& p, int r) {
+  P16Lane x = {0, 0, 0};
+  if (r < p.num_reqs) {
+    x.len = p.kv_lens[r];
+    if (p.qsl != nullptr) {
+      x.q0 = p.qsl[r];
+      x.q1 = p.qsl[r + 1];
+    }
+  }
+  return x;
+}
+// Its tiles and groups.
 struct P16Count {
   int64_t tiles;
   int32_t groups;
 };
 template <int kRows>
-__device__ __forceinline__ P16Count p16_lane_count(const P16Params& p, int r) {
+__device__ __forceinline__ P16Count p16_count(const P16Params& p, const P16Lane& n, int r) {
   if (r >= p.num_reqs) return {0, 0};
-  int len = p.kv_lens[r], q0 = 0, q1 = 0;
-  if (p.qsl != nullptr) {
-    q0 = p.qsl[r];
-    q1 = p.qsl[r + 1];
-  }
-  const P16Req x = p16_request_of<kRows>(p, r, q0, q1, len);
+  const P16Req x = p16_request_of<kRows>(p, r, n.q0, n.q1, n.len);
   return {static_cast<int64_t>(x.n_gr) * x.n_kt, x.n_gr};
 }
 
@@ -139,6 +150,7 @@ struct P16Cursor {
   int64_t base, end;  // tiles before request r0, and through r0 + 63
   int64_t incl;       // the lane's inclusive prefix within the 64
   int32_t groups, group_incl;  // groups before request r0; prefix (p16_counted)
+  P16Lane of;                  // the lane's request
 };
 
 // Groups are counted beside the tiles where their number is the note's place
@@ -150,7 +162,8 @@ __device__ __forceinline__ bool p16_counted(const P16Params& p) {
 // The cursor at the 64 requests from r0 on.
 template <int kRows>
 __device__ __forceinline__ void p16_window(const P16Params& p, P16Cursor& c, int lane) {
-  const P16Count n = p16_lane_count<kRows>(p, c.r0 + lane);
+  c.of = p16_lane(p, c.r0 + lane);
+  const P16Count n = p16_count<kRows>(p, c.of, c.r0 + lane);
   c.incl = wave_scan64(n.tiles, lane);
   c.end = c.base + readlane64(c.incl, 63);
   if (p16_counted(p)) c.group_incl = wave_scan32(n.groups);
@@ -166,7 +179,8 @@ __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, i
   p16_window<kRows>(p, c, lane);
   if (p.num_reqs <= 64) return c.end;
   int64_t more = 0;
-  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) more += p16_lane_count<kRows>(p, r0 + lane).tiles;
+  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) 
+    more += p16_count<kRows>(p, p16_lane(p, r0 + lane), r0 + lane).tiles;
   return c.end + readlane64(wave_scan64(more, lane), 63);
 }
 
@@ -188,17 +202,15 @@ __device__ __forceinline__ P16Group p16_locate(const P16Params& p, P16Cursor& c,
     p16_window<kRows>(p, c, lane);
   }
   const int64_t local = at - c.base;
-  const int j = min(static_cast<int>(__popcll(__ballot(c.incl <= local))), 63);
+  const int j = __builtin_amdgcn_readfirstlane(
+      min(static_cast<int>(__popcll(__ballot(c.incl <= local))), 63));
   const int64_t before = j > 0 ? readlane64(c.incl, j - 1) : 0;
   P16Group u;
   u.number = c.groups + (j > 0 ? __builtin_amdgcn_readlane(c.group_incl, j - 1) : 0);
   u.r = __builtin_amdgcn_readfirstlane(min(c.r0 + j, p.num_reqs - 1));
-  int len = ld_ro(p.kv_lens, u.r), q0 = 0, q1 = 0;
-  if (p.qsl != nullptr) {
-    q0 = ld_ro(p.qsl, u.r);
-    q1 = ld_ro(p.qsl, u.r + 1);
-  }
-  u.req = p16_request_of<kRows>(p, u.r, q0, q1, len);
+  u.req = p16_request_of<kRows>(p, u.r, __builtin_amdgcn_readlane(c.of.q0, j),
+                                __builtin_amdgcn_readlane(c.of.q1, j),
+                                __builtin_amdgcn_readlane(c.of.len, j));
   // Within a request: less than 2^31 tiles, by the launcher's check.
   const uint32_t in_req = static_cast<uint32_t>(local - before);
   const uint32_t n_kt = static_cast<uint32_t>(u.req.n_kt);
@@ -278,7 +290,8 @@ __device__ __forceinline__ void p16_note_groups(const P16Params& p, const P16Cur
   if (!p16_counted(p)) return;
   int32_t n = __builtin_amdgcn_readlane(c.group_incl, 63);
   for (int r0 = 64; r0 < p.num_reqs; r0 += 64)
-    n += __builtin_amdgcn_readlane(wave_scan32(p16_lane_count<kRows>(p, r0 + lane).groups), 63);
+    n += __builtin_amdgcn_readlane(
+        wave_scan32(p16_count<kRows>(p, p16_lane(p, r0 + lane), r0 + lane).groups), 63);
   if (threadIdx.x == 0) p16_cut<D>(p, 0)->slots_wg = static_cast<uint32_t>(n);
 }
 

@@ -155,19 +155,22 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     }
     // The wave's 16 keys of tile t into buffer `buf`; keys past the last
     // one repeat it.
-    auto load = [&](int t, int buf) {
-      int kb = kKT * t + 16 * wave;
-      kb = min(kb, (len - 1) & ~15);
+    auto block = [&](int t) { return min(kKT * t + 16 * wave, (len - 1) & ~15); };
+    auto page = [&](int t) {  // its entry of the block table
+      if constexpr (!kPage16) return 0u;
+      return mulhi32(static_cast<uint32_t>(block(t)), p.bs_div.mul) >> p.bs_div.shift;
+    };
+    auto load = [&](int t, int buf, int32_t entry) {
+      const int kb = block(t);
       char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
       char* vd = kd + 2 * W::kBuf;
       if constexpr (kPage16) {
-        const uint32_t pg = mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
-        int32_t id = ld_ro(table, pg);
-        id = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks) ? id : 0;
-        const int64_t first = kb - static_cast<int32_t>(pg * p.bs_div.d);
-        const char* ks = p.k.base + static_cast<int64_t>(id) * p.k.s_block + first * p.k.s_slot +
+        const int64_t id =
+            static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks) ? entry : 0;
+        const int64_t first = kb - static_cast<int32_t>(page(t) * p.bs_div.d);
+        const char* ks = p.k.base + id * p.k.s_block + first * p.k.s_slot +
                          static_cast<int64_t>(u.head) * p.k.s_head;
-        const char* vs = p.v.base + static_cast<int64_t>(id) * p.v.s_block + first * p.v.s_slot +
+        const char* vs = p.v.base + id * p.v.s_block + first * p.v.s_slot +
                          static_cast<int64_t>(u.head) * p.v.s_head;
         if (kb + 16 <= len) {
 #pragma unroll
@@ -210,7 +213,13 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     // The last unit's reads of both buffers are done (its stores may be on
     // their way).
     lds_barrier();
-    if (gr.kt < t_end) load(gr.kt, 0);
+    // Page numbers are read a tile before their loads.
+    int32_t entry = 0;
+    if (gr.kt < t_end) {
+      entry = kPage16 ? ld_ro(table, page(gr.kt)) : 0;
+      load(gr.kt, 0, entry);
+      entry = kPage16 ? ld_ro(table, page(gr.kt + 1)) : 0;
+    }
     u32x4 q[W::kQ];
     {
       const char* src = p.q + token * p.s_q_tok + head * p.s_q_head + 16 * h;
@@ -228,7 +237,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     for (int t = gr.kt; t < t_end; ++t, buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
-      if (t + 1 < t_end) load(t + 1, buf ^ 1);
+      if (t + 1 < t_end) {
+        load(t + 1, buf ^ 1, entry);
+        entry = kPage16 ? ld_ro(table, page(t + 2)) : 0;
+      }
       const char* kt = lds + buf * W::kBuf;
       const char* vt = kt + 2 * W::kBuf;
 

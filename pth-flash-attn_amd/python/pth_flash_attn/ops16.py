@@ -158,14 +158,19 @@ def build_step_tables_fake(block_table, slot_mapping, seq_lens, query_start_loc,
 FAKES = {name: globals()[f"{name}_fake"] for name in NAMES}
 
 
+_OVERLOADS: dict = {}  # the loaded library's ops, looked up once
+
+
 def _op(name: str):
-    try:
-        return getattr(torch.ops.pth_flash_attn, name).default
-    except AttributeError:
-        raise RuntimeError(
-            f"{name}: the op library is not loaded; run python pth-flash-attn_amd/build.py and "
-            "import pth_flash_attn.ops"
-        ) from None
+    op = _OVERLOADS.get(name)
+    if op is None:
+        if not hasattr(torch.ops.pth_flash_attn, name):
+            raise RuntimeError(
+                f"{name}: the op library is not loaded; run python pth-flash-attn_amd/build.py "
+                "and import pth_flash_attn.ops"
+            )
+        op = _OVERLOADS[name] = getattr(torch.ops.pth_flash_attn, name).default
+    return op
 
 
 def build_step_tables(
