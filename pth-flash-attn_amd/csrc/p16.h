@@ -143,14 +143,17 @@ __device__ __forceinline__ P16Count p16_count(const P16Params& p, const P16Lane&
   return {static_cast<int64_t>(x.n_gr) * x.n_kt, x.n_gr};
 }
 
-// Forward-only walk over the requests, 64 at a time (every lane the same but
-// for `incl`).
+// Walk over the requests, 64 (a window) at a time. Lane i knows its request of
+// the window, and, up to 64 windows, how many tiles and groups end with window
+// i, so that a work-group goes to its own at once.
 struct P16Cursor {
-  int r0;
-  int64_t base, end;  // tiles before request r0, and through r0 + 63
-  int64_t incl;       // the lane's inclusive prefix within the 64
-  int32_t groups, group_incl;  // groups before request r0; prefix (p16_counted)
+  int r0;             // the window's first request
+  int64_t base, end;  // tiles before it, and through it
+  int64_t incl;       // the lane's inclusive prefix within it
+  int32_t groups, group_incl;  // groups before it; the lane's prefix (p16_counted)
   P16Lane of;                  // the lane's request
+  int64_t window_end;
+  int32_t window_groups;
 };
 
 // Groups are counted beside the tiles where their number is the note's place
@@ -169,7 +172,7 @@ __device__ __forceinline__ void p16_window(const P16Params& p, P16Cursor& c, int
   if (p16_counted(p)) c.group_incl = wave_scan32(n.groups);
 }
 
-// All tiles of the launch; the cursor at its first 64 requests.
+// All tiles of the launch; the cursor at its first window.
 template <int kRows>
 __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, int lane) {
   c.r0 = 0;
@@ -178,10 +181,22 @@ __device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, i
   c.group_incl = 0;
   p16_window<kRows>(p, c, lane);
   if (p.num_reqs <= 64) return c.end;
-  int64_t more = 0;
-  for (int r0 = 64; r0 < p.num_reqs; r0 += 64) 
-    more += p16_count<kRows>(p, p16_lane(p, r0 + lane), r0 + lane).tiles;
-  return c.end + readlane64(wave_scan64(more, lane), 63);
+  int64_t all = c.end;
+  int32_t groups = p16_counted(p) ? __builtin_amdgcn_readlane(c.group_incl, 63) : 0;
+  c.window_end = all;
+  c.window_groups = groups;
+#pragma unroll 2
+  for (int w = 1; w < (p.num_reqs + 63) >> 6; ++w) {
+    const int r = 64 * w + lane;
+    const P16Count n = p16_count<kRows>(p, p16_lane(p, r), r);
+    all += readlane64(wave_scan64(n.tiles, lane), 63);
+    if (p16_counted(p)) groups += __builtin_amdgcn_readlane(wave_scan32(n.groups), 63);
+    if (lane >= w) {
+      c.window_end = all;
+      c.window_groups = groups;
+    }
+  }
+  return all;
 }
 
 // A group, and the tile of it that a position falls on.
@@ -195,11 +210,22 @@ struct P16Group {
 template <int kRows>
 __device__ __forceinline__ P16Group p16_locate(const P16Params& p, P16Cursor& c, int64_t at,
                                                int lane) {
-  while (at >= c.end && c.r0 + 64 < p.num_reqs) {
-    c.r0 += 64;
-    c.base = c.end;
-    c.groups += __builtin_amdgcn_readlane(c.group_incl, 63);
-    p16_window<kRows>(p, c, lane);
+  if (at >= c.end && p.num_reqs > 64) {
+    // Past the 64th window, which says what all after it hold, one by one.
+    const int w = static_cast<int>(__popcll(__ballot(c.window_end <= at)));
+    if (c.r0 < 64 * 63 && w > 0) {
+      const int to = min(w, 63);
+      c.r0 = 64 * to;
+      c.base = readlane64(c.window_end, to - 1);
+      c.groups = __builtin_amdgcn_readlane(c.window_groups, to - 1);
+      p16_window<kRows>(p, c, lane);
+    }
+    while (at >= c.end && c.r0 + 64 < p.num_reqs) {
+      c.r0 += 64;
+      c.base = c.end;
+      c.groups += __builtin_amdgcn_readlane(c.group_incl, 63);
+      p16_window<kRows>(p, c, lane);
+    }
   }
   const int64_t local = at - c.base;
   const int j = __builtin_amdgcn_readfirstlane(

@@ -83,6 +83,29 @@ def test_decode_long_and_many(D):
     assert torch.equal(got, decode(c, q, D**-0.5))  # deterministic
 
 
+@pytest.mark.parametrize("R", [64, 65, 128, 1000, 4096, 4097, 4500])
+def test_many_requests(R):
+    """Around 64 requests and around 64 times 64; a few tokens each."""
+    gen = torch.Generator().manual_seed(R)
+    lens = torch.randint(0, 40, (R,), generator=gen).tolist()
+    lens[R // 2] = 3000
+    c = make_cache(lens, Hkv=1, D=64, block=16, dtype=BF, seed=R)
+    q = queries(R, 2, 64, BF, R)
+    got = decode(c, q, 0.125)
+    few = list(range(0, R, max(1, R // 40))) + [R // 2, R - 1]
+    for r in few:
+        assert_close(got[r : r + 1], *reference(q[r : r + 1], c.keys[r : r + 1], [1], 0.125, pair=True))
+    q_lens = torch.randint(0, 12, (R,), generator=gen).tolist()
+    starts = starts_of(q_lens)
+    q = queries(sum(q_lens), 2, 64, BF, R + 1)
+    got = cross(c, q, q_lens, 0.125, starts=starts)
+    at = starts.tolist()
+    for r in few:
+        rows = slice(at[r], at[r + 1])
+        assert_close(got[rows], *reference(q[rows], c.keys[r : r + 1], q_lens[r : r + 1], 0.125))
+    assert not got.isnan().any()
+
+
 def test_decode_long_alone():
     c = make_cache([131072], Hkv=2, D=128, block=16, dtype=BF, seed=6)
     q = queries(1, 8, 128, BF, 6)
