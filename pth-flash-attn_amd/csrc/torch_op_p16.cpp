@@ -49,13 +49,17 @@ int64_t extent_bytes(const Tensor& t) {
   }
   return __builtin_mul_overflow(total, static_cast<int64_t>(t.element_size()), &total) ? -1 : total;
 }
-bool overlap(const Tensor& a, const Tensor& b) {
-  const int64_t na = extent_bytes(a), nb = extent_bytes(b);
-  if (na <= 0 || nb <= 0) return false;
-  const auto pa = reinterpret_cast<uintptr_t>(a.data_ptr());
-  const auto pb = reinterpret_cast<uintptr_t>(b.data_ptr());
-  return pa < pb + static_cast<uintptr_t>(nb) && pb < pa + static_cast<uintptr_t>(na);
+// The bytes that a tensor spans.
+struct Span {
+  uintptr_t begin, end;
+};
+Span span_of(const char* op, const Tensor& t) {
+  const int64_t n = extent_bytes(t);
+  OP_CHECK(n >= 0, "negative strides, or a byte extent that overflows int64");
+  const auto p = n > 0 ? reinterpret_cast<uintptr_t>(t.data_ptr()) : 0;
+  return {p, p + static_cast<uintptr_t>(n)};
 }
+bool overlap(const Span& a, const Span& b) { return a.begin < b.end && b.begin < a.end; }
 
 // The kernels are built for gfx950; a device's name does not change.
 void check_device_arch(const char* op, const Tensor& t) {
@@ -160,14 +164,19 @@ void attend(const char* op, const char* lens_name, const Tensor& out, const Tens
             int64_t max_len, double softmax_scale, const Tensor& ws, int64_t window) {
   check_attention(op, lens_name, out, q, k_cache, v_cache, block_table, lens, query_start_loc,
                   max_len, softmax_scale, ws, window);
-  for (const Tensor* t : {&out, &q, &k_cache, &v_cache, &block_table})
-    OP_CHECK(extent_bytes(*t) >= 0, "negative strides, or a byte extent that overflows int64");
-  OP_CHECK(!overlap(out, ws), "out and ws must not overlap");
+  const Span s_out = span_of(op, out), s_ws = span_of(op, ws), s_q = span_of(op, q);
+  OP_CHECK(!overlap(s_out, s_ws), "out and ws must not overlap");
+  OP_CHECK(!overlap(s_ws, s_q), "ws must not overlap an input");
   for (const Tensor* t : {&k_cache, &v_cache, &block_table, &lens}) {
-    OP_CHECK(!overlap(out, *t), "out must not overlap an input");
-    OP_CHECK(!overlap(ws, *t), "ws must not overlap an input");
+    const Span s = span_of(op, *t);
+    OP_CHECK(!overlap(s_out, s), "out must not overlap an input");
+    OP_CHECK(!overlap(s_ws, s), "ws must not overlap an input");
   }
-  OP_CHECK(!overlap(ws, q), "ws must not overlap an input");
+  if (query_start_loc != nullptr) {
+    const Span s = span_of(op, *query_start_loc);
+    OP_CHECK(!overlap(s_out, s), "out must not overlap an input");
+    OP_CHECK(!overlap(s_ws, s), "ws must not overlap an input");
+  }
   OP_CHECK(fits32(q.size(0)) && fits32(k_cache.size(0)) && fits32(k_cache.size(1)) &&
                fits32(block_table.size(1)),
            "a size exceeds int32");
@@ -254,8 +263,11 @@ void reshape_and_cache_16bit(const Tensor& key, const Tensor& value, const Tenso
            "slot_mapping must be contiguous int64 [T]");
   for (const Tensor* t : {&value, &k_cache, &v_cache, &slot_mapping})
     OP_CHECK(t->device() == key.device(), "all tensors must be on the device of key");
-  for (const Tensor* t : {&key, &value, &k_cache, &v_cache})
-    OP_CHECK(extent_bytes(*t) >= 0, "negative strides, or a byte extent that overflows int64");
+  const Span s_k = span_of(op, k_cache), s_v = span_of(op, v_cache);
+  for (const Tensor* t : {&key, &value, &slot_mapping}) {
+    const Span s = span_of(op, *t);
+    OP_CHECK(!overlap(s_k, s) && !overlap(s_v, s), "the cache must not overlap an input");
+  }
   OP_CHECK(fits32(T) && fits32(k_cache.size(0)) && fits32(k_cache.size(1)) && fits32(Hkv),
            "a size exceeds int32");
   check_on_gpu(op, key);
@@ -321,13 +333,14 @@ void build_step_tables(const Tensor& block_table, const Tensor& slot_mapping,
   for (const Tensor* t : ins)
     OP_CHECK(t->device() == context_lens.device(),
              "all tensors must be on the device of context_lens");
-  OP_CHECK(extent_bytes(block_table) >= 0,
-           "negative strides, or a byte extent that overflows int64");
+  Span s[9];
+  for (size_t i = 0; i < 5; ++i) s[i] = span_of(op, *outs[i]);
+  for (size_t i = 0; i < 4; ++i) s[5 + i] = span_of(op, *ins[i]);
   for (size_t i = 0; i < 5; ++i) {
     for (size_t j = i + 1; j < 5; ++j)
-      OP_CHECK(!overlap(*outs[i], *outs[j]), "the outputs must not overlap each other");
-    for (const Tensor* t : ins)
-      OP_CHECK(!overlap(*outs[i], *t), "an output must not overlap an input");
+      OP_CHECK(!overlap(s[i], s[j]), "the outputs must not overlap each other");
+    for (size_t j = 5; j < 9; ++j)
+      OP_CHECK(!overlap(s[i], s[j]), "an output must not overlap an input");
   }
   check_on_gpu(op, context_lens);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(context_lens.device());
