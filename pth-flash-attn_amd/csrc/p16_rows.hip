@@ -21,8 +21,9 @@
 // scalar unit, a chunk before. So a wave always has 4 to 16 KB in flight.
 //
 // Numerics. Scores, m, l and o are 32 bits. P is a 16-bit pair hi + lo (16 to
-// 22 significant bits): the second product costs matrix time that this kernel
-// has to spare, being bound by the cache's bytes. A masked key takes the
+// 22 significant bits, in fp16 scaled by 2^14 for its short range): the second
+// product costs matrix time that this kernel has to spare, being bound by the
+// cache's bytes. A masked key takes the
 // address of a visible one and the weight 0, so nothing behind a request's
 // last key, or in another's page, can reach a sum, whatever it holds.
 
@@ -148,6 +149,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
   using R = RowsDim<D>;
   using V = typename VRun<R::kCols>::type;
   constexpr int kBM = kP16RowsRows;
+  constexpr float kBias = kF16 ? 14.0f : 0.0f;  // P is scaled by 2^kBias
   // The sums of the waves that are not their unit's first, at the end; Q
   // before it, if it lives here.
   __shared__ f32x4 s_x[kP16Waves][R::kO][64];
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
         l *= alpha;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_amdgcn_exp2f(t[e] - ref);
+          x[e] = __builtin_amdgcn_exp2f(t[e] - (ref - kBias));
           l += x[e];
         }
         u32x4 hi, lo;

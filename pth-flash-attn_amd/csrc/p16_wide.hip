@@ -18,8 +18,8 @@
 // a score passes it by 2^kSlack, so most tiles rescale nothing. P is rounded
 // once to the inputs' type, as the output is: both errors are independent, and
 // together sqrt(2) of the output's own; l sums the rounded P, by dot products
-// of its pairs. In fp16, whose range is short, P is scaled by 2^8: weights down
-// to 2^-22 of a row's largest keep all 11 bits.
+// of its pairs. In fp16, whose range is short, P is scaled by 2^12: weights down
+// to 2^-26 of a row's largest keep all 11 bits.
 
 #include "attn_device.h"
 #include "p16.h"
@@ -99,8 +99,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
     const P16Params p) {
   using W = WideOf<D>;
   constexpr int kBM = kP16WideRows, kKT = kP16WideKeys;
-  constexpr float kSlack = kF16 ? 7.0f : 8.0f;
-  constexpr float kBias = kF16 ? 8.0f : 0.0f;
+  constexpr float kSlack = kF16 ? 3.0f : 8.0f;
+  constexpr float kBias = kF16 ? 12.0f : 0.0f;
   __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
 
   const int lane = threadIdx.x & 63;

@@ -285,6 +285,33 @@ def test_sharp_rows(n, dtype):
     assert_close(cross(c, q, [n, n], 0.3), *reference(q, c.keys, [n, n], 0.3, pair=n == 1))
 
 
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("below", [10, 20, 24, 26])
+def test_one_large_weight_and_many_small(n, dtype, below):
+    """30,000 keys 2^-below of the first one's weight: their sum counts. The
+    first one's V is 0 and theirs 1; all numbers are powers of two, so that the
+    output is x / (1 + x) rounded once, and P is exact."""
+    N = 30000
+    c = make_cache([N], Hkv=1, D=64, block=16, dtype=dtype, seed=31)
+    k, v = torch.zeros(N, 1, 64, dtype=dtype, device=DEV), torch.ones(N, 1, 64, dtype=dtype,
+                                                                      device=DEV)
+    k[1:, 0, 0] = -float(below)
+    v[0] = 0.0
+    pos = torch.arange(N, device=DEV)
+    page = c.table[0].long()[pos // 16]
+    c.k[page, pos % 16], c.v[page, pos % 16] = k, v
+    q = torch.zeros(n, 1, 64, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1.0
+    got = cross(c, q, [n], math.log(2.0)).double()
+    x = (N - 1) * 2.0**-below
+    want = x / (1 + x)
+    # ln 2 in 32 bits and its product with log2(e) (2 u), exp2 (2 u), each times
+    # `below` or less, and 30,000 additions in 32 bits; the output's rounding.
+    h, u = torch.finfo(dtype).eps / 2, 2.0**-24
+    assert ((got - want).abs() <= want * (h + u * (4 * below + 4 + 2 * N))).all()
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 4 GiB, its last pages in use."""
     block, Hkv, D = 64, 8, 128
