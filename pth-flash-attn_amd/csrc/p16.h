@@ -52,7 +52,9 @@ struct P16Params {
   int32_t team;           // units of a group: 1, 2 or 4
   int32_t key_tile_log2;  // keys of a tile
   int32_t slot_rows;      // rows of a unit that a slot holds: no unit has more
-  int32_t notes;          // notes by group number: at most so many; 0: by work-group
+  // Notes by group number: at most so many; 0: by work-group; -1: none, no
+  // group is cut.
+  int32_t notes;
   float scale_log2;       // softmax_scale * log2(e)
 };
 
@@ -159,7 +161,7 @@ struct P16Cursor {
 // Groups are counted beside the tiles where their number is the note's place
 // and the requests have different ones.
 __device__ __forceinline__ bool p16_counted(const P16Params& p) {
-  return p.notes != 0 && p.qsl != nullptr;
+  return p.notes > 0 && p.qsl != nullptr;
 }
 
 // The cursor at the 64 requests from r0 on.
@@ -307,7 +309,7 @@ __device__ __forceinline__ void p16_note(const P16Params& p, const P16Group& gr,
 }
 template <int D>
 __device__ __forceinline__ void p16_note_none(const P16Params& p, int wg) {
-  if (!p.notes) p16_cut<D>(p, wg)->slots_wg = 0u;
+  if (p.notes == 0) p16_cut<D>(p, wg)->slots_wg = 0u;
 }
 // The note before the first group's: how many groups there are. By the first
 // work-group, in any case.

@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
   __shared__ float s_m[kCrews], s_l[kCrews];
   const int col = threadIdx.x % kVec, crew = threadIdx.x / kVec;
   if (p16_counted(p) && blockIdx.x >= p16_cut<D>(p, 0)->slots_wg) return;
-  const P16Cut cut = *p16_cut<D>(p, p.notes ? 1 + blockIdx.x : blockIdx.x);
+  const P16Cut cut = *p16_cut<D>(p, p.notes > 0 ? 1 + blockIdx.x : blockIdx.x);
   const int slots = cut.slots_wg & ((1u << kP16CutShift) - 1);
   const int wg = cut.slots_wg >> kP16CutShift;
   if (slots == 0) return;
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
 template <int D, bool kF16>
 void combine(const P16Params& p, bool wide, dim3 grid, hipStream_t stream) {
   if (wide) p16_combine<D, kF16, kP16WideRows, 256><<<grid, 256, 0, stream>>>(p);
-  else if (p.notes) p16_combine<D, kF16, kP16RowsRows, 512><<<grid, 512, 0, stream>>>(p);
+  else if (p.notes > 0) p16_combine<D, kF16, kP16RowsRows, 512><<<grid, 512, 0, stream>>>(p);
   else p16_combine<D, kF16, kP16RowsRows, 256><<<grid, 256, 0, stream>>>(p);
 }
 
@@ -119,7 +119,7 @@ void combine(const P16Params& p, bool wide, dim3 grid, hipStream_t stream) {
 
 hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
                                      int y, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.notes ? p.notes : p.num_wg), static_cast<unsigned>(y));
+  const dim3 grid(static_cast<unsigned>(p.notes > 0 ? p.notes : p.num_wg), static_cast<unsigned>(y));
   switch (head_size) {
     case 64: f16 ? combine<64, true>(p, wide, grid, stream) : combine<64, false>(p, wide, grid, stream); break;
     case 256: f16 ? combine<256, true>(p, wide, grid, stream) : combine<256, false>(p, wide, grid, stream); break;

@@ -13,7 +13,9 @@
 namespace pa {
 namespace {
 
-// Slots per group up to which the combine is cheap.
+// Slots per group up to which a larger team pays (one request to 128k keys, 32q /
+// 8kv of 128: 96.6, 86.8 and 83.6 us for teams of 1, 2 and 4, which has 128; the
+// join takes 4.6 to 4.8).
 constexpr int64_t kMostSlots = 128;
 
 bool rows_aligned(const void* p, int64_t a, int64_t b) {
@@ -41,13 +43,31 @@ int32_t team_of(const P16Params& p, int32_t cus) {
   return team;
 }
 
-// Work-groups per compute unit of the 16-row kernel. One, four waves, reads
-// the cache fastest (more streams at once cost the memory more than they
-// hide); where a work-group takes several groups, others fill the gaps between
-// them, as many as fit.
+// Work-groups of the 16-row kernel that a compute unit holds.
+int64_t resident_rows(int32_t head_size) { return head_size == 64 ? 3 : head_size == 128 ? 2 : 1; }
+
+// Its work-groups per compute unit where groups are cut. One, four waves, reads
+// the cache fastest: more streams at once cost the memory more than they hide
+// (64 requests to 32k keys at D = 128: 626 us with one, 646 with two, 652 with
+// three). Where a work-group takes several groups, others fill the gaps between
+// them, as many as fit (48 requests to 4k, 16 heads of 64 in HND pages: 92 us
+// with one, 78 with two, 76 with three).
 int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
-  const int64_t fit = head_size == 64 ? 3 : head_size == 128 ? 2 : 1;
-  return std::min(fit, std::max<int64_t>(1, groups / cus));
+  return std::min(resident_rows(head_size), std::max<int64_t>(1, groups / cus));
+}
+
+// Whether every group is left whole, so that there is nothing to join: where
+// all are short. Measured, whole call, cut and whole, 32q / 8kv of 128 (bounds
+// of 64, 256, 512 and 1,024 keys), requests of one token:
+//     8 requests  10.7, 6.5   11.5,  8.6   12.6, 12.0   15.1, 20.5 us
+//    64           11.9, 7.5   19.3, 14.8   25.7, 24.6   40.0, 44.2
+// of 1 to 64 tokens against so many states:
+//     8            8.5, 8.7   19.2, 12.8   25.4, 18.4   28.9, 29.5
+//    64           25.8, 25.9  51.1, 40.3   63.9, 60.9   94.7, 95.1
+// D = 64 is alike; at D = 256, with one work-group per compute unit, 8 requests
+// of one token take 12.7, 9.7 and 13.3, 14.4 at 64 and 256.
+bool whole_groups(int32_t head_size, int64_t span, bool wide, int64_t units, int32_t cus) {
+  return span <= (head_size == 256 ? 128 : 512) && (!wide || units <= 8 * cus);
 }
 
 }  // namespace
@@ -129,14 +149,20 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
   PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
   p.team = wide ? 1 : team_of(p, cus);
-  p.key_tile_log2 = wide ? 6 : 7 - (p.team >> 1);
-  p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
   // Bounds of the partition: groups of all requests, key tiles of one.
   const int64_t row_tiles = a.query_start_loc == nullptr
                                 ? a.num_reqs * ((p.group + bm - 1) / bm)
                                 : rows / bm + a.num_reqs;
   const int64_t span = p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + 15)
                                     : p.max_keys;
+  const int64_t units = row_tiles * a.num_kv_heads;
+  const bool whole = whole_groups(a.head_size, span, wide, units, cus);
+  if (whole)
+    while (p.team > 1 && units / p.team < resident_rows(a.head_size) * cus) p.team /= 2;
+  p.key_tile_log2 = wide ? 6 : 7 - (p.team >> 1);
+  if (whole)
+    while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
+  p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
   const int64_t key_tiles = std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
   const int64_t groups = a.query_start_loc == nullptr
                              ? a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team)
@@ -145,13 +171,17 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
              "the launch exceeds 2^31 tiles");
   const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : a.head_size == 64 ? 3 : 2) : rows_per_cu(a.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
-  if (groups <= p.num_wg) p.notes = static_cast<int32_t>(groups);
+  if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
+  p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
   const bool f16 = a.dtype == PTH_ATTN_F16, page16 = a.block_size % 16 == 0;
   hipError_t err = wide ? launch_p16_wide_kernel(p, f16, page16, a.head_size, stream)
                         : launch_p16_rows_kernel(p, f16, page16, a.head_size, stream);
+  // Work-groups of the join per note: a row or eight each, until the device is
+  // full (256 tokens against 4,096 states: 23 us with one, 8.3 with eight).
   const int32_t items = p.team * p.slot_rows;
-  const int32_t y = p.notes ? std::min(items, std::max(wide ? 4 : 1, (wide ? 8 : 2) * cus / p.notes)) : wide ? 4 : 1;
-  // A group of one tile is never cut.
+  const int32_t y = p.notes > 0 ? std::min(items, std::max(wide ? 4 : 1, (wide ? 8 : 2) * cus / p.notes))
+                    : wide      ? 4
+                                : 1;
   if (err == hipSuccess && key_tiles > 1)
     err = launch_p16_combine_kernel(p, f16, wide, a.head_size, y, stream);
   if (err != hipSuccess)

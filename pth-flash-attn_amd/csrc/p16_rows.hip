@@ -195,9 +195,9 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
 
     Walker<kPage16> w{p, p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride, gr.req.lo,
                       gr.req.len, u.head};
-    const int step = 1 << p.key_tile_log2;  // 32 x parts
-    const int k_end = min(gr.req.base + (gr.kt + take) * step, gr.req.len);
-    int k0 = gr.req.base + gr.kt * step + 32 * part;
+    const int step = 32 * parts;
+    const int k_end = min(gr.req.base + ((gr.kt + take) << p.key_tile_log2), gr.req.len);
+    int k0 = gr.req.base + (gr.kt << p.key_tile_log2) + 32 * part;
 
     // The page numbers are on their way while Q is read.
     int32_t first_entry[2] = {0, 0};
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void p16_rows
       chunk(std::false_type{});
     }
 
-    if (gr.kt == 0 && (!whole || p.notes)) {
+    if (gr.kt == 0 && (!whole || p.notes > 0)) {
       noted |= !whole;
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, begin, takers, !whole);
     }

@@ -208,17 +208,18 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       }
     };
 
-    const int t_end = len > 0 ? gr.kt + take : gr.kt;
+    const int t_begin = (gr.kt << p.key_tile_log2) / kKT;
+    const int t_end = (min((gr.kt + take) << p.key_tile_log2, len) + kKT - 1) / kKT;
     int buf = 0;
     // The last unit's reads of both buffers are done (its stores may be on
     // their way).
     lds_barrier();
     // Page numbers are read a tile before their loads.
     int32_t entry = 0;
-    if (gr.kt < t_end) {
-      entry = kPage16 ? ld_ro(table, page(gr.kt)) : 0;
-      load(gr.kt, 0, entry);
-      entry = kPage16 ? ld_ro(table, page(gr.kt + 1)) : 0;
+    if (t_begin < t_end) {
+      entry = kPage16 ? ld_ro(table, page(t_begin)) : 0;
+      load(t_begin, 0, entry);
+      entry = kPage16 ? ld_ro(table, page(t_begin + 1)) : 0;
     }
     u32x4 q[W::kQ];
     {
@@ -229,12 +230,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
         if (!live) q[j] = (u32x4){0u, 0u, 0u, 0u};
       }
     }
-    if (gr.kt == 0 && (!whole || p.notes)) {
+    if (gr.kt == 0 && (!whole || p.notes > 0)) {
       noted |= !whole;
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
-    for (int t = gr.kt; t < t_end; ++t, buf ^= 1) {
+    for (int t = t_begin; t < t_end; ++t, buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
       if (t + 1 < t_end) {

@@ -160,6 +160,22 @@ def test_cross_cut_units(D, dtype):
     assert torch.equal(got, cross(c, q, q_lens, D**-0.5))
 
 
+@pytest.mark.parametrize("bound", [64, 128, 129, 512, 513])
+@pytest.mark.parametrize("heads", [(2, 1), (16, 4)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_bounds_at_which_groups_stay_whole(bound, heads, D):
+    lens = [bound, 0, 1, bound - 1, 16, bound // 2] * 3
+    c = make_cache(lens, Hkv=heads[1], D=D, block=16, dtype=BF, seed=bound)
+    q = queries(len(lens), heads[0], D, BF, bound)
+    assert_close(decode(c, q, D**-0.5), *reference(q, c.keys, [1] * 18, D**-0.5, pair=True))
+    q_lens = [40, 3, 1, 0, 17, 130] * 3
+    q = queries(sum(q_lens), heads[0], D, BF, bound)
+    assert_close(cross(c, q, q_lens, D**-0.5), *reference(q, c.keys, q_lens, D**-0.5))
+    # A bound above the lengths: the same rows, another partition.
+    far = cross(c, q, q_lens, D**-0.5, max_len=20 * bound)
+    assert_close(far, *reference(q, c.keys, q_lens, D**-0.5))
+
+
 def test_cross_many_requests():
     gen = torch.Generator().manual_seed(11)
     lens = torch.randint(0, 200, (140,), generator=gen).tolist()
