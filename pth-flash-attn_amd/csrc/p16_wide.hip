@@ -14,6 +14,13 @@
 // piece, V's so that four consecutive rows' same four pieces lie on different
 // banks.
 //
+// Order of the keys. A group's tiles may be taken in any order, and the
+// work-groups of an XCD, which have different row tiles of the same few KV
+// heads, take them so that they read the same tile at about the same time:
+// after s tiles, a work-group is at tile s modulo the group's number. A whole
+// group starts there; of a cut one, the work-group that begins with the rest
+// takes the first tiles, and the one that ends with its beginning the last.
+//
 // Numerics. Scores, m, l and o are 32 bits; the running maximum moves only when
 // a score passes it by 2^kSlack, so most tiles rescale nothing. P is rounded
 // once to the inputs' type, as the output is: both errors are independent, and
@@ -123,6 +130,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
   int64_t at = p16_share(tiles, wg, takers);
   const int64_t end = p16_share(tiles, wg + 1, takers);
   bool noted = false;
+  uint32_t steps = 0;  // key tiles that this work-group has done
 
   while (at < end) {
     const P16Group gr = p16_locate<kBM>(p, cur, at, lane);
@@ -208,18 +216,33 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       }
     };
 
-    const int t_begin = (gr.kt << p.key_tile_log2) / kKT;
-    const int t_end = (min((gr.kt + take) << p.key_tile_log2, len) + kKT - 1) / kKT;
+    // The piece's 64-key tiles: `count` of the group's nt from `t_first` on,
+    // round its end. Which ones: see the top.
+    const int nt = (len + kKT - 1) / kKT;
+    const int count = len == 0 ? 0 : gr.req.n_kt == nt ? take : nt;
+    uint32_t t_first;
+    if (whole) {
+      t_first = nt > 0 ? steps % static_cast<uint32_t>(nt) : 0u;
+    } else if (gr.kt == 0) {
+      t_first = static_cast<uint32_t>(nt - take);
+    } else {
+      const int64_t start = at - gr.kt;
+      const int64_t cut = p16_share(tiles, p16_holder(tiles, start, takers) + 1, takers);
+      t_first = static_cast<uint32_t>(gr.kt - static_cast<int>(cut - start));
+    }
+    steps += static_cast<uint32_t>(count);
+    const int t0 = __builtin_amdgcn_readfirstlane(static_cast<int>(t_first));
+    auto after = [&](int t) { return t + 1 == nt ? 0 : t + 1; };
     int buf = 0;
     // The last unit's reads of both buffers are done (its stores may be on
     // their way).
     lds_barrier();
     // Page numbers are read a tile before their loads.
     int32_t entry = 0;
-    if (t_begin < t_end) {
-      entry = kPage16 ? ld_ro(table, page(t_begin)) : 0;
-      load(t_begin, 0, entry);
-      entry = kPage16 ? ld_ro(table, page(t_begin + 1)) : 0;
+    if (count > 0) {
+      entry = kPage16 ? ld_ro(table, page(t0)) : 0;
+      load(t0, 0, entry);
+      entry = kPage16 ? ld_ro(table, page(after(t0))) : 0;
     }
     u32x4 q[W::kQ];
     {
@@ -235,12 +258,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
-    for (int t = t_begin; t < t_end; ++t, buf ^= 1) {
+    for (int i = 0, t = t0, next = after(t0); i < count; ++i, t = next, next = after(next), buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
-      if (t + 1 < t_end) {
-        load(t + 1, buf ^ 1, entry);
-        entry = kPage16 ? ld_ro(table, page(t + 2)) : 0;
+      if (i + 1 < count) {
+        load(next, buf ^ 1, entry);
+        entry = kPage16 ? ld_ro(table, page(after(next))) : 0;
       }
       const char* kt = lds + buf * W::kBuf;
       const char* vt = kt + 2 * W::kBuf;
@@ -275,11 +298,11 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       // 32 j + l % 32.
       u32x4 vf[2][W::kO];
       auto read_v = [&](int i) {
-        const int t0 = 4 * h + ((lane & 15) >> 2);
+        const int r0 = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
         for (int j = 0; j < W::kO; ++j) {
           const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-          const char* a = vt + (16 * i + t0) * W::kRow + 16 * W::v_piece(t0, byte >> 4) + (byte & 15);
+          const char* a = vt + (16 * i + r0) * W::kRow + 16 * W::v_piece(r0, byte >> 4) + (byte & 15);
           const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
           vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
         }
