@@ -151,7 +151,10 @@ int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream) {
              "k_cache and v_cache must have 16-byte aligned rows");
   Write16Params w{};
   w.items = static_cast<int64_t>(a.num_tokens) * a.num_kv_heads;
-  PA_REQUIRE(w.items < 0x7fffffff, "num_tokens x num_kv_heads exceeds 2^31");
+  // A launch has at most 2^32 threads; one moves eight values.
+  PA_REQUIRE(w.items < 0x7fffffff && w.items * (a.head_size / 8) <= 0xffffff00,
+             "num_tokens x num_kv_heads must be less than 2^31, its product with head_size "
+             "2^35");
   w.key = static_cast<const char*>(a.key);
   w.value = static_cast<const char*>(a.value);
   w.s_k_tok = a.key_stride_token;

@@ -156,3 +156,25 @@ def test_writer_refusals(field, value, message):
     setattr(a, field, value)
     assert lib.write_kv16(a) == capi.PTH_ATTN_EINVAL
     assert message in lib.last_error()
+
+
+@needs_lib
+def test_tables_rows_that_overlap_are_refused():
+    lib = capi.AttnLib()
+    a, _keep = _tables()
+    a.block_table_row_stride = 3
+    assert lib.step_tables(a) == capi.PTH_ATTN_EINVAL
+    assert "rows of block_table must not overlap" in lib.last_error()
+
+
+@needs_lib
+@pytest.mark.parametrize(("head_size", "heads"), [(64, 128), (128, 64), (256, 32)])
+def test_writer_launch_bound(head_size, heads):
+    """2^22 tokens of 2^13 values: as many threads as a launch does not have."""
+    lib = capi.AttnLib()
+    kv = torch.zeros(1, 2, 1, heads, head_size, dtype=torch.bfloat16)
+    x, slots = torch.zeros(1, heads, head_size, dtype=torch.bfloat16), torch.zeros(1).long()
+    a = capi.write16_args(key=x, value=x, k_cache=kv[:, 0], v_cache=kv[:, 1], slot_mapping=slots)
+    a.num_tokens = 1 << 22
+    assert a.num_tokens * heads * head_size == 1 << 35
+    assert lib.write_kv16(a) == capi.PTH_ATTN_EINVAL and "2^35" in lib.last_error()
