@@ -216,6 +216,8 @@ int32_t launch_step_tables(const PthAttnTablesArgs& a, hipStream_t stream) {
   PA_REQUIRE(a.num_slots == 0 || a.slot_mapping, "slot_mapping must be non-NULL");
   PA_REQUIRE(a.num_reqs == 0 || a.block_table_width == 0 || a.block_table,
              "block_table must be non-NULL");
+  PA_REQUIRE(a.num_reqs <= 1 || a.block_table_row_stride >= a.block_table_width,
+             "the rows of block_table must not overlap");
   PA_REQUIRE(a.num_free == 0 || a.free_pages, "free_pages must be non-NULL");
   TablesParams p{};
   p.block_table = a.block_table;

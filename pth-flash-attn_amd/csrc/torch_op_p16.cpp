@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -58,6 +59,21 @@ Span span_of(const char* op, const Tensor& t) {
   OP_CHECK(n >= 0, "negative strides, or a byte extent that overflows int64");
   const auto p = n > 0 ? reinterpret_cast<uintptr_t>(t.data_ptr()) : 0;
   return {p, p + static_cast<uintptr_t>(n)};
+}
+// Whether two elements may share memory: a dimension steps within the reach of
+// those of smaller strides.
+bool overlaps_itself(const Tensor& t) {
+  const int64_t n = t.dim();
+  int64_t order[4] = {0, 1, 2, 3};
+  std::sort(order, order + n, [&](int64_t a, int64_t b) { return t.stride(a) < t.stride(b); });
+  int64_t reach = 1;
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t d = order[i];
+    if (t.size(d) <= 1) continue;
+    if (t.stride(d) < reach) return true;
+    reach = t.stride(d) * (t.size(d) - 1) + reach;
+  }
+  return false;
 }
 bool overlap(const Span& a, const Span& b) { return a.begin < b.end && b.begin < a.end; }
 
@@ -164,6 +180,7 @@ void attend(const char* op, const char* lens_name, const Tensor& out, const Tens
             int64_t max_len, double softmax_scale, const Tensor& ws, int64_t window) {
   check_attention(op, lens_name, out, q, k_cache, v_cache, block_table, lens, query_start_loc,
                   max_len, softmax_scale, ws, window);
+  OP_CHECK(!overlaps_itself(out), "out must not overlap itself");
   const Span s_out = span_of(op, out), s_ws = span_of(op, ws), s_q = span_of(op, q);
   OP_CHECK(!overlap(s_out, s_ws), "out and ws must not overlap");
   OP_CHECK(!overlap(s_ws, s_q), "ws must not overlap an input");
@@ -177,7 +194,7 @@ void attend(const char* op, const char* lens_name, const Tensor& out, const Tens
     OP_CHECK(!overlap(s_out, s), "out must not overlap an input");
     OP_CHECK(!overlap(s_ws, s), "ws must not overlap an input");
   }
-  OP_CHECK(fits32(q.size(0)) && fits32(k_cache.size(0)) && fits32(k_cache.size(1)) &&
+  OP_CHECK(fits32(q.size(0)) && fits32(q.size(1)) && fits32(k_cache.size(0)) && fits32(k_cache.size(1)) &&
                fits32(block_table.size(1)),
            "a size exceeds int32");
   check_on_gpu(op, q);
@@ -263,6 +280,8 @@ void reshape_and_cache_16bit(const Tensor& key, const Tensor& value, const Tenso
            "slot_mapping must be contiguous int64 [T]");
   for (const Tensor* t : {&value, &k_cache, &v_cache, &slot_mapping})
     OP_CHECK(t->device() == key.device(), "all tensors must be on the device of key");
+  OP_CHECK(!overlaps_itself(k_cache) && !overlaps_itself(v_cache),
+           "k_cache and v_cache must not overlap themselves");
   const Span s_k = span_of(op, k_cache), s_v = span_of(op, v_cache);
   for (const Tensor* t : {&key, &value, &slot_mapping}) {
     const Span s = span_of(op, *t);
@@ -320,6 +339,7 @@ void build_step_tables(const Tensor& block_table, const Tensor& slot_mapping,
                block_table.stride(1) == 1 && block_table.size(0) >= R,
            "block_table must be int32 [>= num_reqs, max_blocks] with stride 1 in its last "
            "dimension");
+  OP_CHECK(!overlaps_itself(block_table), "the rows of block_table must not overlap");
   OP_CHECK(slot_mapping.dim() == 1 && slot_mapping.scalar_type() == ScalarType::Long &&
                slot_mapping.is_contiguous(),
            "slot_mapping must be contiguous int64 [T]");

@@ -42,6 +42,18 @@ def _int32_vector(t: torch.Tensor, n: int | None = None) -> bool:
             and (n is None or t.shape[0] == n))
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements may share memory: a dimension steps within the
+    reach of those of smaller strides."""
+    reach = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size > 1:
+            if stride < reach:
+                return True
+            reach += stride * (size - 1)
+    return False
+
+
 def _check_attention(op: str, lens_name: str, out: torch.Tensor, q: torch.Tensor,
                      k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                      lens: torch.Tensor, query_start_loc: torch.Tensor | None, max_len: int,
@@ -89,6 +101,7 @@ def _check_attention(op: str, lens_name: str, out: torch.Tensor, q: torch.Tensor
     if query_start_loc is not None:
         others.append(query_start_loc)
     check(all(t.device == q.device for t in others), "all tensors must be on the device of q")
+    check(not _overlaps_itself(out), "out must not overlap itself")
 
 
 def paged_decode_fwd_fake(out, q, k_cache, v_cache, block_table, seq_lens, max_seq_len,
@@ -129,6 +142,8 @@ def reshape_and_cache_16bit_fake(key, value, k_cache, v_cache, slot_mapping) -> 
           "slot_mapping must be contiguous int64 [T]")
     check(all(t.device == key.device for t in (value, k_cache, v_cache, slot_mapping)),
           "all tensors must be on the device of key")
+    check(not _overlaps_itself(k_cache) and not _overlaps_itself(v_cache),
+          "k_cache and v_cache must not overlap themselves")
 
 
 def build_step_tables_fake(block_table, slot_mapping, seq_lens, query_start_loc, pool_out,
@@ -146,6 +161,7 @@ def build_step_tables_fake(block_table, slot_mapping, seq_lens, query_start_loc,
           and block_table.stride(1) == 1 and block_table.shape[0] >= R,
           "block_table must be int32 [>= num_reqs, max_blocks] with stride 1 in its last "
           "dimension")
+    check(not _overlaps_itself(block_table), "the rows of block_table must not overlap")
     check(slot_mapping.dim() == 1 and slot_mapping.dtype == torch.int64
           and slot_mapping.is_contiguous(), "slot_mapping must be contiguous int64 [T]")
     check(block_size >= 1, "block_size must be >= 1, got ", block_size)
@@ -229,7 +245,10 @@ def paged_decode_fwd(
 
     ``q`` / ``out`` [R, Hq, D]; query head h reads KV head h // (Hq / Hkv). The
     token sees the last ``window`` (all, if 0) of the request's ``seq_lens[r]``
-    keys, its own among them; a request without keys gives zeros.
+    keys, its own among them; a request without keys gives zeros. What a page
+    holds outside of these keys reaches no output. A NaN or a score of +inf
+    makes its row NaN, and an infinite value its column infinite or NaN.
+    ``out`` may be ``q`` itself; other than that they share no memory.
     ``max_seq_len`` bounds the lengths (longer ones are cut there, and at the
     block table's reach). ``ws`` is workspace of
     ``planner.paged16_workspace_floats`` floats; it holds nothing between calls,

@@ -106,6 +106,18 @@ def test_overlaps_are_refused(call):
         call({**a, "ws": a["lens"].view(torch.float32)})
 
 
+@pytest.mark.parametrize("call", [_decode, _cross])
+def test_out_that_overlaps_itself_is_refused(call):
+    a = _args()
+    for bad in (a["out"][:1].expand_as(a["q"]), a["out"][:, :1].expand_as(a["q"]),
+                torch.zeros(512, dtype=BF).as_strided(a["out"].shape, (128, 64, 1))):
+        for fake in (False, True):
+            with pytest.raises(RuntimeError, match="out must not overlap itself"):
+                call({**a, "out": bad}, fake=fake)
+    turned = torch.zeros(4, 2, 64, dtype=BF).transpose(0, 1)  # heads outside, as good
+    call({**a, "out": turned}, fake=True)
+
+
 def test_views_of_a_cache():
     kv = torch.arange(2 * 2 * 16 * 3 * 64, dtype=torch.float32).to(BF).view(2, 2, 3, 16, 64)
     k, v = paged16_views(kv, layout="HND")

@@ -411,6 +411,19 @@ def test_compile_traces_and_opcheck():
                           test_utils=("test_schema", "test_faketensor"))
 
 
+@pytest.mark.parametrize("n", [1, 24, 200])
+def test_out_is_q(n):
+    """Whole and cut units, one and several waves of a unit, in place."""
+    for lens, block in (([700, 33, 0, 129], 16), ([9000, 33, 0, 4000], 48)):
+        c = make_cache(lens, Hkv=2, D=128, block=block, dtype=BF, seed=n)
+        q = queries(4 * n, 8, 128, BF, n)
+        both = q.clone()
+        if n == 1:
+            assert torch.equal(decode(c, both, 0.1, out=both), decode(c, q, 0.1))
+        else:
+            assert torch.equal(cross(c, both, [n] * 4, 0.1, out=both), cross(c, q, [n] * 4, 0.1))
+
+
 def test_empty_batches():
     c = make_cache([10], Hkv=1, D=64, block=16, dtype=BF, seed=24)
     q = queries(0, 4, 64, BF, 24)

@@ -210,3 +210,12 @@ def test_overlaps_are_refused():
     args["seq_lens"], args["query_start_loc"] = both[:3], both[2:6]
     with pytest.raises(RuntimeError, match="the outputs must not overlap each other"):
         ops.build_step_tables(**args)
+
+
+@needs_op
+def test_rows_that_overlap_are_refused():
+    args = _cpu_args()
+    args["block_table"] = torch.zeros(1, 4, dtype=torch.int32).expand(3, 4)
+    for f in (ops.build_step_tables, ops.ops16.build_step_tables_fake):
+        with pytest.raises(RuntimeError, match="the rows of block_table must not overlap"):
+            f(**args)

@@ -107,3 +107,13 @@ def test_unaligned_cache_is_refused():
     x = torch.zeros(1, 1, 64, dtype=BF, device="cuda")
     with pytest.raises(RuntimeError, match="16-byte aligned rows"):
         ops.reshape_and_cache_16bit(x, x, kv[:, 0], kv[:, 1], torch.tensor([1], device="cuda"))
+
+
+@needs_op
+def test_cache_that_overlaps_itself_is_refused():
+    args = _cpu()
+    for bad in (dict(k_cache=args["k_cache"][:, :, :1].expand_as(args["k_cache"])),
+                dict(v_cache=args["v_cache"][:1].expand_as(args["v_cache"]))):
+        for f in (ops.reshape_and_cache_16bit, ops.ops16.reshape_and_cache_16bit_fake):
+            with pytest.raises(RuntimeError, match="must not overlap themselves"):
+                f(**{**args, **bad})
