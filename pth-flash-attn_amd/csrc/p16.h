@@ -262,7 +262,8 @@ __device__ __forceinline__ int64_t p16_share(int64_t tiles, int w, int num_wg) {
 __device__ __forceinline__ int p16_holder(int64_t tiles, int64_t at, int num_wg) {
   const uint64_t x = static_cast<uint64_t>(at + 1) * static_cast<uint32_t>(num_wg) +
                      static_cast<uint64_t>(tiles) - 1;
-  if (x >> 32 == 0) return static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(tiles)) - 1;
+  if (x >> 32 == 0)
+    return static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(tiles)) - 1;
   return static_cast<int>(x / static_cast<uint64_t>(tiles)) - 1;
 }
 
@@ -299,9 +300,10 @@ template <int D>
 __device__ __forceinline__ void p16_note(const P16Params& p, const P16Group& gr, int wg,
                                          int64_t tiles, int64_t first, int takers, bool cut) {
   P16Cut c = {0u, gr.req.q0, gr.req.rows, gr.group};
-  if (cut)
-    c.slots_wg = static_cast<uint32_t>(p16_holder(tiles, first + gr.req.n_kt - 1, takers) - wg + 1) |
-                 static_cast<uint32_t>(wg) << kP16CutShift;
+  if (cut) {
+    const int last = p16_holder(tiles, first + gr.req.n_kt - 1, takers);
+    c.slots_wg = static_cast<uint32_t>(last - wg + 1) | static_cast<uint32_t>(wg) << kP16CutShift;
+  }
   // Starts that run backwards can make more groups than there are notes.
   const int number = (p16_counted(p) ? gr.number : gr.r * gr.req.n_gr) + gr.group;
   if (p.notes == 0 || static_cast<uint32_t>(number) < static_cast<uint32_t>(p.notes))

@@ -1,10 +1,16 @@
 // p16_combine.hip -- joins the groups that the partition of p16.h cut:
-// work-group (i, y) the rows y, y + gridDim.y ... of the group of note i. Per row M = max m_s, L = sum l_s 2^(m_s - M),
-// out = sum o_s 2^(m_s - M) / L, the slots s in an order that the sizes fix.
+// work-group (i, y) the rows y, y + gridDim.y ... of the group of note i. Per row
+//   M = max m_s, L = sum l_s 2^(m_s - M), out = sum o_s 2^(m_s - M) / L,
+// the slots s in an order that the sizes fix.
 //
-// A crew of D / 4 lanes reads a row, four columns a lane. With few slots each
-// crew joins a row by itself; with many they share one row's slots and join in
-// LDS.
+// A crew of D / 4 lanes reads a row, four columns a lane. With few slots, or
+// twice as many rows, each crew joins a row by itself; otherwise they share one
+// row's slots and join in LDS (64 rows of 17 slots, whole call of 8 requests to
+// 6,000 states: 41.0 us alone, 46.4 shared).
+//
+// Bound: latency (a note, then slots that the launch before wrote). One request
+// to 128k keys, 128 slots of 4 rows: 4.6 us; 64 requests to 32k keys 5.1. Of
+// 128-row units it is their bytes: 4 long prompts, up to 68 MB of slots, 20 us.
 
 #include "attn_device.h"
 #include "p16.h"
@@ -37,8 +43,8 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
   x.n_rt = (cut.rows + kBM - 1) / kBM;
   const int first = cut.group * p.team;
   const int subs = min(p.team, p.num_kv_heads * x.n_rt - first);
-  const bool alone = slots <= 8;
   const int items = subs * p.slot_rows;  // rows of the group, as a slot holds them
+  const bool alone = slots <= max(8, items / 2);
   const int step = alone ? 1 : kCrews;
   for (int i = alone ? crew + kCrews * static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.y);
        i < items; i += (alone ? kCrews : 1) * static_cast<int>(gridDim.y)) {
@@ -109,21 +115,27 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
 }
 
 template <int D, bool kF16>
-void combine(const P16Params& p, bool wide, dim3 grid, hipStream_t stream) {
+void combine_of(const P16Params& p, bool wide, dim3 grid, hipStream_t stream) {
   if (wide) p16_combine<D, kF16, kP16WideRows, 256><<<grid, 256, 0, stream>>>(p);
   else if (p.notes > 0) p16_combine<D, kF16, kP16RowsRows, 512><<<grid, 512, 0, stream>>>(p);
   else p16_combine<D, kF16, kP16RowsRows, 256><<<grid, 256, 0, stream>>>(p);
+}
+template <int D>
+void combine(const P16Params& p, bool f16, bool wide, dim3 grid, hipStream_t stream) {
+  if (f16) combine_of<D, true>(p, wide, grid, stream);
+  else combine_of<D, false>(p, wide, grid, stream);
 }
 
 }  // namespace
 
 hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
                                      int y, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.notes > 0 ? p.notes : p.num_wg), static_cast<unsigned>(y));
+  const dim3 grid(static_cast<unsigned>(p.notes > 0 ? p.notes : p.num_wg),
+                  static_cast<unsigned>(y));
   switch (head_size) {
-    case 64: f16 ? combine<64, true>(p, wide, grid, stream) : combine<64, false>(p, wide, grid, stream); break;
-    case 256: f16 ? combine<256, true>(p, wide, grid, stream) : combine<256, false>(p, wide, grid, stream); break;
-    default: f16 ? combine<128, true>(p, wide, grid, stream) : combine<128, false>(p, wide, grid, stream);
+    case 64: combine<64>(p, f16, wide, grid, stream); break;
+    case 256: combine<256>(p, f16, wide, grid, stream); break;
+    default: combine<128>(p, f16, wide, grid, stream);
   }
   return hipGetLastError();
 }

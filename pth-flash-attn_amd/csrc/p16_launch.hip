@@ -17,6 +17,14 @@ namespace {
 // 8kv of 128: 96.6, 86.8 and 83.6 us for teams of 1, 2 and 4, which has 128; the
 // join takes 4.6 to 4.8).
 constexpr int64_t kMostSlots = 128;
+// Key rows that a work-group reads for each row of sums in its slots, below
+// which the slots' bytes cost more than a larger team's reads save. Whole call,
+// teams of 1, 2 and 4 (with 4: the ratio), 4 tokens per request, 32q / 8kv of 128:
+//     8 requests to 1,500 states (2.9)  18.1, 18.1, 20.1 us
+//    16                          (5.9)  27.0, 25.6, 27.0
+//     8             6,000       (11.7)  43.3, 40.5, 41.0
+//     2            30,000       (14.6)  53.4, 49.2, 48.5
+constexpr int64_t kLeastReads = 8;
 
 bool rows_aligned(const void* p, int64_t a, int64_t b) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
@@ -33,27 +41,30 @@ CacheStream stream_of(const PthAttnStream& s) {
 
 // Units that a work-group of the 16-row kernel computes side by side, one for
 // each wave or pair of waves: neighbours in the cache (the KV heads of NHD
-// pages), or row tiles of the same keys, as long as enough groups remain.
-int32_t team_of(const P16Params& p, int32_t cus) {
+// pages), or row tiles of the same keys, as long as enough groups remain and,
+// where they are cut, their slots stay small beside the keys. `rows`: a unit's.
+int32_t team_of(const P16Params& p, int64_t span, int64_t rows, bool whole, int32_t cus) {
   const int64_t n_rt = p.qsl ? 1 : (p.group + kP16RowsRows - 1) / kP16RowsRows;
+  const int64_t units = p.num_reqs * (p.num_kv_heads * n_rt);
   const bool heads_adjacent = p.k.s_head < p.k.s_slot && p.v.s_head < p.v.s_slot;
   const int64_t beside = heads_adjacent ? p.num_kv_heads * n_rt : n_rt;
   int32_t team = beside % 4 == 0 ? 4 : beside % 2 == 0 ? 2 : 1;
-  while (team > 1 && p.num_reqs * p.num_kv_heads * n_rt / team * kMostSlots < cus) team /= 2;
+  while (team > 1 && units / team * kMostSlots < cus) team /= 2;
+  while (!whole && team > 1 && units * span < kLeastReads * 2 * team * rows * cus) team /= 2;
   return team;
 }
 
-// Work-groups of the 16-row kernel that a compute unit holds.
-int64_t resident_rows(int32_t head_size) { return head_size == 64 ? 3 : head_size == 128 ? 2 : 1; }
+// Work-groups of either attention kernel that a compute unit holds.
+int64_t resident(int32_t head_size) { return head_size == 64 ? 3 : head_size == 128 ? 2 : 1; }
 
-// Its work-groups per compute unit where groups are cut. One, four waves, reads
-// the cache fastest: more streams at once cost the memory more than they hide
-// (64 requests to 32k keys at D = 128: 626 us with one, 646 with two, 652 with
-// three). Where a work-group takes several groups, others fill the gaps between
-// them, as many as fit (48 requests to 4k, 16 heads of 64 in HND pages: 92 us
-// with one, 78 with two, 76 with three).
+// The 16-row kernel's work-groups per compute unit where groups are cut. One,
+// four waves, reads the cache fastest: more streams at once cost the memory more
+// than they hide (64 requests to 32k keys at D = 128: 626 us with one, 646 with
+// two, 652 with three). Where a work-group takes several groups, others fill the
+// gaps between them, as many as fit (48 requests to 4k, 16 heads of 64 in HND
+// pages: 92 us with one, 78 with two, 76 with three).
 int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
-  return std::min(resident_rows(head_size), std::max<int64_t>(1, groups / cus));
+  return std::min(resident(head_size), std::max<int64_t>(1, groups / cus));
 }
 
 // Whether every group is left whole, so that there is nothing to join: where
@@ -143,12 +154,16 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   p.window = a.window;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
 
+  // More rows than the small kernel's tile of a KV head: the other, whose tiles
+  // eight times as many rows share (17 rows per request, 16q / 16kv of 64 against
+  // 1,500 states: 1, 8 and 64 requests 11.0, 19.5 and 93 us, the small one's row
+  // tiles 13.6, 22.6 and 120; 16 rows 12.0, 17.1 and 76 with the small one, and
+  // 10.8, 19.5 and 91 with the other).
   const bool wide = a.query_start_loc != nullptr &&
                     static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
   const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
   PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
-  p.team = wide ? 1 : team_of(p, cus);
   // Bounds of the partition: groups of all requests, key tiles of one.
   const int64_t row_tiles = a.query_start_loc == nullptr
                                 ? a.num_reqs * ((p.group + bm - 1) / bm)
@@ -157,19 +172,23 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
                                     : p.max_keys;
   const int64_t units = row_tiles * a.num_kv_heads;
   const bool whole = whole_groups(a.head_size, span, wide, units, cus);
+  const int64_t tokens = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
+  p.team = wide ? 1 : team_of(p, span, std::min(bm, tokens * p.group), whole, cus);
   if (whole)
-    while (p.team > 1 && units / p.team < resident_rows(a.head_size) * cus) p.team /= 2;
+    while (p.team > 1 && units / p.team < resident(a.head_size) * cus) p.team /= 2;
   p.key_tile_log2 = wide ? 6 : 7 - (p.team >> 1);
   if (whole)
     while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
   p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
-  const int64_t key_tiles = std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
-  const int64_t groups = a.query_start_loc == nullptr
-                             ? a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team)
-                             : row_tiles * a.num_kv_heads / p.team + (p.team > 1 ? a.num_reqs : 0);
-  PA_REQUIRE(row_tiles * a.num_kv_heads < INT32_MAX / key_tiles,
-             "the launch exceeds 2^31 tiles");
-  const int64_t fill = cus * (wide ? (a.head_size == 256 ? 1 : a.head_size == 64 ? 3 : 2) : rows_per_cu(a.head_size, groups, cus));
+  const int64_t key_tiles =
+      std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
+  const int64_t groups =
+      a.query_start_loc == nullptr
+          ? a.num_reqs * ((row_tiles / a.num_reqs * a.num_kv_heads + p.team - 1) / p.team)
+          : units / p.team + (p.team > 1 ? a.num_reqs : 0);
+  PA_REQUIRE(units < INT32_MAX / key_tiles, "the launch exceeds 2^31 tiles");
+  const int64_t fill =
+      cus * (wide ? resident(a.head_size) : rows_per_cu(a.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
   if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
   p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
@@ -178,10 +197,11 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
                         : launch_p16_rows_kernel(p, f16, page16, a.head_size, stream);
   // Work-groups of the join per note: a row or eight each, until the device is
   // full (256 tokens against 4,096 states: 23 us with one, 8.3 with eight).
-  const int32_t items = p.team * p.slot_rows;
-  const int32_t y = p.notes > 0 ? std::min(items, std::max(wide ? 4 : 1, (wide ? 8 : 2) * cus / p.notes))
-                    : wide      ? 4
-                                : 1;
+  // Of 16-row units, four times as many as compute units (4 tokens of 8 requests
+  // against 1,500 states, D = 256: whole call 29.1 us with twice, 25.7).
+  const int32_t items = p.team * p.slot_rows, least = wide ? 4 : 1;
+  const int32_t y =
+      p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
   if (err == hipSuccess && key_tiles > 1)
     err = launch_p16_combine_kernel(p, f16, wide, a.head_size, y, stream);
   if (err != hipSuccess)

@@ -27,6 +27,21 @@
 // together sqrt(2) of the output's own; l sums the rounded P, by dot products
 // of its pairs. In fp16, whose range is short, P is scaled by 2^12: weights down
 // to 2^-26 of a row's largest keep all 11 bits.
+//
+// Bound: the matrix cores and the softmax's VALU work, which one SIMD's two
+// waves overlap, at the clock that the power leaves. 4 prompts of 1,500 to 2,048
+// rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11 operations):
+// 780 us, 860 TFLOP/s (a library's 8192^3 product: 1,205); 852 before the keys'
+// order above (fabric reads 3.95 GB, now 0.52). MFMA is busy 48 % of the time,
+// VALU 42 %, without bank conflicts, at 1.83 GHz; inputs of zeros, which draw less
+// power, take 495 us where others take 620. No faster, and so not here (4 x 2,048
+// rows against 4,096 keys, shortest of 20 calls 605 us): 256 rows in two halves
+// of four waves that take turns at the matrix cores (727), a tile's PV products
+// between the next one's softmax (602), wave priorities, a loop of two tiles
+// with fixed buffers, staggered starts, buffer loads (597, but D = 256 2 %
+// slower), waves without rows that leave out the products (short prompts: 41 us
+// either way).
+// D = 64 runs at 680 TFLOP/s (its softmax is twice the share), D = 256 at 670.
 
 #include "attn_device.h"
 #include "p16.h"
@@ -191,10 +206,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
           for (int i = 0; i < W::kLoads; ++i) {
             const int t16 = (64 * i + lane) / W::kPieces, c = (64 * i + lane) % W::kPieces;
             const uint32_t from = min(t16, len - 1 - kb);
-            dma16(ks + (__umul24(from, static_cast<uint32_t>(p.k.s_slot)) + 16 * W::k_piece(t16, c)),
-                  kd + 1024 * i);
-            dma16(vs + (__umul24(from, static_cast<uint32_t>(p.v.s_slot)) + 16 * W::v_piece(t16, c)),
-                  vd + 1024 * i);
+            const uint32_t k_row = __umul24(from, static_cast<uint32_t>(p.k.s_slot));
+            const uint32_t v_row = __umul24(from, static_cast<uint32_t>(p.v.s_slot));
+            dma16(ks + (k_row + 16 * W::k_piece(t16, c)), kd + 1024 * i);
+            dma16(vs + (v_row + 16 * W::v_piece(t16, c)), vd + 1024 * i);
           }
         }
       } else {
@@ -258,7 +273,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
-    for (int i = 0, t = t0, next = after(t0); i < count; ++i, t = next, next = after(next), buf ^= 1) {
+    for (int i = 0, t = t0, next = after(t0); i < count;
+         ++i, t = next, next = after(next), buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
       if (i + 1 < count) {
@@ -302,7 +318,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
 #pragma unroll
         for (int j = 0; j < W::kO; ++j) {
           const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-          const char* a = vt + (16 * i + r0) * W::kRow + 16 * W::v_piece(r0, byte >> 4) + (byte & 15);
+          const char* a =
+              vt + (16 * i + r0) * W::kRow + 16 * W::v_piece(r0, byte >> 4) + (byte & 15);
           const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
           vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
         }

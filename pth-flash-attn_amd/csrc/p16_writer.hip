@@ -5,7 +5,8 @@
 // each. Rows of the source that are not on 16-byte addresses are read value by
 // value.
 //
-// Bound: HBM.
+// Bound: HBM. 16,384 tokens of 8 heads of 128 from fp32 (201 MB): 40.5 us, 4.97
+// TB/s, a large copy's rate (4.91). 64 tokens of bf16: 2.6 us, a launch.
 
 #include <hip/hip_runtime.h>
 
@@ -179,7 +180,8 @@ int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream) {
   }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess)
-    return fail(PTH_ATTN_ECUDA, std::string("16-bit cache writer launch: ") + hipGetErrorString(err));
+    return fail(PTH_ATTN_ECUDA,
+                std::string("16-bit cache writer launch: ") + hipGetErrorString(err));
   return PTH_ATTN_OK;
 }
 

@@ -10,10 +10,13 @@
 // pages and of the requests' own outputs: one launch, no atomics in memory.
 // Sums saturate at kCap, above every bound that they are compared with.
 //
-// Bound: latency, of three dependent reads (lengths, page, and the launch).
+// Bound: latency, of the launch and two dependent reads (lengths, page), with the
+// steps of a search in LDS between them: 8 requests of one token 3.2 us, 1,024
+// requests with 33,000 new tokens 7.3 us.
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <string>
 
 #include "attn_stream.h"
@@ -178,7 +181,8 @@ __global__ __launch_bounds__(256) void step_tables(const TablesParams p) {
       const uint32_t first = s_first[i], k = x - before;
       if (first == kRefused) continue;
       const uint32_t have = p.bs_div.div(s_ctx[i] + bs - 1);
-      p.block_table[static_cast<int64_t>(r0 + i) * p.bt_stride + have + k] = p.free_pages[first + k];
+      p.block_table[static_cast<int64_t>(r0 + i) * p.bt_stride + have + k] =
+          p.free_pages[first + k];
     }
     tokens = tok_end;
     pages = page_end;
@@ -235,8 +239,8 @@ int32_t launch_step_tables(const PthAttnTablesArgs& a, hipStream_t stream) {
   p.width = a.block_table_width;
   p.num_reqs = a.num_reqs;
   p.bs_div = Div32::make(static_cast<uint32_t>(a.block_size));
-  const dim3 grid(static_cast<unsigned>((a.num_slots + kTokens - 1) / kTokens + (a.num_slots == 0))),
-      block(256);
+  const int64_t work_groups = (a.num_slots + kTokens - 1) / kTokens;
+  const dim3 grid(static_cast<unsigned>(std::max<int64_t>(work_groups, 1))), block(256);
   if (a.num_reqs <= 256) hipLaunchKernelGGL(step_tables<1>, grid, block, 0, stream, p);
   else hipLaunchKernelGGL(step_tables<4>, grid, block, 0, stream, p);
   const hipError_t err = hipGetLastError();

@@ -194,8 +194,8 @@ void attend(const char* op, const char* lens_name, const Tensor& out, const Tens
     OP_CHECK(!overlap(s_out, s), "out must not overlap an input");
     OP_CHECK(!overlap(s_ws, s), "ws must not overlap an input");
   }
-  OP_CHECK(fits32(q.size(0)) && fits32(q.size(1)) && fits32(k_cache.size(0)) && fits32(k_cache.size(1)) &&
-               fits32(block_table.size(1)),
+  OP_CHECK(fits32(q.size(0)) && fits32(q.size(1)) && fits32(k_cache.size(0)) &&
+               fits32(k_cache.size(1)) && fits32(block_table.size(1)),
            "a size exceeds int32");
   check_on_gpu(op, q);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());

@@ -153,8 +153,9 @@ def build_step_tables_fake(block_table, slot_mapping, seq_lens, query_start_loc,
     check(_int32_vector(context_lens), "context_lens must be contiguous int32 [n]")
     R = context_lens.shape[0]
     for t, n, name in ((query_lens, R, "query_lens"), (seq_lens, R, "seq_lens"),
-                       (query_start_loc, R + 1, "query_start_loc"), (free_pages, None, "free_pages"),
-                       (pool_in, 2, "pool_in"), (pool_out, 2, "pool_out")):
+                       (query_start_loc, R + 1, "query_start_loc"),
+                       (free_pages, None, "free_pages"), (pool_in, 2, "pool_in"),
+                       (pool_out, 2, "pool_out")):
         check(_int32_vector(t, n), name, " must be contiguous int32 [", "n" if n is None else n,
               "]")
     check(block_table.dim() == 2 and block_table.dtype == torch.int32

@@ -160,6 +160,19 @@ def test_cross_cut_units(D, dtype):
     assert torch.equal(got, cross(c, q, q_lens, D**-0.5))
 
 
+@pytest.mark.parametrize("longest", [700, 1500, 2200, 6000])
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_cross_few_rows_of_long_states(longest, layout):
+    """Full tiles of 16 rows, cut: one, two and four units side by side, joined
+    row by row and slot by slot."""
+    lens, q_lens = [longest, longest // 2, 33, 0, longest - 1, 1, 17, 600], [4, 1, 3, 4, 4, 2, 4, 0]
+    c = make_cache(lens, Hkv=8, D=128, block=16, dtype=BF, seed=longest, layout=layout)
+    q = queries(sum(q_lens), 32, 128, BF, 13)
+    got = cross(c, q, q_lens, 0.09)
+    assert last_kernel() == "p16_rows"
+    assert_close(got, *reference(q, c.keys, q_lens, 0.09, pair=True))
+
+
 @pytest.mark.parametrize("bound", [64, 128, 129, 512, 513])
 @pytest.mark.parametrize("heads", [(2, 1), (16, 4)])
 @pytest.mark.parametrize("D", [64, 128, 256])
