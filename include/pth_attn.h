@@ -192,7 +192,8 @@ typedef struct PthAttnWriteArgs {
  * of tokens that belong to no request are not written. kv_lens are brought
  * into [0, max_kv_len] and to the block table's reach, query_start_loc into
  * [0, num_tokens], and a page number outside the cache is read as page 0:
- * nothing out of bounds is touched whatever these tensors hold. */
+ * nothing out of bounds is touched whatever these tensors hold. out may be q
+ * itself; other than that it shares no memory with another tensor. */
 typedef struct PthAttnP16Args {
   int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
   int32_t struct_bytes; /* = sizeof(PthAttnP16Args) */
@@ -221,7 +222,7 @@ typedef struct PthAttnP16Args {
   int32_t num_reqs;
   int32_t num_tokens;
   int32_t num_q_heads;
-  int32_t max_query_len; /* of a request (a choice of kernel only) */
+  int32_t max_query_len; /* of a request (a choice of kernel and split only) */
   int32_t window;        /* 0 = none */
   float softmax_scale;
   float* ws; /* pth_attn_paged16_workspace_floats(head_size) floats */
@@ -394,7 +395,8 @@ int32_t pth_attn_write16_args_bytes(void);
  *     token t, -1 for one of a refused request, behind a negative page number,
  *     or behind the last request
  *   pool_out = {pool_in[0] + pages taken, requests refused}
- * No output may overlap an input (block_table is both). */
+ * No output may overlap an input (block_table is both) or another output, and
+ * block_table's rows do not overlap. */
 int32_t pth_attn_step_tables(const PthAttnTablesArgs* args, void* stream);
 int32_t pth_attn_tables_args_bytes(void);
 

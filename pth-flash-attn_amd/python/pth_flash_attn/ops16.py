@@ -274,7 +274,7 @@ def cross_attn_fwd(
     ``q`` / ``out`` [T, Hq, D]: request r's tokens are ``query_start_loc[r]`` to
     ``query_start_loc[r + 1]``, and each sees all ``encoder_lens[r]`` keys
     (zeros where there are none). Rows that belong to no request are left as
-    they were. ``max_query_len`` chooses the kernel (any value is correct);
+    they were. ``max_query_len`` chooses kernel and split (any value is correct);
     ``max_encoder_len``, ``ws`` and the rest are as in ``paged_decode_fwd``.
     """
     _op("cross_attn_fwd")(out, q, k_cache, v_cache, block_table, encoder_lens, query_start_loc,

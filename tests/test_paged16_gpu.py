@@ -413,6 +413,30 @@ def test_graph_replays_as_lengths_change(n):
         assert_close(out, *reference(q, keys, [n] * 3, 0.1, pair=n == 1))
 
 
+def test_graphs_share_a_workspace():
+    """Captured calls of other shapes, head sizes and kernels leave nothing in
+    the workspace that the next one reads."""
+    ws = torch.full((max(workspace(D).numel() for D in (64, 128, 256)),), math.nan, device=DEV)
+    graphs = []
+    for i, (D, lens, n) in enumerate([(128, [3000, 40, 0], 1), (64, [2000, 1999], 50),
+                                      (256, [700], 4), (64, [800] * 9, 3)]):
+        c = make_cache(lens, Hkv=4, D=D, block=16, dtype=BF, seed=40 + i)
+        q = queries(len(lens) * n, 16, D, BF, 40 + i)
+        out, starts = torch.empty_like(q), starts_of([n] * len(lens))
+        want = cross(c, q, [n] * len(lens), 0.1)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cross(c, q, [n] * len(lens), 0.1, ws=ws, out=out, starts=starts)
+        graphs.append((graph, out, want, (c, q, starts)))
+    for order in ([0, 1, 2, 3], [3, 1, 0, 2], [2, 2, 1, 0, 3]):
+        for i in order:
+            graphs[i][1].fill_(math.nan)
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in graphs:
+            assert torch.equal(out, want)
+
+
 def test_compile_traces_and_opcheck():
     c = make_cache([60, 30], Hkv=2, D=64, block=16, dtype=BF, seed=23)
     q, ws = queries(2, 4, 64, BF, 23), workspace(64)
