@@ -68,17 +68,36 @@ int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
 }
 
 // Whether every group is left whole, so that there is nothing to join: where
-// all are short. Measured, whole call, cut and whole, 32q / 8kv of 128 (bounds
-// of 64, 256, 512 and 1,024 keys), requests of one token:
+// all are short. Measured, whole call, cut and whole, 32q / 8kv of 128, requests
+// of one token (bounds of 64, 256, 512 and 1,024 keys):
 //     8 requests  10.7, 6.5   11.5,  8.6   12.6, 12.0   15.1, 20.5 us
 //    64           11.9, 7.5   19.3, 14.8   25.7, 24.6   40.0, 44.2
-// of 1 to 64 tokens against so many states:
-//     8            8.5, 8.7   19.2, 12.8   25.4, 18.4   28.9, 29.5
-//    64           25.8, 25.9  51.1, 40.3   63.9, 60.9   94.7, 95.1
 // D = 64 is alike; at D = 256, with one work-group per compute unit, 8 requests
 // of one token take 12.7, 9.7 and 13.3, 14.4 at 64 and 256.
-bool whole_groups(int32_t head_size, int64_t span, bool wide, int64_t units, int32_t cus) {
-  return span <= (head_size == 256 ? 128 : 512) && (!wide || units <= 8 * cus);
+bool whole_rows(int32_t head_size, int64_t span) {
+  return span <= (head_size == 256 ? 128 : 512);
+}
+// The same of 128-row units, whose slots are larger and so joined later: requests
+// of 25 to 100 tokens against a third of so many states or more (700, 1,000,
+// 1,500, 2,000), 32q / 8kv of 128:
+//     1 request   17.2, 17.1   16.0, 20.9   17.4, 27.2
+//     6 requests  28.8, 21.8   30.0, 28.6   33.8, 37.9   35.6, 48.6
+//    20           46.1, 30.0   52.8, 36.5   62.0, 54.0   71.8, 69.3
+//    28           56.5, 49.1   67.0, 66.7   81.6, 90.8   99.6, 115
+//    64          107.2, 84.3  130.5, 108   169.1, 148
+// 20 requests' units all but fill the device once, and then longer ones may stay
+// whole, too (D = 64 likewise: 53.3, 44.2 at 1,500); many units of one request,
+// whose lengths are alike, cost the end of the last (8 requests of 4,000 tokens:
+// 238, 239 at 500 and 341, 391 at 1,000; 16 of 2,000 255, 225 and 355, 358). At
+// D = 256, 16q / 4kv: 8 requests 38.6, 34.0 at 500, 43.5, 54.9 at 1,000; 16, three
+// quarters of the device, 58.0, 52.7; 400, whose shares are many short units,
+// 418, 445 at 500.
+bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
+  const int64_t round = resident(head_size) * cus;
+  int64_t most = head_size == 256 ? 512 : 1024;
+  if (units < cus / 8 || units > 8 * cus) most = head_size == 256 ? 128 : 512;
+  else if (10 * units >= 7 * round && units <= round) most = 1536;
+  return span <= most;
 }
 
 }  // namespace
@@ -171,7 +190,8 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   const int64_t span = p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + 15)
                                     : p.max_keys;
   const int64_t units = row_tiles * a.num_kv_heads;
-  const bool whole = whole_groups(a.head_size, span, wide, units, cus);
+  const bool whole =
+      wide ? whole_wide(a.head_size, span, units, cus) : whole_rows(a.head_size, span);
   const int64_t tokens = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
   p.team = wide ? 1 : team_of(p, span, std::min(bm, tokens * p.group), whole, cus);
   if (whole)

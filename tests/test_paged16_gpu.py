@@ -189,6 +189,21 @@ def test_bounds_at_which_groups_stay_whole(bound, heads, D):
     assert_close(far, *reference(q, c.keys, q_lens, D**-0.5))
 
 
+@pytest.mark.parametrize("bound", [512, 513, 1024, 1025, 1536, 1537])
+@pytest.mark.parametrize(("D", "heads", "R"), [(64, (16, 16), 16), (128, (32, 8), 18),
+                                               (256, (16, 4), 16), (128, (2, 1), 6)])
+def test_bounds_at_which_wide_groups_stay_whole(bound, D, heads, R):
+    """Units of about three quarters of the device, and of next to nothing."""
+    lens = ([bound, 0, bound // 3, bound - 1, 65] * R)[:R]
+    step = 128 * heads[1] // heads[0]
+    q_lens = ([step, 2 * step + 1, 1, 3 * step - 1, 0, 2 * step] * R)[:R]
+    c = make_cache(lens, Hkv=heads[1], D=D, block=32, dtype=HF, seed=bound)
+    q = queries(sum(q_lens), heads[0], D, HF, bound)
+    got = cross(c, q, q_lens, D**-0.5)
+    assert last_kernel() == "p16_wide"
+    assert_close(got, *reference(q, c.keys, q_lens, D**-0.5))
+
+
 def test_cross_many_requests():
     gen = torch.Generator().manual_seed(11)
     lens = torch.randint(0, 200, (140,), generator=gen).tolist()
