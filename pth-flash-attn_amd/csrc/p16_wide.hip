@@ -39,8 +39,7 @@
 // of four waves that take turns at the matrix cores (727), a tile's PV products
 // between the next one's softmax (602), wave priorities, a loop of two tiles
 // with fixed buffers, staggered starts, buffer loads (597, but D = 256 2 %
-// slower), waves without rows that leave out the products (short prompts: 41 us
-// either way).
+// slower).
 // D = 64 runs at 680 TFLOP/s (its softmax is twice the share), D = 256 at 670.
 
 #include "attn_device.h"
@@ -273,6 +272,22 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
+    // At D = 64, with three work-groups per compute unit, a wave without rows
+    // leaves its SIMD to the others' and only loads: 16 short prompts 41.1 -> 39.6
+    // us, and so for other ragged ones; at 128 36.2 -> 37.2, at 256 the same.
+    if constexpr (D == 64) {
+      if (32 * wave >= rows) {
+        for (int i = 0, next = after(t0); i < count; ++i, next = after(next), buf ^= 1) {
+          wait_vmcnt<0>();
+          __syncthreads();
+          if (i + 1 < count) {
+            load(next, buf ^ 1, entry);
+            entry = kPage16 ? ld_ro(table, page(after(next))) : 0;
+          }
+        }
+        continue;
+      }
+    }
     for (int i = 0, t = t0, next = after(t0); i < count;
          ++i, t = next, next = after(next), buf ^= 1) {
       wait_vmcnt<0>();
