@@ -37,9 +37,8 @@
 // power, take 495 us where others take 620. No faster, and so not here (4 x 2,048
 // rows against 4,096 keys, shortest of 20 calls 605 us): 256 rows in two halves
 // of four waves that take turns at the matrix cores (727), a tile's PV products
-// between the next one's softmax (602), wave priorities, a loop of two tiles
-// with fixed buffers, staggered starts, buffer loads (597, but D = 256 2 %
-// slower).
+// between the next one's softmax (602), a loop of two tiles with fixed buffers,
+// staggered starts.
 // D = 64 runs at 680 TFLOP/s (its softmax is twice the share), D = 256 at 670.
 
 #include "attn_device.h"
@@ -100,6 +99,18 @@ __device__ __forceinline__ float add_pair(uint32_t w, float sum) {
                                            __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
 }
 
+// dma16 from a wave's base and 32-bit offsets of its lanes. As a buffer load it
+// is not counted with LDS reads, which behind a global one in flight wait for
+// all of them at once (D = 256 742 -> 708 us, with column4's restrict).
+__device__ __forceinline__ void dma16_from(__amdgpu_buffer_rsrc_t base, uint32_t offset, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      base, (void __attribute__((address_space(3)))*)(lds), 16, static_cast<int>(offset), 0, 0, 0);
+}
+// A buffer of 2 GiB from p on: the callers' offsets are less than 2^29.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0x7fffffff, 0x00027000);
+}
+
 // A barrier for LDS alone: __syncthreads also waits for stores to memory.
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -108,8 +119,10 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // Column l % 16 of four rows of a row-major 16-bit matrix in LDS: lane i of
-// each 16 gives the address of row i / 4, columns 4 (i % 4).
-__device__ __forceinline__ u32x2 column4(const char* a) {
+// each 16 gives the address of row i / 4, columns 4 (i % 4). Without restrict
+// the compiler has the read wait for every load to LDS in flight, the next
+// tile's.
+__device__ __forceinline__ u32x2 column4(const char* __restrict__ a) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                        (i16x4 __attribute__((address_space(3)))*)(
                                            const_cast<char*>(a))));
@@ -194,11 +207,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
                          static_cast<int64_t>(u.head) * p.k.s_head;
         const char* vs = p.v.base + id * p.v.s_block + first * p.v.s_slot +
                          static_cast<int64_t>(u.head) * p.v.s_head;
+        const __amdgpu_buffer_rsrc_t kr = buffer_at(ks), vr = buffer_at(vs);
         if (kb + 16 <= len) {
 #pragma unroll
           for (int i = 0; i < W::kLoads; ++i) {
-            dma16(ks + k_off[i], kd + 1024 * i);
-            dma16(vs + v_off[i], vd + 1024 * i);
+            dma16_from(kr, k_off[i], kd + 1024 * i);
+            dma16_from(vr, v_off[i], vd + 1024 * i);
           }
         } else {
 #pragma unroll
@@ -207,8 +221,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
             const uint32_t from = min(t16, len - 1 - kb);
             const uint32_t k_row = __umul24(from, static_cast<uint32_t>(p.k.s_slot));
             const uint32_t v_row = __umul24(from, static_cast<uint32_t>(p.v.s_slot));
-            dma16(ks + (k_row + 16 * W::k_piece(t16, c)), kd + 1024 * i);
-            dma16(vs + (v_row + 16 * W::v_piece(t16, c)), vd + 1024 * i);
+            dma16_from(kr, k_row + 16 * W::k_piece(t16, c), kd + 1024 * i);
+            dma16_from(vr, v_row + 16 * W::v_piece(t16, c), vd + 1024 * i);
           }
         }
       } else {
@@ -292,10 +306,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
          ++i, t = next, next = after(next), buf ^= 1) {
       wait_vmcnt<0>();
       __syncthreads();  // tile t is in LDS, and nobody reads tile t - 1 any more
-      if (i + 1 < count) {
-        load(next, buf ^ 1, entry);
-        entry = kPage16 ? ld_ro(table, page(after(next))) : 0;
-      }
+      if (i + 1 < count) load(next, buf ^ 1, entry);
       const char* kt = lds + buf * W::kBuf;
       const char* vt = kt + 2 * W::kBuf;
 
@@ -339,7 +350,18 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
           vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
         }
       };
+      // The softmax before the products of the SIMD's other waves, so that one
+      // wave's softmax runs beside another's products (4 x 2,048 rows against
+      // 4,096 keys 556 -> 540 us, D = 64 345 -> 329; the products first: 541, 333).
+      __builtin_amdgcn_s_setprio(1);
       read_v(0);
+      // The page number for the next tile but one, on its way during the
+      // softmax and waited for behind it: counted with LDS reads, which it
+      // would otherwise make wait for all.
+      if constexpr (kPage16) {
+        __builtin_amdgcn_sched_barrier(0);
+        entry = ld_ro(table, page(after(next)));
+      }
       if (kKT * t + kKT > len) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -389,6 +411,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
           l = add_pair<kF16>(w, l);
           pf[2 * b + (i >> 3)][(i & 7) >> 1] = w;
         }
+      if constexpr (kPage16) asm volatile("" ::"s"(entry));
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         __builtin_amdgcn_sched_barrier(0);
