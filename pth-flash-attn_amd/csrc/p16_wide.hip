@@ -350,10 +350,11 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
           vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
         }
       };
-      // The softmax before the products of the SIMD's other waves, so that one
-      // wave's softmax runs beside another's products (4 x 2,048 rows against
-      // 4,096 keys 556 -> 540 us, D = 64 345 -> 329; the products first: 541, 333).
-      __builtin_amdgcn_s_setprio(1);
+      // The softmax goes before the scores, and these before the PV products, of
+      // the SIMD's other waves, so that they run beside each other (4 x 2,048 rows
+      // against 4,096 keys: 586 us with the softmax before both, 576 so; on
+      // another card 556 without, 540 with the first, 541 with the products first).
+      __builtin_amdgcn_s_setprio(2);
       read_v(0);
       // The page number for the next tile but one, on its way during the
       // softmax and waited for behind it: counted with LDS reads, which it
@@ -421,6 +422,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
 #pragma unroll
         for (int j = 0; j < W::kO; ++j) o[j] = mfma32<kF16>(vf[i & 1][j], pf[i], o[j]);
       }
+      __builtin_amdgcn_s_setprio(1);
     }
 
     const SwapPair ls = swap_halves(l);
