@@ -28,18 +28,19 @@
 // of its pairs. In fp16, whose range is short, P is scaled by 2^12: weights down
 // to 2^-26 of a row's largest keep all 11 bits.
 //
-// Bound: the matrix cores and the softmax's VALU work, which one SIMD's two
-// waves overlap, at the clock that the power leaves. 4 prompts of 1,500 to 2,048
-// rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11 operations):
-// 780 us, 860 TFLOP/s (a library's 8192^3 product: 1,205); 852 before the keys'
-// order above (fabric reads 3.95 GB, now 0.52). MFMA is busy 48 % of the time,
-// VALU 42 %, without bank conflicts, at 1.83 GHz; inputs of zeros, which draw less
-// power, take 495 us where others take 620. No faster, and so not here (4 x 2,048
-// rows against 4,096 keys, shortest of 20 calls 605 us): 256 rows in two halves
-// of four waves that take turns at the matrix cores (727), a tile's PV products
-// between the next one's softmax (602), a loop of two tiles with fixed buffers,
-// staggered starts.
-// D = 64 runs at 680 TFLOP/s (its softmax is twice the share), D = 256 at 670.
+// Bound: the matrix cores and the softmax's VALU work, which the SIMD's waves
+// run beside each other, at the clock that the power leaves. 4 prompts of 1,500
+// to 2,048 rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11
+// operations), whole call: 665 to 729 us by card, 0.92 to 1.0 PFLOP/s (a library's
+// 8192^3 product: 1.2); MFMA is busy 54 % of the time, VALU 46 %, without bank
+// conflicts. On the way there: 749 us before the keys' order above (fabric reads
+// 3.95 GB, now 0.52), 700 before the waits and priorities below. 4 x 2,048 rows
+// against 4,096 keys run at 0.95 PFLOP/s, 0.77 at D = 64 (the softmax is twice
+// the share) and 0.75 at D = 256 (one wave per SIMD). No faster, and so not here:
+// 256 rows in two halves of four waves that take turns at the matrix cores, a
+// tile's PV products between the next one's softmax, a loop of two tiles with
+// fixed buffers, staggered starts, and, at D = 64, two tiles on their way instead
+// of one (32 rows of 64 requests against 1,500 keys 85.9 -> 91.8 us).
 
 #include "attn_device.h"
 #include "p16.h"
