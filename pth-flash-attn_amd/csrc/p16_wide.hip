@@ -31,11 +31,11 @@
 // Bound: the matrix cores and the softmax's VALU work, which the SIMD's waves
 // run beside each other, at the clock that the power leaves. 4 prompts of 1,500
 // to 2,048 rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11
-// operations), whole call: 674 to 729 us by card, 0.92 to 0.99 PFLOP/s (a library's
+// operations), whole call: 670 to 729 us by card, 0.92 to 1.0 PFLOP/s (a library's
 // 8192^3 product: 1.2); MFMA is busy 54 % of the time, VALU 46 %, without bank
 // conflicts. On the way there: 749 us before the keys' order above (fabric reads
-// 3.95 GB, now 0.52), 700 before the waits and priorities below (then 674). 4 x 2,048 rows
-// against 4,096 keys run at 0.95 PFLOP/s, 0.77 at D = 64 (the softmax is twice
+// 3.95 GB, now 0.52), 700 before the waits and priorities below (then 674). 4 x
+// 2,048 rows against 4,096 keys run at 0.95 PFLOP/s, 0.77 at D = 64 (the softmax is twice
 // the share) and 0.75 at D = 256 (one wave per SIMD). No faster, and so not here:
 // 256 rows in two halves of four waves that take turns at the matrix cores, a
 // tile's PV products between the next one's softmax, a loop of two tiles with
@@ -103,7 +103,8 @@ __device__ __forceinline__ float add_pair(uint32_t w, float sum) {
 // dma16 from a wave's base and 32-bit offsets of its lanes. As a buffer load it
 // is not counted with LDS reads, which behind a global one in flight wait for
 // all of them at once (D = 256 742 -> 708 us, with column4's restrict).
-__device__ __forceinline__ void dma16_from(__amdgpu_buffer_rsrc_t base, uint32_t offset, char* lds) {
+__device__ __forceinline__ void dma16_from(__amdgpu_buffer_rsrc_t base, uint32_t offset,
+                                           char* lds) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(
       base, (void __attribute__((address_space(3)))*)(lds), 16, static_cast<int>(offset), 0, 0, 0);
 }
@@ -287,10 +288,11 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
-    // At D = 64, with three work-groups per compute unit, a wave without rows
-    // leaves its SIMD to the others' and only loads: 16 short prompts 41.1 -> 39.6
-    // us, and so for other ragged ones; at 128 36.2 -> 37.2, at 256 the same.
-    if constexpr (D == 64) {
+    // A wave without rows only loads, and leaves its SIMD to the others: 32 rows
+    // of 64 requests against 1,500 keys 82.6 -> 79.0 us, 20 ragged requests 34.6
+    // -> 33.8 (16 short prompts at D = 64 41.1 -> 39.6). At D = 256 there is no
+    // other wave, and the registers' spills grow (708 -> 733).
+    if constexpr (D != 256) {
       if (32 * wave >= rows) {
         for (int i = 0, next = after(t0); i < count; ++i, next = after(next), buf ^= 1) {
           wait_vmcnt<0>();
