@@ -174,10 +174,10 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
 
   // More rows than the small kernel's tile of a KV head: the other, whose tiles
-  // eight times as many rows share (17 rows per request, 16q / 16kv of 64 against
-  // 1,500 states: 1, 8 and 64 requests 11.0, 19.5 and 93 us, the small one's row
-  // tiles 13.6, 22.6 and 120; 16 rows 12.0, 17.1 and 76 with the small one, and
-  // 10.8, 19.5 and 91 with the other).
+  // eight times as many rows share. 16q / 16kv of 64 against 1,500 states, 1, 8
+  // and 64 requests: of 32 rows 13.6, 17.8 and 85.9 us, the small one's row tiles
+  // 18.2, 23.6 and 130; of 16 rows 13.1, 16.7 and 81.7, 12.7, 17.5 and 76.4 with
+  // the small one.
   const bool wide = a.query_start_loc != nullptr &&
                     static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
   const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
