@@ -218,8 +218,10 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   // Work-groups of the join per note: a row or eight each, until the device is
   // full (256 tokens against 4,096 states: 23 us with one, 8.3 with eight).
   // Of 16-row units, four times as many as compute units (4 tokens of 8 requests
-  // against 1,500 states, D = 256: whole call 29.1 us with twice, 25.7).
-  const int32_t items = p.team * p.slot_rows, least = wide ? 4 : 1;
+  // against 1,500 states, D = 256: whole call 29.1 us with twice, 25.7). Of 128-row
+  // units at least 16, a row of a work-group's crew each (28 requests of 25 to 100
+  // tokens to 2,000 states 88.9 us with 4, 86.4; others alike within 1 %).
+  const int32_t items = p.team * p.slot_rows, least = wide ? 16 : 1;
   const int32_t y =
       p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
   if (err == hipSuccess && key_tiles > 1)

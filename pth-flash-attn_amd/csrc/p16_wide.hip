@@ -31,7 +31,7 @@
 // Bound: the matrix cores and the softmax's VALU work, which the SIMD's waves
 // run beside each other, at the clock that the power leaves. 4 prompts of 1,500
 // to 2,048 rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11
-// operations), whole call: 670 to 729 us by card, 0.92 to 1.0 PFLOP/s (a library's
+// operations), whole call: 663 to 729 us by card, 0.92 to 1.0 PFLOP/s (a library's
 // 8192^3 product: 1.2); MFMA is busy 54 % of the time, VALU 46 %, without bank
 // conflicts. On the way there: 749 us before the keys' order above (fabric reads
 // 3.95 GB, now 0.52), 700 before the waits and priorities below (then 674). 4 x
