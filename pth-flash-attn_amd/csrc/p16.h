@@ -25,6 +25,7 @@
 #pragma once
 
 #include "attn_stream.h"
+#include "p16_geometry.h"
 
 namespace pa {
 
@@ -106,8 +107,9 @@ __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int 
     q0 = r;
     q1 = r + 1;
   }
-  x.q0 = min(max(q0, 0), p.num_tokens);
-  x.rows = max(min(q1, p.num_tokens) - x.q0, 0) * p.group;
+  const P16Tokens t = p16_tokens(q0, q1, p.num_tokens);
+  x.q0 = t.first;
+  x.rows = t.count * p.group;
   x.len = min(max(len, 0), p.max_keys);
   x.lo = p.window > 0 ? max(x.len - p.window, 0) : 0;
   x.base = x.lo & ~15;
