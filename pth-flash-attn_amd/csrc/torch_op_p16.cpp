@@ -77,6 +77,71 @@ bool overlaps_itself(const Tensor& t) {
 }
 bool overlap(const Span& a, const Span& b) { return a.begin < b.end && b.begin < a.end; }
 
+bool same_view(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+// Whether two tensors of one type, at most 4-D, share an element: whether
+// sum n_i s_i is the distance between their first elements for some n_i in
+// [lo_i, hi_i], s_i the strides of both (b's counted backwards), from the
+// largest on. What the smaller ones reach leaves one or two n_i of each where
+// the strides nest; views that would take more than kMost steps count as
+// sharing one.
+class SharedElement {
+ public:
+  static bool of(const Tensor& a, const Tensor& b) {
+    SharedElement x;
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    for (int64_t i = 0; i < a.dim(); ++i) x.add(a.stride(i), 0, a.size(i) - 1);
+    for (int64_t i = 0; i < b.dim(); ++i) x.add(b.stride(i), 1 - b.size(i), 0);
+    std::sort(x.terms_, x.terms_ + x.n_,
+              [](const Term& p, const Term& q) { return p.stride > q.stride; });
+    for (int64_t i = x.n_; i-- > 0;) {
+      x.lo_[i] = x.lo_[i + 1] + x.terms_[i].lo * x.terms_[i].stride;
+      x.hi_[i] = x.hi_[i + 1] + x.terms_[i].hi * x.terms_[i].stride;
+    }
+    const int64_t apart = reinterpret_cast<intptr_t>(b.data_ptr()) -
+                          reinterpret_cast<intptr_t>(a.data_ptr());
+    const int64_t size = static_cast<int64_t>(a.element_size());
+    return apart % size != 0 || x.reaches(0, apart / size);
+  }
+
+ private:
+  static constexpr int kMost = 1 << 16;
+  struct Term {
+    int64_t stride, lo, hi;
+  };
+  Term terms_[8];
+  int64_t n_ = 0, lo_[9] = {}, hi_[9] = {};
+  int steps_ = 0;
+
+  void add(int64_t stride, int64_t lo, int64_t hi) {
+    if (stride == 0 || lo == hi) return;
+    for (int64_t i = 0; i < n_; ++i) {
+      if (terms_[i].stride != stride) continue;
+      terms_[i].lo += lo;
+      terms_[i].hi += hi;
+      return;
+    }
+    terms_[n_++] = {stride, lo, hi};
+  }
+  // Whether the terms from i on can sum to x.
+  bool reaches(int64_t i, int64_t x) {
+    if (x < lo_[i] || x > hi_[i]) return false;
+    if (i == n_) return true;
+    if (++steps_ > kMost) return true;
+    const Term& t = terms_[i];
+    const auto floor = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t from = std::max(t.lo, -floor(hi_[i + 1] - x, t.stride));
+    const int64_t to = std::min(t.hi, floor(x - lo_[i + 1], t.stride));
+    for (int64_t n = from; n <= to; ++n)
+      if (reaches(i + 1, x - n * t.stride)) return true;
+    return false;
+  }
+};
+
 // The kernels are built for gfx950; a device's name does not change.
 void check_device_arch(const char* op, const Tensor& t) {
   constexpr int kMost = 64;
@@ -184,6 +249,8 @@ void attend(const char* op, const char* lens_name, const Tensor& out, const Tens
   const Span s_out = span_of(op, out), s_ws = span_of(op, ws), s_q = span_of(op, q);
   OP_CHECK(!overlap(s_out, s_ws), "out and ws must not overlap");
   OP_CHECK(!overlap(s_ws, s_q), "ws must not overlap an input");
+  OP_CHECK(!overlap(s_out, s_q) || same_view(out, q) || !SharedElement::of(out, q),
+           "out must be q itself or share no memory with it");
   for (const Tensor* t : {&k_cache, &v_cache, &block_table, &lens}) {
     const Span s = span_of(op, *t);
     OP_CHECK(!overlap(s_out, s), "out must not overlap an input");

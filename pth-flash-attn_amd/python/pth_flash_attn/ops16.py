@@ -249,7 +249,9 @@ def paged_decode_fwd(
     keys, its own among them; a request without keys gives zeros. What a page
     holds outside of these keys reaches no output. A NaN or a score of +inf
     makes its row NaN, and an infinite value its column infinite or NaN.
-    ``out`` may be ``q`` itself; other than that they share no memory.
+    ``out`` may be ``q`` itself; other than that they share no memory (both may be
+    views of one buffer, as parts of its columns; where telling that apart takes
+    more than 2^16 steps, they are refused).
     ``max_seq_len`` bounds the lengths (longer ones are cut there, and at the
     block table's reach). ``ws`` is workspace of
     ``planner.paged16_workspace_floats`` floats; it holds nothing between calls,

@@ -1,13 +1,13 @@
 """Attention over a paged 16-bit cache where its integer tensors hold anything:
 requests whose own are in order keep their results, and nothing else is
-written."""
+written; and where out and q are columns of one buffer."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from paged16_cases import DEV, assert_close, cross, make_cache, queries, reference
+from paged16_cases import DEV, assert_close, cross, decode, make_cache, queries, reference
 
 pytestmark = pytest.mark.gpu
 LOW = -(2**31)
@@ -30,3 +30,17 @@ def test_starts_far_below_zero(n, heads, low):
     want, tol = reference(q[:200], c.keys[:2], q_lens, 0.125, pair=n * Hq // Hkv <= 16)
     assert_close(out[:200], want, tol)
     assert (out[200:] == 7.0).all()
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [70, 0, 130]])
+def test_out_beside_q_in_one_buffer(q_lens):
+    c = make_cache([900, 40, 333], Hkv=2, D=128, block=16, dtype=torch.bfloat16, seed=3)
+    T = sum(q_lens)
+    fused = queries(T, 20, 128, torch.bfloat16, 3)
+    before, q, out = fused.clone(), fused[:, :8], fused[:, 12:]
+    if T == 3:
+        decode(c, q, 0.1, out=out)
+    else:
+        cross(c, q, q_lens, 0.1, out=out)
+    assert_close(out, *reference(before[:, :8], c.keys, q_lens, 0.1, pair=T == 3))
+    assert torch.equal(fused[:, :12], before[:, :12])
