@@ -25,8 +25,11 @@
 // a score passes it by 2^kSlack, so most tiles rescale nothing. P is rounded
 // once to the inputs' type, as the output is: both errors are independent, and
 // together sqrt(2) of the output's own; l sums the rounded P, by dot products
-// of its pairs. In fp16, whose range is short, P is scaled by 2^12: weights down
-// to 2^-26 of a row's largest keep all 11 bits.
+// of its pairs. P is scaled by 2^kBias. In bf16 by 2^-kSlack: with the maximum that
+// far behind no weight passes 1, so that sums of values near the type's largest
+// leave 32 bits no sooner than with the exact maximum. In fp16, whose range is
+// short, by 2^12: weights down to 2^-26 of a row's largest keep all 11 bits (2^15
+// x 2^16 x 2^31 keys are within 32 bits).
 //
 // Bound: the matrix cores and the softmax's VALU work, which the SIMD's waves
 // run beside each other, at the clock that the power leaves. 4 prompts of 1,500
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void p16_wide(
   using W = WideOf<D>;
   constexpr int kBM = kP16WideRows, kKT = kP16WideKeys;
   constexpr float kSlack = kF16 ? 3.0f : 8.0f;
-  constexpr float kBias = kF16 ? 12.0f : 0.0f;
+  constexpr float kBias = kF16 ? 12.0f : -kSlack;
   __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
 
   const int lane = threadIdx.x & 63;
