@@ -377,7 +377,9 @@ int32_t pth_attn_paged16_args_bytes(void);
 int64_t pth_attn_paged16_workspace_floats(int32_t head_size);
 
 /* Keys and values into a paged 16-bit cache: a copy, or (fp32) one rounding
- * to nearest even. Slots are distinct; a slot outside the cache is skipped. */
+ * to nearest even. Slots are distinct; a slot outside the cache is skipped. The
+ * caches share no memory with each other (if key and value differ) or with
+ * an input. */
 int32_t pth_attn_write_kv16(const PthAttnWrite16Args* args, void* stream);
 int32_t pth_attn_write16_args_bytes(void);
 

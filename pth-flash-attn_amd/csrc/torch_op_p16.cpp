@@ -350,6 +350,10 @@ void reshape_and_cache_16bit(const Tensor& key, const Tensor& value, const Tenso
   OP_CHECK(!overlaps_itself(k_cache) && !overlaps_itself(v_cache),
            "k_cache and v_cache must not overlap themselves");
   const Span s_k = span_of(op, k_cache), s_v = span_of(op, v_cache);
+  OP_CHECK(!overlap(s_k, s_v) || !SharedElement::of(k_cache, v_cache) ||
+               (same_view(k_cache, v_cache) && same_view(key, value)),
+           "k_cache and v_cache must share no memory, unless both are one view and so are key "
+           "and value");
   for (const Tensor* t : {&key, &value, &slot_mapping}) {
     const Span s = span_of(op, *t);
     OP_CHECK(!overlap(s_k, s) && !overlap(s_v, s), "the cache must not overlap an input");

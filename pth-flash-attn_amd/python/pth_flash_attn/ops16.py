@@ -232,7 +232,8 @@ def reshape_and_cache_16bit(key: torch.Tensor, value: torch.Tensor, k_cache: tor
     Token t goes to slot ``slot_mapping[t]`` (page ``slot // block_size``,
     in-page slot ``slot % block_size``); a slot outside the cache, as -1, skips
     it. Slots are distinct. The values have the cache's dtype, or are float32
-    and rounded once, to nearest even. Cache rows are 16-byte aligned.
+    and rounded once, to nearest even. Cache rows are 16-byte aligned. The two
+    caches share no memory, unless both are one view, written by one tensor.
     """
     _op("reshape_and_cache_16bit")(key, value, k_cache, v_cache, slot_mapping)
 

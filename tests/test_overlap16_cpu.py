@@ -93,3 +93,37 @@ def test_random_views_of_one_buffer():
         assert (SHARED if shares else ON_GPU) in said, (shape, views)
         seen[shares] += 1
     assert min(seen.values()) > 50
+
+
+def write(k_cache, v_cache, key, value):
+    with pytest.raises(RuntimeError) as e:
+        ops.reshape_and_cache_16bit(key, value, k_cache, v_cache,
+                                    torch.zeros(key.shape[0], dtype=torch.int64))
+    return str(e.value)
+
+
+def test_caches_that_share_memory_are_refused():
+    """A token's key and value would go to one place, in no order."""
+    kv = torch.zeros(6, 2, 16, 2, 64, dtype=BF)
+    k, v = paged16_views(kv)
+    key, value = torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF)
+    shifted = kv.flatten()[8:].as_strided(k[:5].shape, k.stride())
+    for a, b in ((k, k), (k[1:], k[:-1]), (k[:, :8], k[:, 4:12]), (k[:3], k[2:5]), (k[:5], shifted)):
+        assert "k_cache and v_cache must share no memory" in write(a, b, key, value)
+    # One cache for both is written by one tensor for both.
+    assert "must share no memory" in write(k, k, key, value)
+    assert ON_GPU in write(k, k, key, key)
+
+
+def test_caches_of_one_buffer_are_taken():
+    key, value = torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF)
+    for layout, inner in (("NHD", (16, 2)), ("HND", (2, 16))):
+        kv = torch.zeros(6, 2, *inner, 64, dtype=BF)
+        assert ON_GPU in write(*paged16_views(kv, layout=layout), key, value)
+    mixed = torch.zeros(6, 4096, dtype=BF)  # keys NHD, values HND
+    assert ON_GPU in write(mixed[:, :2048].view(6, 16, 2, 64),
+                           mixed[:, 2048:].view(6, 2, 16, 64).transpose(1, 2), key, value)
+    beside = torch.zeros(6, 16, 2, 128, dtype=BF)  # a head's key and value side by side
+    assert ON_GPU in write(beside[..., :64], beside[..., 64:], key, value)
+    apart = torch.zeros(2, 6, 16, 2, 64, dtype=BF)
+    assert ON_GPU in write(apart[0], apart[1], key, value)

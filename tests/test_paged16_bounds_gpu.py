@@ -4,10 +4,14 @@ written; and where out and q are columns of one buffer."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
-from paged16_cases import DEV, assert_close, cross, decode, make_cache, queries, reference
+from paged16_cases import (DEV, assert_close, cross, decode, make_cache, queries, reference,
+                           workspace)
+from pth_flash_attn import ops
 
 pytestmark = pytest.mark.gpu
 LOW = -(2**31)
@@ -44,3 +48,22 @@ def test_out_beside_q_in_one_buffer(q_lens):
         cross(c, q, q_lens, 0.1, out=out)
     assert_close(out, *reference(before[:, :8], c.keys, q_lens, 0.1, pair=T == 3))
     assert torch.equal(fused[:, :12], before[:, :12])
+
+
+def test_caches_of_one_buffer():
+    """Keys NHD and values HND in one page, and one cache for both."""
+    T, Hkv, D = 40, 2, 64
+    key, value = (queries(T, Hkv, D, torch.bfloat16, i) for i in (1, 2))
+    slots = torch.arange(16, 16 + T, device=DEV)
+    table = torch.tensor([[1, 2, 3]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([T], dtype=torch.int32, device=DEV)
+    q, n = queries(1, 4, D, torch.bfloat16, 3), 16 * Hkv * D
+    pages = torch.full((5, 2 * n), math.nan, dtype=torch.bfloat16, device=DEV)
+    k = pages[:, :n].view(5, 16, Hkv, D)
+    v = pages[:, n:].view(5, Hkv, 16, D).transpose(1, 2)
+    for caches, values in (((k, v), value), ((k, k), key)):
+        pages.fill_(math.nan)
+        ops.reshape_and_cache_16bit(key, values, *caches, slots)
+        out = torch.empty_like(q)
+        ops.paged_decode_fwd(out, q, *caches, table, lens, T, 0.1, workspace(D))
+        assert_close(out, *reference(q, [(key, values)], [1], 0.1, pair=True))
