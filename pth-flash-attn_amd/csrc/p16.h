@@ -59,12 +59,6 @@ struct P16Params {
   float scale_log2;       // softmax_scale * log2(e)
 };
 
-// Row tiles of the two kernels, and the wide one's key tile (the other's is 32
-// for each wave of a unit).
-constexpr int kP16Waves = 4;
-constexpr int kP16RowsRows = 16;
-constexpr int kP16WideRows = 32 * kP16Waves, kP16WideKeys = 64;
-
 // A cut group: the slots that hold it (0: none is cut) and, above kP16CutShift,
 // the work-group that begins it; its request's first query token and rows, its
 // place among the request's groups.
@@ -73,15 +67,6 @@ struct P16Cut {
   int32_t q0, rows, group;
 };
 constexpr int kP16CutShift = 16;
-
-// Workspace: rows of D sums with a maximum and a sum each, as many as the
-// work-groups of a compute unit (at most kP16WgPerCu) have in their slots, and
-// a P16Cut for each work-group and one before them.
-constexpr int kP16WgPerCu = 8;
-inline int64_t p16_workspace_floats(int32_t head_size, int32_t cus) {
-  const int64_t rows = head_size == 64 ? 768 : 512;
-  return cus * (rows * (head_size + 2) + 4 * kP16WgPerCu);
-}
 
 #if defined(__HIPCC__)
 

@@ -8,6 +8,27 @@
 
 namespace pa {
 
+// Row tiles of the two kernels, and the wide one's key tile (the other's is 32
+// for each wave of a unit).
+constexpr int kP16Waves = 4;
+constexpr int kP16RowsRows = 16;
+constexpr int kP16WideRows = 32 * kP16Waves, kP16WideKeys = 64;
+
+// Work-groups of either attention kernel that a compute unit holds, by their
+// registers, and so the most whose slots are in use where groups are cut.
+PA_HD constexpr int32_t p16_resident(int32_t head_size) {
+  return head_size == 64 ? 3 : head_size == 128 ? 2 : 1;
+}
+
+// Workspace: two slots of each such work-group, of the most rows that a slot of
+// either kernel has, D sums with a maximum and a sum to each row; behind them
+// the notes (P16Cut), one for each work-group and one before them.
+constexpr int32_t kP16NoteWords = 32;  // of a compute unit
+inline int64_t p16_workspace_floats(int32_t head_size, int32_t cus) {
+  const int64_t rows = int64_t{2} * p16_resident(head_size) * kP16WideRows;
+  return cus * (rows * (head_size + 2) + kP16NoteWords);
+}
+
 // A request's query tokens: `count` from `first` on.
 struct P16Tokens {
   int32_t first, count;

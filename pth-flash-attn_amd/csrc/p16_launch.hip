@@ -54,9 +54,6 @@ int32_t team_of(const P16Params& p, int64_t span, int64_t rows, bool whole, int3
   return team;
 }
 
-// Work-groups of either attention kernel that a compute unit holds.
-int64_t resident(int32_t head_size) { return head_size == 64 ? 3 : head_size == 128 ? 2 : 1; }
-
 // The 16-row kernel's work-groups per compute unit where groups are cut. One,
 // four waves, reads the cache fastest: more streams at once cost the memory more
 // than they hide (64 requests to 32k keys at D = 128: 626 us with one, 646 with
@@ -64,7 +61,7 @@ int64_t resident(int32_t head_size) { return head_size == 64 ? 3 : head_size == 
 // gaps between them, as many as fit (48 requests to 4k, 16 heads of 64 in HND
 // pages: 92 us with one, 78 with two, 76 with three).
 int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
-  return std::min(resident(head_size), std::max<int64_t>(1, groups / cus));
+  return std::min<int64_t>(p16_resident(head_size), std::max<int64_t>(1, groups / cus));
 }
 
 // Whether every group is left whole, so that there is nothing to join: where
@@ -93,7 +90,7 @@ bool whole_rows(int32_t head_size, int64_t span) {
 // quarters of the device, 58.0, 52.7; 400, whose shares are many short units,
 // 418, 445 at 500.
 bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
-  const int64_t round = resident(head_size) * cus;
+  const int64_t round = int64_t{p16_resident(head_size)} * cus;
   int64_t most = head_size == 256 ? 512 : 1024;
   if (units < cus / 8 || units > 8 * cus) most = head_size == 256 ? 128 : 512;
   else if (10 * units >= 7 * round && units <= round) most = 1536;
@@ -195,7 +192,7 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   const int64_t tokens = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
   p.team = wide ? 1 : team_of(p, span, std::min(bm, tokens * p.group), whole, cus);
   if (whole)
-    while (p.team > 1 && units / p.team < resident(a.head_size) * cus) p.team /= 2;
+    while (p.team > 1 && units / p.team < p16_resident(a.head_size) * cus) p.team /= 2;
   p.key_tile_log2 = wide ? 6 : 7 - (p.team >> 1);
   if (whole)
     while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
@@ -208,7 +205,7 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
           : units / p.team + (p.team > 1 ? a.num_reqs : 0);
   PA_REQUIRE(units < INT32_MAX / key_tiles, "the launch exceeds 2^31 tiles");
   const int64_t fill =
-      cus * (wide ? resident(a.head_size) : rows_per_cu(a.head_size, groups, cus));
+      cus * (wide ? p16_resident(a.head_size) : rows_per_cu(a.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
   if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
   p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;

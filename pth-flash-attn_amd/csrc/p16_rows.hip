@@ -51,7 +51,7 @@ struct RowsDim {
   static constexpr int kCols = D < 128 ? D / 16 : 8; // columns per V load
   static constexpr int kPieces = D / (16 * kCols);   // V loads per key row
   static constexpr int kO = D / 16;                  // PV products per chunk
-  static constexpr int kPerSimd = D == 64 ? 3 : D == 128 ? 2 : 1;
+  static constexpr int kPerSimd = p16_resident(D);   // a work-group has a wave on each SIMD
   // At D = 256 the registers do not hold Q beside K, V and O.
   static constexpr bool kQInLds = D == 256;
 };

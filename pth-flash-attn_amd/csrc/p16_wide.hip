@@ -57,7 +57,7 @@ typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
 struct WideOf {
-  static constexpr int kPerSimd = D == 256 ? 1 : D == 64 ? 3 : 2;
+  static constexpr int kPerSimd = p16_resident(D);  // a work-group has a wave on each SIMD
   static constexpr int kQ = D / 16;      // QK products per 32 keys
   static constexpr int kO = D / 32;      // output tiles
   static constexpr int kRow = 2 * D;     // bytes of a key row

@@ -297,16 +297,16 @@ def workspace_bytes(*, ws_token_splits: int, Hq: int, D: int) -> int:
 
 
 # Rows of partial sums per compute unit that the 16-bit cache's kernels can have
-# in flight (two slots of each of its work-groups), by head size, and 4-byte
-# words of the notes beside them.
-PAGED16_ROWS_PER_CU = {64: 768, 128: 512, 256: 512}
+# in flight (two slots of up to 128 rows for each of its 3, 2 or 1 work-groups),
+# by head size, and 4-byte words of the notes beside them.
+PAGED16_ROWS_PER_CU = {64: 768, 128: 512, 256: 256}
 PAGED16_NOTE_WORDS_PER_CU = 32
 
 
 def paged16_workspace_floats(*, D: int, num_sms: int) -> int:
     """fp32 elements of the workspace of ``paged_decode_fwd`` / ``cross_attn_fwd``:
-    per compute unit 512 rows (768 at D = 64) of D sums, a maximum and a weight
-    sum, and 32 words, whatever the batch, its heads and its lengths (no
+    per compute unit 512 rows (768 at D = 64, 256 at D = 256) of D sums, a maximum
+    and a weight sum, and 32 words, whatever the batch, its heads and its lengths (no
     counterpart in the reference)."""
     d = _head_size(D)
     per_cu = PAGED16_ROWS_PER_CU[d] * (d + 2) + PAGED16_NOTE_WORDS_PER_CU

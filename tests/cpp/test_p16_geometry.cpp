@@ -42,8 +42,27 @@ static void tokens() {
   std::printf("tokens ok\n");
 }
 
+// The workspace holds the slots and notes of as many work-groups as a device
+// has resident, for any team and rows of a unit, and no more than the largest
+// of these takes.
+static void workspace() {
+  for (int32_t d : {64, 128, 256})
+    for (int32_t cus : {1, 256, 304}) {
+      const int64_t have = p16_workspace_floats(d, cus);
+      int64_t most = 0;
+      const int64_t wgs = int64_t{cus} * p16_resident(d);
+      for (int64_t rows : {1, 5, kP16RowsRows, 2 * kP16RowsRows, 4 * kP16RowsRows, kP16WideRows})
+        most = std::max(most, 2 * wgs * rows * (d + 2));
+      CHECK(most + 4 * (wgs + 1) <= have, "D %d: %lld of %lld", d, (long long)most, (long long)have);
+      CHECK(have - most <= kP16NoteWords * cus, "D %d: %lld floats unused", d,
+            (long long)(have - most));
+      std::printf("workspace %d %d %lld\n", d, cus, (long long)have);
+    }
+}
+
 int main() {
   tokens();
+  workspace();
   std::printf("ALL OK\n");
   return 0;
 }

@@ -9,6 +9,8 @@ from pathlib import Path
 
 import pytest
 
+from pth_flash_attn import planner
+
 REPO = Path(__file__).resolve().parent.parent
 
 
@@ -22,3 +24,14 @@ def test_geometry16_header(tmp_path):
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stdout + res.stderr
     assert "ALL OK" in res.stdout
+    # The planner's sizes are the launcher's.
+    sizes = [tuple(map(int, line.split()[1:])) for line in res.stdout.splitlines()
+             if line.startswith("workspace")]
+    assert {d for d, _, _ in sizes} == {64, 128, 256}
+    for d, cus, floats in sizes:
+        assert planner.paged16_workspace_floats(D=d, num_sms=cus) == floats
+
+
+def test_workspace_sizes():
+    assert [planner.paged16_workspace_floats(D=d, num_sms=256) for d in (64, 128, 256)] == [
+        256 * (768 * 66 + 32), 256 * (512 * 130 + 32), 256 * (256 * 258 + 32)]

@@ -11,7 +11,7 @@ import torch
 
 from paged16_cases import (DEV, assert_close, cross, decode, make_cache, queries, reference,
                            workspace)
-from pth_flash_attn import ops
+from pth_flash_attn import capi, ops, planner
 
 pytestmark = pytest.mark.gpu
 LOW = -(2**31)
@@ -67,3 +67,23 @@ def test_caches_of_one_buffer():
         out = torch.empty_like(q)
         ops.paged_decode_fwd(out, q, *caches, table, lens, T, 0.1, workspace(D))
         assert_close(out, *reference(q, [(key, values)], [1], 0.1, pair=True))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_workspace_of_the_planner_s_size_is_enough(D):
+    """Both kernels with every work-group's slots in use leave what lies behind
+    the workspace as it was; a float less is refused."""
+    cus = torch.cuda.get_device_properties(DEV).multi_processor_count
+    floats = planner.paged16_workspace_floats(D=D, num_sms=cus)
+    assert capi.AttnLib().lib.pth_attn_paged16_workspace_floats(D) == floats
+    buf = torch.full((floats + 4096,), 7.0, device=DEV)
+    for Hkv, n, lens in ((16, 1, [2100 + 7 * i for i in range(64)]), (8, 130, [1700] * 12)):
+        c = make_cache(lens, Hkv=Hkv, D=D, block=16, dtype=torch.bfloat16, seed=D)
+        q_lens = [n] * len(lens)
+        q = queries(sum(q_lens), 4 * Hkv, D, torch.bfloat16, D)
+        out = cross(c, q, q_lens, D**-0.5, ws=buf[:floats])
+        assert capi.AttnLib().last_kernel() == ("p16_rows" if n == 1 else "p16_wide")
+        assert_close(out, *reference(q, c.keys, q_lens, D**-0.5, pair=n == 1))
+        assert (buf[floats:] == 7.0).all()
+        with pytest.raises(RuntimeError, match="ws must be 16-byte aligned and hold"):
+            cross(c, q, q_lens, D**-0.5, ws=buf[: floats - 1])
