@@ -187,9 +187,10 @@ typedef struct PthAttnWriteArgs {
  * own 16-bit type. No counterpart in the reference. Request r has kv_lens[r]
  * keys and, with query_start_loc NULL, the one query token r (num_tokens ==
  * num_reqs); otherwise the tokens [query_start_loc[r], query_start_loc[r + 1]),
- * each of which sees all of the request's keys. window > 0 (one query token
- * per request only): the last `window` keys. A row that sees no key is 0; rows
- * of tokens that belong to no request are not written. kv_lens are brought
+ * each of which sees all of the request's keys (there is no causal mask: over
+ * the decoder's own cache, of requests with at most one new token). window > 0
+ * (query_start_loc NULL only): the last `window` keys. A row that sees no key is
+ * 0; rows of tokens that belong to no request are not written. kv_lens are brought
  * into [0, max_kv_len] and to the block table's reach, query_start_loc into
  * [0, num_tokens], and a page number outside the cache is read as page 0:
  * nothing out of bounds is touched whatever these tensors hold. out may be q
