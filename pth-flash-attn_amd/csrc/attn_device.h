@@ -15,6 +15,7 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -35,6 +36,14 @@ __device__ __forceinline__ float i8_to_f32(uint32_t w, int byte) {
 
 __device__ __forceinline__ bf16x2 pack_bf16(float a, float b) {
   return __builtin_convertvector((f32x2){a, b}, bf16x2);
+}
+// Two fp32 -> a word of two 16-bit values, a low, to nearest even.
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  else
+    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
 }
 
 // Eight int8 (two dwords, byte order) -> eight bf16.

@@ -18,16 +18,6 @@
 namespace pa {
 namespace {
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if constexpr (kF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
-  else
-    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
-}
-
 template <int D, bool kF16, int kBM, int kThreads>
 __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
   constexpr int kVec = D / 4, kCrews = kThreads / kVec, kAhead = kThreads > 256 ? 8 : 4;

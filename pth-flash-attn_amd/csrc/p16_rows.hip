@@ -73,17 +73,6 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-// Two fp32 -> two 16-bit values, to nearest even.
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if constexpr (kF16)
-    return __builtin_bit_cast(uint32_t,
-                              __builtin_convertvector((f32x2){a, b}, f16x2));
-  else
-    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
-}
 template <bool kF16>
 __device__ __forceinline__ float low16(uint32_t w) {
   if constexpr (kF16) return static_cast<float>(__builtin_bit_cast(f16x2, w)[0]);

@@ -52,7 +52,6 @@ namespace pa {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef int16_t i16x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
@@ -81,14 +80,6 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if constexpr (kF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
-  else
-    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
 }
 
 // sum + the two values of a pair.

@@ -30,16 +30,6 @@ struct Write16Params {
   int32_t num_kv_heads;
 };
 
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
-template <bool kF16>
-__device__ __forceinline__ uint32_t round2(float a, float b) {
-  if constexpr (kF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
-  else
-    return __builtin_bit_cast(uint32_t, pack_bf16(a, b));
-}
-
 // Eight values of a source row as the cache holds them. kF32: fp32 values;
 // kWide: on a 16-byte address.
 template <bool kF16, bool kF32, bool kWide>
@@ -55,8 +45,8 @@ __device__ __forceinline__ u32x4 eight(const char* src) {
       a = (f32x4){x[0], x[1], x[2], x[3]};
       b = (f32x4){x[4], x[5], x[6], x[7]};
     }
-    r = (u32x4){round2<kF16>(a[0], a[1]), round2<kF16>(a[2], a[3]), round2<kF16>(b[0], b[1]),
-                round2<kF16>(b[2], b[3])};
+    r = (u32x4){pack16<kF16>(a[0], a[1]), pack16<kF16>(a[2], a[3]), pack16<kF16>(b[0], b[1]),
+                pack16<kF16>(b[2], b[3])};
   } else if constexpr (kWide) {
     r = *reinterpret_cast<const u32x4*>(src);
   } else {
