@@ -26,13 +26,16 @@ constexpr int64_t kMostSlots = 128;
 //     2            30,000       (14.6)  53.4, 49.2, 48.5
 constexpr int64_t kLeastReads = 8;
 
+// A stride of a dimension of n elements, as far as it is used.
+int64_t used(int64_t stride, int64_t n) { return n > 1 ? stride : 0; }
 bool rows_aligned(const void* p, int64_t a, int64_t b) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
 }
-bool stream_ok(const PthAttnStream& s) {
-  return rows_aligned(s.data, s.stride_block, s.stride_slot) && s.stride_head % 16 == 0 &&
-         s.stride_block >= 0 && s.stride_head >= 0 && s.stride_slot >= 0 &&
-         s.stride_slot < (1 << 24);
+bool stream_ok(const PthAttnStream& s, const PthAttnP16Args& a) {
+  const int64_t block = used(s.stride_block, a.num_blocks), slot = used(s.stride_slot, a.block_size);
+  const int64_t head = used(s.stride_head, a.num_kv_heads);
+  return rows_aligned(s.data, block, slot) && head % 16 == 0 && block >= 0 && head >= 0 &&
+         slot >= 0 && slot < (1 << 24);
 }
 CacheStream stream_of(const PthAttnStream& s) {
   return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
@@ -129,10 +132,12 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   PA_REQUIRE(a.q && a.out && a.k_cache.data && a.v_cache.data && a.kv_lens,
              "q, out, k_cache, v_cache and kv_lens must be non-NULL");
   PA_REQUIRE(a.block_table || a.block_table_width == 0, "block_table must be non-NULL");
-  PA_REQUIRE(rows_aligned(a.q, a.q_stride_token, a.q_stride_head) &&
-                 rows_aligned(a.out, a.out_stride_token, a.out_stride_head),
+  PA_REQUIRE(rows_aligned(a.q, used(a.q_stride_token, a.num_tokens),
+                          used(a.q_stride_head, a.num_q_heads)) &&
+                 rows_aligned(a.out, used(a.out_stride_token, a.num_tokens),
+                              used(a.out_stride_head, a.num_q_heads)),
              "q and out must have 16-byte aligned rows");
-  PA_REQUIRE(stream_ok(a.k_cache) && stream_ok(a.v_cache),
+  PA_REQUIRE(stream_ok(a.k_cache, a) && stream_ok(a.v_cache, a),
              "k_cache and v_cache must have 16-byte aligned rows, strides >= 0 and less than "
              "2^24 bytes between slots");
   const int32_t cus = resident_workgroups();

@@ -88,8 +88,14 @@ CacheStream stream_of(const PthAttnStream& s) {
   return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
                      s.stride_head};
 }
+// A stride of a dimension of n elements, as far as it is used.
+int64_t used(int64_t stride, int64_t n) { return n > 1 ? stride : 0; }
 bool on16(const void* p, int64_t a, int64_t b, int64_t c) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0 && c % 16 == 0;
+}
+bool cache_on16(const PthAttnStream& s, const PthAttnWrite16Args& a) {
+  return on16(s.data, used(s.stride_block, a.num_blocks), used(s.stride_slot, a.block_size),
+              used(s.stride_head, a.num_kv_heads));
 }
 
 template <int D>
@@ -135,10 +141,7 @@ int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream) {
                  a.key_stride_token % elt == 0 && a.key_stride_head % elt == 0 &&
                  a.value_stride_token % elt == 0 && a.value_stride_head % elt == 0,
              "key and value must be aligned to their element");
-  PA_REQUIRE(on16(a.k_cache.data, a.k_cache.stride_block, a.k_cache.stride_slot,
-                  a.k_cache.stride_head) &&
-                 on16(a.v_cache.data, a.v_cache.stride_block, a.v_cache.stride_slot,
-                      a.v_cache.stride_head),
+  PA_REQUIRE(cache_on16(a.k_cache, a) && cache_on16(a.v_cache, a),
              "k_cache and v_cache must have 16-byte aligned rows");
   Write16Params w{};
   w.items = static_cast<int64_t>(a.num_tokens) * a.num_kv_heads;
@@ -160,8 +163,10 @@ int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream) {
   w.num_slots = static_cast<int64_t>(a.num_blocks) * a.block_size;
   w.bs_div = Div32::make(static_cast<uint32_t>(a.block_size));
   w.heads_div = Div32::make(static_cast<uint32_t>(a.num_kv_heads));
-  const bool wide = on16(a.key, a.key_stride_token, a.key_stride_head, 0) &&
-                    on16(a.value, a.value_stride_token, a.value_stride_head, 0);
+  const bool wide = on16(a.key, used(a.key_stride_token, a.num_tokens),
+                         used(a.key_stride_head, a.num_kv_heads), 0) &&
+                    on16(a.value, used(a.value_stride_token, a.num_tokens),
+                         used(a.value_stride_head, a.num_kv_heads), 0);
   const bool f16 = a.cache_dtype == PTH_ATTN_F16;
   switch (a.head_size) {
     case 64: write16<64>(w, f16, f32, wide, stream); break;
