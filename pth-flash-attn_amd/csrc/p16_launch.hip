@@ -32,7 +32,8 @@ bool rows_aligned(const void* p, int64_t a, int64_t b) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
 }
 bool stream_ok(const PthAttnStream& s, const PthAttnP16Args& a) {
-  const int64_t block = used(s.stride_block, a.num_blocks), slot = used(s.stride_slot, a.block_size);
+  const int64_t block = used(s.stride_block, a.num_blocks);
+  const int64_t slot = used(s.stride_slot, a.block_size);
   const int64_t head = used(s.stride_head, a.num_kv_heads);
   return rows_aligned(s.data, block, slot) && head % 16 == 0 && block >= 0 && head >= 0 &&
          slot >= 0 && slot < (1 << 24);
@@ -91,7 +92,9 @@ bool whole_rows(int32_t head_size, int64_t span) {
 // 238, 239 at 500 and 341, 391 at 1,000; 16 of 2,000 255, 225 and 355, 358). At
 // D = 256, 16q / 4kv: 8 requests 38.6, 34.0 at 500, 43.5, 54.9 at 1,000; 16, three
 // quarters of the device, 58.0, 52.7; 400, whose shares are many short units,
-// 418, 445 at 500.
+// 418, 445 at 500. The bounds are bands of the units' number, not costs, and miss
+// two lines above: 64 requests at 1,500 (three rounds of units) and 20 at 2,000 are
+// cut.
 bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   const int64_t round = int64_t{p16_resident(head_size)} * cus;
   int64_t most = head_size == 256 ? 512 : 1024;
@@ -176,10 +179,13 @@ int32_t launch_p16(const PthAttnP16Args& a, hipStream_t stream) {
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
 
   // More rows than the small kernel's tile of a KV head: the other, whose tiles
-  // eight times as many rows share. 16q / 16kv of 64 against 1,500 states, 1, 8
-  // and 64 requests: of 32 rows 13.6, 17.8 and 85.9 us, the small one's row tiles
-  // 18.2, 23.6 and 130; of 16 rows 13.1, 16.7 and 81.7, 12.7, 17.5 and 76.4 with
-  // the small one.
+  // eight times as many rows share. Whole call, small kernel and wide one, 1, 8
+  // and 64 requests against 1,500 states:
+  //                    16 rows                             20 rows
+  //   16q / 16kv of 64 13.0, 13.9  18.0, 17.4  76.4, 82.1  11.8, 14.3  25.7, 16.9  117, 83.4 us
+  //   32q / 8kv of 128 13.0, 12.2  18.5, 18.3  75.1, 78.0  13.5, 12.3  27.3, 18.6  105, 78.3
+  //   16q / 4kv of 256 16.5, 16.6  22.5, 22.8  76.8, 85.7  17.4, 17.0  28.3, 23.1  119, 86.0
+  // One request at D = 64 would keep the small one.
   const bool wide = a.query_start_loc != nullptr &&
                     static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
   const int64_t bm = wide ? kP16WideRows : kP16RowsRows;

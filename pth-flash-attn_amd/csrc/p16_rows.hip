@@ -34,8 +34,8 @@
 // work-group, which so reads whole slots, 656; one work-group per compute unit
 // instead of two 626. MFMA is busy 7 % of the SIMDs' time, VALU 17 %. At short
 // lengths the bound is latency, of four dependent reads (lengths, page number,
-// K, the join's): one request to 1,024 keys 6.7 us + 2.6 of join, 16 windows of
-// 4,096 keys at D = 256 29.4 us (4.6 TB/s).
+// K, the join's): one request to 1,024 keys 6.9 us + 2.5 of join, 16 windows of
+// 4,096 keys at D = 256 29.2 us (4.6 TB/s).
 
 #include <type_traits>
 

@@ -1,7 +1,8 @@
 // p16_wide.hip -- cross attention of many query rows over a paged 16-bit
 // cache: every row of a request sees all of the request's keys. A unit is 128
 // rows of one KV head (p16.h), 32 for each of four waves, which share the key
-// tiles of 64 in LDS; two work-groups per compute unit (one at D = 256).
+// tiles of 64 in LDS; two work-groups per compute unit (three at D = 64, one at
+// D = 256).
 //
 // Layout. v_mfma_f32_32x32x16 with the keys (or the output columns) on M and
 // the wave's query rows on N: lane l holds row l % 32, and of a 32-key score
@@ -34,12 +35,13 @@
 // Bound: the matrix cores and the softmax's VALU work, which the SIMD's waves
 // run beside each other, at the clock that the power leaves. 4 prompts of 1,500
 // to 2,048 rows against 1,601 to 6,404 keys (32q / 8kv of 128, bf16, 6.7e11
-// operations), whole call: 663 to 729 us by card, 0.92 to 1.0 PFLOP/s (a library's
+// operations), whole call: 652 to 729 us by card, 0.92 to 1.03 PFLOP/s (a library's
 // 8192^3 product: 1.2); MFMA is busy 54 % of the time, VALU 46 %, without bank
 // conflicts. On the way there: 749 us before the keys' order above (fabric reads
 // 3.95 GB, now 0.52), 700 before the waits and priorities below (then 674). 4 x
-// 2,048 rows against 4,096 keys run at 0.95 PFLOP/s, 0.77 at D = 64 (the softmax is twice
-// the share) and 0.75 at D = 256 (one wave per SIMD). No faster, and so not here:
+// 2,048 rows against 4,096 keys (the card of 652): 513 to 519 us, 1.06 PFLOP/s; at
+// D = 64 320 to 325 us, 0.85 (the softmax is twice the share); at D = 256, 16q / 8kv,
+// 704 to 709 us, 0.78 (one wave per SIMD). No faster, and so not here:
 // 256 rows in two halves of four waves that take turns at the matrix cores, a
 // tile's PV products between the next one's softmax, a loop of two tiles with
 // fixed buffers, staggered starts, and, at D = 64, two tiles on their way instead

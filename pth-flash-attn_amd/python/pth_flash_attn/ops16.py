@@ -248,11 +248,11 @@ def paged_decode_fwd(
     ``q`` / ``out`` [R, Hq, D], row r request r's; query head h reads KV head
     h // (Hq / Hkv). (Where ``build_step_tables`` has packed the tokens of a step
     in which some requests bring none, ``cross_attn_fwd`` with that step's
-    ``seq_lens`` and ``query_start_loc`` takes the packed rows.) The token sees the last ``window`` (all, if 0) of the request's ``seq_lens[r]``
-    keys, its own among them; a request without keys gives zeros. What a page
-    holds outside of these keys reaches no output. A NaN or a score of +inf
-    makes its row NaN, and an infinite value its column infinite or NaN.
-    ``out`` may be ``q`` itself; other than that they share no memory (both may be
+    ``seq_lens`` and ``query_start_loc`` takes the packed rows.) The token sees the
+    last ``window`` (all, if 0) of the request's ``seq_lens[r]`` keys, its own among
+    them; a request without keys gives zeros. What a page holds outside of these
+    keys reaches no output. A NaN or a score of +inf makes its row NaN, and an
+    infinite value its column infinite or NaN. ``out`` may be ``q`` itself; other than that they share no memory (both may be
     views of one buffer, as parts of its columns; where telling that apart takes
     more than 2^16 steps, they are refused).
     ``max_seq_len`` bounds the lengths (longer ones are cut there, and at the
@@ -278,9 +278,9 @@ def cross_attn_fwd(
 
     ``q`` / ``out`` [T, Hq, D]: request r's tokens are ``query_start_loc[r]`` to
     ``query_start_loc[r + 1]``, and each sees all ``encoder_lens[r]`` keys
-    (zeros where there are none); there is no causal mask. Rows that belong to no request are left as
-    they were. ``max_query_len`` chooses kernel and split (any value is correct);
-    ``max_encoder_len``, ``ws`` and the rest are as in ``paged_decode_fwd``.
+    (zeros where there are none); there is no causal mask. Rows that belong to no
+    request are left as they were. ``max_query_len`` chooses kernel and split (any
+    value is correct); ``max_encoder_len``, ``ws`` and the rest are as in ``paged_decode_fwd``.
     """
     _op("cross_attn_fwd")(out, q, k_cache, v_cache, block_table, encoder_lens, query_start_loc,
                           max_query_len, max_encoder_len, softmax_scale, ws)

@@ -53,7 +53,8 @@ static void workspace() {
       const int64_t wgs = int64_t{cus} * p16_resident(d);
       for (int64_t rows : {1, 5, kP16RowsRows, 2 * kP16RowsRows, 4 * kP16RowsRows, kP16WideRows})
         most = std::max(most, 2 * wgs * rows * (d + 2));
-      CHECK(most + 4 * (wgs + 1) <= have, "D %d: %lld of %lld", d, (long long)most, (long long)have);
+      CHECK(most + 4 * (wgs + 1) <= have, "D %d: %lld of %lld", d, (long long)most,
+            (long long)have);
       CHECK(have - most <= kP16NoteWords * cus, "D %d: %lld floats unused", d,
             (long long)(have - most));
       std::printf("workspace %d %d %lld\n", d, cus, (long long)have);

@@ -108,7 +108,8 @@ def test_caches_that_share_memory_are_refused():
     k, v = paged16_views(kv)
     key, value = torch.zeros(3, 2, 64, dtype=BF), torch.zeros(3, 2, 64, dtype=BF)
     shifted = kv.flatten()[8:].as_strided(k[:5].shape, k.stride())
-    for a, b in ((k, k), (k[1:], k[:-1]), (k[:, :8], k[:, 4:12]), (k[:3], k[2:5]), (k[:5], shifted)):
+    for a, b in ((k, k), (k[1:], k[:-1]), (k[:, :8], k[:, 4:12]), (k[:3], k[2:5]),
+                 (k[:5], shifted)):
         assert "k_cache and v_cache must share no memory" in write(a, b, key, value)
     # One cache for both is written by one tensor for both.
     assert "must share no memory" in write(k, k, key, value)

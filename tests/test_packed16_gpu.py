@@ -19,7 +19,8 @@ I32 = dict(dtype=torch.int32, device=DEV)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("new", [[0, 1, 1, 0, 1], [1, 0, 0, 1, 1], [1, 1, 1, 1, 1], [0, 0, 0, 0, 0]])
+@pytest.mark.parametrize("new", [[0, 1, 1, 0, 1], [1, 0, 0, 1, 1], [1, 1, 1, 1, 1],
+                                 [0, 0, 0, 0, 0]])
 def test_packed_decode_step(new, D):
     Hq, Hkv, R, T = 8, 2, 5, 7  # two rows of padding or more
     ctx = [40, 15, 16, 300, 0]

@@ -10,7 +10,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from paged16_cases import DEV, assert_close, cross, decode, make_cache, queries, reference, starts_of
+from paged16_cases import (DEV, assert_close, cross, decode, make_cache, queries, reference,
+                           starts_of)
 from pth_flash_attn import capi
 
 pytestmark = pytest.mark.gpu
