@@ -278,6 +278,132 @@ typedef struct PthAttnTablesArgs {
   int32_t reserved;
 } PthAttnTablesArgs;
 
+/* Arguments of pth_attn_rotary: rotary positions. Columns [0, rot_dim) of a
+ * head are pairs (j, j + rot_dim / 2), or (2 j, 2 j + 1) if interleaved; the
+ * rest is copied. Pair j of token t turns by positions[t] * turns[j] / 2^64 of
+ * a circle (turns read as unsigned), backwards if inverse, and is multiplied by
+ * scale. A tensor may be rotated in place; other than that no output shares
+ * memory with an input or the other output. No counterpart in the reference. */
+typedef struct PthAttnRotaryArgs {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnRotaryArgs) */
+
+  const void* q; /* [num_tokens, num_q_heads, head_size]; strides in bytes */
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  const void* k; /* [num_tokens, num_kv_heads, head_size] */
+  int64_t k_stride_token;
+  int64_t k_stride_head;
+  void* q_out;
+  int64_t q_out_stride_token;
+  int64_t q_out_stride_head;
+  void* k_out;
+  int64_t k_out_stride_token;
+  int64_t k_out_stride_head;
+  const int64_t* positions; /* [num_tokens] */
+  const int64_t* turns;     /* [rot_dim / 2] */
+  int32_t dtype;            /* PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16 */
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 1 .. 1024 */
+  int32_t rot_dim;   /* even, 2 .. head_size */
+  int32_t interleaved;
+  int32_t inverse;
+  float scale;
+  int32_t reserved;
+} PthAttnRotaryArgs;
+
+/* A paged cache in 8-bit floating point (OCP e4m3) with a scale for each block
+ * of 16 slots and KV head: codes [num_blocks, block_size, num_kv_heads,
+ * head_size] (block_size a multiple of 16, rows 16-byte aligned), exponents
+ * [num_blocks, block_size / 16, num_kv_heads] contiguous. A value is code x
+ * 2^(e - 127); e = 0 stands for the scale 0, and above 246, which no writer
+ * leaves, e counts as 246. No counterpart in the reference. */
+typedef struct PthAttnCacheF8 {
+  PthAttnStream k_cache;
+  PthAttnStream v_cache;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+} PthAttnCacheF8;
+
+/* Arguments of pth_attn_write_f8. */
+typedef struct PthAttnWriteF8Args {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnWriteF8Args) */
+
+  PthAttnCacheF8 cache;
+  const void* key;   /* [num_tokens, num_kv_heads, head_size] */
+  const void* value; /* [num_tokens, num_kv_heads, head_size] */
+  int64_t key_stride_token; /* bytes */
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  const int64_t* slot_mapping; /* [num_tokens]; outside the cache: skipped */
+  int32_t kv_dtype;            /* PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16 */
+  int32_t num_tokens;
+} PthAttnWriteF8Args;
+
+/* Arguments of pth_attn_gather_f8. */
+typedef struct PthAttnGatherF8Args {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnGatherF8Args) */
+
+  PthAttnCacheF8 cache;
+  void* key;   /* [num_tokens, num_kv_heads, head_size], rows 16-byte aligned */
+  void* value; /* [num_tokens, num_kv_heads, head_size] */
+  int64_t key_stride_token; /* bytes */
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  const int32_t* block_table; /* [>= num_reqs, block_table_width] */
+  int64_t block_table_row_stride; /* ELEMENTS between rows */
+  const int32_t* row_start_loc; /* [num_reqs + 1] */
+  const int32_t* first;         /* [num_reqs] or NULL: 0 */
+  int32_t block_table_width;
+  int32_t num_reqs;
+  int32_t kv_dtype; /* PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16 */
+  int32_t num_tokens;
+} PthAttnGatherF8Args;
+
+/* Arguments of pth_attn_paged_f8: attention over such a cache. Request r's
+ * query tokens are query_start_loc[r] .. query_start_loc[r + 1] of q and out
+ * (NULL: token r alone), and its keys kv_lens[r]. Causal: the n tokens are the
+ * last n of the keys, each sees those up to its own, the last `window` of them
+ * (0: all). Not causal: each sees all keys. A row without keys is 0. */
+typedef struct PthAttnPagedF8Args {
+  int32_t abi_version;  /* = PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* = sizeof(PthAttnPagedF8Args) */
+
+  PthAttnCacheF8 cache;
+  const void* q; /* [num_tokens, num_q_heads, head_size]; strides in bytes */
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  void* out; /* as q */
+  int64_t out_stride_token;
+  int64_t out_stride_head;
+  const int32_t* block_table; /* [>= num_reqs, block_table_width] */
+  int64_t block_table_row_stride; /* ELEMENTS between rows */
+  const int32_t* kv_lens;         /* [num_reqs] */
+  const int32_t* query_start_loc; /* [num_reqs + 1] or NULL */
+  int32_t block_table_width;
+  int32_t max_kv_len; /* no request has more keys */
+  int32_t dtype;      /* of q and out: PTH_ATTN_F16 or PTH_ATTN_BF16 */
+  int32_t num_reqs;
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t max_query_len; /* of a request (a choice of kernel and split only) */
+  int32_t window;        /* 0 = none; needs causal */
+  int32_t causal;
+  float softmax_scale;
+  float* ws; /* pth_attn_paged_f8_workspace_floats(head_size) floats */
+  int64_t ws_floats;
+} PthAttnPagedF8Args;
+
 /* Loader choice of pth_attn_attention_ex. Reference: attn_capi.h:32-39.
  * loader: 0 = default, 1 = separate streams (the only loader of this
  * library; 0 and 1 are the same), 2 = whole cell (not built: EINVAL). */
@@ -402,6 +528,38 @@ int32_t pth_attn_write16_args_bytes(void);
  * block_table's rows do not overlap. */
 int32_t pth_attn_step_tables(const PthAttnTablesArgs* args, void* stream);
 int32_t pth_attn_tables_args_bytes(void);
+
+/* Rotary positions of queries and keys: see PthAttnRotaryArgs. Angles are
+ * exact for every position, in 32 bits from there on; one rounding. */
+int32_t pth_attn_rotary(const PthAttnRotaryArgs* args, void* stream);
+int32_t pth_attn_rotary_args_bytes(void);
+
+/* Keys and values into a paged 8-bit cache. Of the tokens that share a slot the
+ * last counts. A block of 16 slots that gets tokens, for each head: e is the
+ * smallest exponent whose scale brings the largest finite new value within 448
+ * (at least 1, at most 246, beyond which values are cut off; 0 if all are 0),
+ * and at least the exponent that the block had, unless its first slot is
+ * written: that begins the block. Codes are rounded to nearest even, NaN for
+ * what is not finite. Where e grew, the block's other slots are brought to the
+ * new scale, rounded again; in a begun block they keep their codes. Tokens come
+ * in any order; one launch. */
+int32_t pth_attn_write_f8(const PthAttnWriteF8Args* args, void* stream);
+int32_t pth_attn_write_f8_args_bytes(void);
+
+/* Row row_start_loc[r] + i of key and value: the cached token first[r] + i of
+ * request r, rounded once. Zeros where the block table holds no page of the
+ * cache for it; rows of no request are left as they were. */
+int32_t pth_attn_gather_f8(const PthAttnGatherF8Args* args, void* stream);
+int32_t pth_attn_gather_f8_args_bytes(void);
+
+/* Attention over a paged 8-bit cache: see PthAttnPagedF8Args. At most two kernels on
+ * `stream`, no allocation, no sync. The workspace holds nothing between calls;
+ * calls that overlap in time need one each. */
+int32_t pth_attn_paged_f8(const PthAttnPagedF8Args* args, void* stream);
+int32_t pth_attn_paged_f8_args_bytes(void);
+/* Floats of its workspace at this head size on the current device, whatever
+ * the batch; 0 if there is no device. */
+int64_t pth_attn_paged_f8_workspace_floats(int32_t head_size);
 
 #ifdef __cplusplus
 } /* extern "C" */

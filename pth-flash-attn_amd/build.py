@@ -29,8 +29,9 @@ ARCH = "gfx950"
 HIP_SOURCES = ("attn_fwd.hip", "attn_staged.hip", "attn_rows.hip", "attn_wide.hip",
                "attn_paged64.hip", "attn_generic.hip", "attn_combine.hip", "attn_launch.hip",
                "attn_writer.hip", "p16_rows.hip", "p16_wide.hip", "p16_combine.hip",
-               "p16_writer.hip", "p16_launch.hip", "step_tables.hip")
-OP_SOURCES = ("torch_op.cpp", "torch_op_p16.cpp")
+               "p16_writer.hip", "p16_launch.hip", "step_tables.hip", "rotary.hip",
+               "fp8_writer.hip", "fp8_rows.hip", "fp8_wide.hip", "fp8_launch.hip")
+OP_SOURCES = ("torch_op.cpp", "torch_op_p16.cpp", "torch_op_fp8.cpp")
 # Packed fp32 VALU ops are disabled for all device code (they have given wrong
 # results on this pool); the host pass warns that it does not know the
 # feature, which is harmless.

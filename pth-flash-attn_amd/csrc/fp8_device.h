@@ -1,0 +1,61 @@
+// fp8_device.h -- device building blocks of a cache in 8-bit floating point
+// (fp8.h): scales, conversions of codes.
+
+#pragma once
+
+#include "fp8.h"
+#include "p16_device.h"
+
+namespace pa {
+namespace {
+
+// 2^(e - 127), 0 for e = 0.
+__device__ __forceinline__ float f8_scale(uint32_t e) {
+  return __builtin_bit_cast(float, min(e, static_cast<uint32_t>(kF8MostExp)) << 23);
+}
+
+// A byte of a wave-uniform address on the scalar unit, which reads the aligned
+// word that holds it (allocations are whole words).
+__device__ __forceinline__ uint32_t ld_ro_byte(const uint8_t* p) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  const uint32_t w = static_cast<uint32_t>(ld_ro(reinterpret_cast<const int32_t*>(a & ~uintptr_t{3}), 0));
+  return w >> (8 * (a & 3)) & 0xffu;
+}
+
+// Two codes of a word (its low or high half) as two 16-bit values, scaled.
+template <bool kF16>
+__device__ __forceinline__ uint32_t f8_pair_lo(uint32_t w, float scale) {
+  if constexpr (kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+}
+template <bool kF16>
+__device__ __forceinline__ uint32_t f8_pair_hi(uint32_t w, float scale) {
+  if constexpr (kF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
+}
+// Eight codes as eight 16-bit values.
+template <bool kF16>
+__device__ __forceinline__ u32x4 f8_eight(uint32_t a, uint32_t b, float scale) {
+  return (u32x4){f8_pair_lo<kF16>(a, scale), f8_pair_hi<kF16>(a, scale), f8_pair_lo<kF16>(b, scale),
+                 f8_pair_hi<kF16>(b, scale)};
+}
+// Whether a word holds a NaN code (0x7f or 0xff).
+__device__ __forceinline__ bool f8_has_nan(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+}
+// Two bf16 values, 0 for a NaN; and 1 for a NaN, 0 otherwise.
+__device__ __forceinline__ uint32_t f8_without_nan(uint32_t w) {
+  return ((w & 0x7fffu) > 0x7f80u ? 0u : w & 0xffffu) |
+         ((w & 0x7fff0000u) > 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t f8_nan_ones(uint32_t w) {
+  return ((w & 0x7fffu) > 0x7f80u ? 0x3f80u : 0u) |
+         ((w & 0x7fff0000u) > 0x7f800000u ? 0x3f800000u : 0u);
+}
+
+}  // namespace
+}  // namespace pa

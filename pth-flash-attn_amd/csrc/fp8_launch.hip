@@ -1,0 +1,207 @@
+// fp8_launch.hip -- host side of attention over a paged cache in 8-bit floating
+// point: checks, the choice of kernel, the partition's size, and the C entry
+// points.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "fp8.h"
+
+namespace pa {
+namespace {
+
+// Slots per group up to which a larger team pays, and key rows that a
+// work-group reads for each row of sums in its slots, below which the slots'
+// bytes cost more than a larger team's reads save: as p16_launch.hip has them,
+// where a key row is twice the bytes.
+constexpr int64_t kMostSlots = 128;
+constexpr int64_t kLeastReads = 16;
+
+bool rows_aligned(const void* p, int64_t a, int64_t b) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
+}
+CacheStream stream_of(const PthAttnStream& s) {
+  return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
+                     s.stride_head};
+}
+
+// Units that a work-group of the 16-row kernel computes side by side, one for
+// each wave or pair of waves: neighbours in the cache (the KV heads of NHD
+// pages), or row tiles of the same keys, as long as enough groups remain and,
+// where they are cut, their slots stay small beside the keys. `rows`: a unit's.
+int32_t team_of(const F8Params& p, int64_t span, int64_t rows, bool whole, int32_t cus) {
+  const int64_t n_rt = p.qsl ? 1 : (p.group + kP16RowsRows - 1) / kP16RowsRows;
+  const int64_t units = p.num_reqs * (p.num_kv_heads * n_rt);
+  const bool heads_adjacent = p.k.s_head < p.k.s_slot && p.v.s_head < p.v.s_slot;
+  const int64_t beside = heads_adjacent ? p.num_kv_heads * n_rt : n_rt;
+  int32_t team = beside % 4 == 0 ? 4 : beside % 2 == 0 ? 2 : 1;
+  while (team > 1 && units / team * kMostSlots < cus) team /= 2;
+  while (!whole && team > 1 && units * span < kLeastReads * 2 * team * rows * cus) team /= 2;
+  return team;
+}
+
+// The 16-row kernel's work-groups per compute unit where groups are cut.
+int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
+  return std::min<int64_t>(p16_resident(head_size), std::max<int64_t>(1, groups / cus));
+}
+
+// Whether every group is left whole, so that there is nothing to join: where
+// all are short.
+bool whole_rows(int32_t head_size, int64_t span) {
+  return span <= (head_size == 256 ? 128 : 512);
+}
+bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
+  const int64_t round = int64_t{p16_resident(head_size)} * cus;
+  int64_t most = head_size == 256 ? 512 : 1024;
+  if (units < cus / 8 || units > 8 * cus) most = head_size == 256 ? 128 : 512;
+  else if (10 * units >= 7 * round && units <= round) most = 1536;
+  return span <= most;
+}
+
+}  // namespace
+
+int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
+  clear_error();
+  PA_REQUIRE(a.abi_version == PTH_ATTN_ABI_VERSION,
+             "abi_version " + std::to_string(a.abi_version) + " != library ABI " +
+                 std::to_string(PTH_ATTN_ABI_VERSION));
+  PA_REQUIRE(a.struct_bytes == static_cast<int32_t>(sizeof(PthAttnPagedF8Args)),
+             "struct_bytes " + std::to_string(a.struct_bytes) + " != sizeof(PthAttnPagedF8Args) " +
+                 std::to_string(sizeof(PthAttnPagedF8Args)));
+  const PthAttnCacheF8& c = a.cache;
+  const std::string sizes = f8_cache_sizes(c);
+  PA_REQUIRE(sizes.empty(), sizes);
+  PA_REQUIRE(a.dtype == PTH_ATTN_F16 || a.dtype == PTH_ATTN_BF16,
+             "dtype must be PTH_ATTN_F16 or PTH_ATTN_BF16");
+  PA_REQUIRE(a.num_reqs >= 0 && a.num_tokens >= 0, "num_reqs and num_tokens must be >= 0");
+  PA_REQUIRE(a.num_q_heads >= 1 && a.num_q_heads % c.num_kv_heads == 0,
+             "num_q_heads must be a positive multiple of num_kv_heads");
+  PA_REQUIRE(a.num_q_heads / c.num_kv_heads <= 64, "at most 64 query heads per KV head");
+  PA_REQUIRE(a.query_start_loc != nullptr || a.num_tokens == a.num_reqs,
+             "without query_start_loc, num_tokens must equal num_reqs");
+  PA_REQUIRE(a.window >= 0, "window must be >= 0");
+  PA_REQUIRE(a.window == 0 || a.causal, "a window needs causal");
+  PA_REQUIRE(a.max_kv_len >= 0 && a.block_table_width >= 0,
+             "max_kv_len and block_table_width must be >= 0");
+  PA_REQUIRE(std::isfinite(a.softmax_scale) && a.softmax_scale > 0.0f,
+             "softmax_scale must be finite and > 0");
+  if (a.num_reqs == 0 || a.num_tokens == 0) return PTH_ATTN_OK;
+  PA_REQUIRE(a.q && a.out && a.kv_lens, "q, out and kv_lens must be non-NULL");
+  PA_REQUIRE(a.block_table || a.block_table_width == 0, "block_table must be non-NULL");
+  PA_REQUIRE(rows_aligned(a.q, used_stride(a.q_stride_token, a.num_tokens),
+                          used_stride(a.q_stride_head, a.num_q_heads)) &&
+                 rows_aligned(a.out, used_stride(a.out_stride_token, a.num_tokens),
+                              used_stride(a.out_stride_head, a.num_q_heads)),
+             "q and out must have 16-byte aligned rows");
+  const std::string bad = f8_cache_rows(c);
+  PA_REQUIRE(bad.empty(), bad);
+  const int32_t cus = resident_workgroups();
+  PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
+  const int64_t need = p16_workspace_floats(c.head_size, cus);
+  PA_REQUIRE(a.ws && reinterpret_cast<uintptr_t>(a.ws) % 16 == 0 && a.ws_floats >= need,
+             "ws must be 16-byte aligned and hold " + std::to_string(need) + " floats, holds " +
+                 std::to_string(a.ws_floats));
+
+  F8Params p{};
+  p.q = static_cast<const char*>(a.q);
+  p.s_q_tok = a.q_stride_token;
+  p.s_q_head = a.q_stride_head;
+  p.out = static_cast<char*>(a.out);
+  p.s_out_tok = a.out_stride_token;
+  p.s_out_head = a.out_stride_head;
+  p.k = stream_of(c.k_cache);
+  p.v = stream_of(c.v_cache);
+  p.block_table = a.block_table;
+  p.bt_stride = a.block_table_row_stride;
+  p.kv_lens = a.kv_lens;
+  p.qsl = a.query_start_loc;
+  p.ws = a.ws;
+  p.group = a.num_q_heads / c.num_kv_heads;
+  p.bs_div = Div32::make(static_cast<uint32_t>(c.block_size));
+  p.g_div = Div32::make(static_cast<uint32_t>(p.group));
+  p.num_blocks = c.num_blocks;
+  const int64_t reach = static_cast<int64_t>(a.block_table_width) * c.block_size;
+  // Key positions stay below 2^31 with a tile to spare.
+  const int64_t most = INT32_MAX - 1024;
+  p.max_keys = static_cast<int32_t>(std::min({static_cast<int64_t>(a.max_kv_len), reach, most}));
+  p.num_reqs = a.num_reqs;
+  p.num_tokens = a.num_tokens;
+  p.num_kv_heads = c.num_kv_heads;
+  p.window = a.window < p.max_keys ? a.window : 0;
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.k_exp = c.k_scale;
+  p.v_exp = c.v_scale;
+  p.n_sub = c.block_size / kF8Span;
+  p.causal = a.causal ? 1 : 0;
+
+  const bool wide = a.query_start_loc != nullptr &&
+                    static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
+  const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
+  const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
+  PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
+  // Bounds of the partition: groups of all requests, key tiles of one. A
+  // request's tokens see its last window + tokens - 1 keys.
+  const int64_t row_tiles = a.query_start_loc == nullptr
+                                ? a.num_reqs * ((p.group + bm - 1) / bm)
+                                : rows / bm + a.num_reqs;
+  const int64_t tokens = a.query_start_loc ? a.num_tokens : 1;
+  const int64_t span = p.window > 0
+                           ? std::min<int64_t>(p.max_keys, int64_t{p.window} + tokens - 1 + 15)
+                           : p.max_keys;
+  const int64_t units = row_tiles * c.num_kv_heads;
+  const bool whole =
+      wide ? whole_wide(c.head_size, span, units, cus) : whole_rows(c.head_size, span);
+  const int64_t each = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
+  p.team = wide ? 1 : team_of(p, span, std::min(bm, each * p.group), whole, cus);
+  if (whole)
+    while (p.team > 1 && units / p.team < p16_resident(c.head_size) * cus) p.team /= 2;
+  p.key_tile_log2 = wide ? 6 : 8 - (p.team >> 1);
+  if (whole)
+    while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
+  p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
+  const int64_t key_tiles =
+      std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
+  const int64_t groups =
+      a.query_start_loc == nullptr
+          ? a.num_reqs * ((row_tiles / a.num_reqs * c.num_kv_heads + p.team - 1) / p.team)
+          : units / p.team + (p.team > 1 ? a.num_reqs : 0);
+  PA_REQUIRE(units < INT32_MAX / key_tiles, "the launch exceeds 2^31 tiles");
+  const int64_t fill =
+      cus * (wide ? p16_resident(c.head_size) : rows_per_cu(c.head_size, groups, cus));
+  p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
+  if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
+  p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
+  const bool f16 = a.dtype == PTH_ATTN_F16;
+  hipError_t err = wide ? launch_f8_wide_kernel(p, f16, c.head_size, stream)
+                        : launch_f8_rows_kernel(p, f16, c.head_size, stream);
+  // Work-groups of the join per note (p16_launch.hip has the measurements).
+  const int32_t items = p.team * p.slot_rows, least = wide ? 16 : 1;
+  const int32_t y =
+      p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
+  if (err == hipSuccess && key_tiles > 1)
+    err = launch_f8_combine_kernel(p, f16, wide, c.head_size, y, stream);
+  if (err != hipSuccess)
+    return fail(PTH_ATTN_ECUDA, std::string("paged 8-bit attention launch: ") + hipGetErrorString(err));
+  return PTH_ATTN_OK;
+}
+
+}  // namespace pa
+
+extern "C" {
+
+int32_t pth_attn_paged_f8_args_bytes(void) { return static_cast<int32_t>(sizeof(PthAttnPagedF8Args)); }
+
+int64_t pth_attn_paged_f8_workspace_floats(int32_t head_size) {
+  return pth_attn_paged16_workspace_floats(head_size);
+}
+
+int32_t pth_attn_paged_f8(const PthAttnPagedF8Args* args, void* stream) {
+  if (args == nullptr) return pa::fail(PTH_ATTN_EINVAL, "args is NULL");
+  return pa::launch_paged_f8(*args, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,425 @@
+// fp8_wide.hip -- attention of many query rows over a paged cache in 8-bit
+// floating point (fp8.h): prompts and long drafts, causal or not. A unit is 128
+// rows of one KV head (p16.h), 32 for each of four waves, which share the key
+// tiles of 64 in LDS.
+//
+// Layout. As p16_wide.hip: v_mfma_f32_32x32x16 with the keys (or the output
+// columns) on M and the wave's query rows on N, K and V row-major in LDS, V read
+// by columns with ds_read_b64_tr_b16. The codes come through registers: a wave
+// loads the 16 keys of one block of scales, a tile ahead, converts them once for
+// all four waves (two values an instruction, the scale with them) and stores
+// them as 16-bit values. Conversion at the products would be done four times,
+// and products of codes would take the queries and the weights apart into codes.
+//
+// Numerics. Scores, m, l and o are 32 bits; the running maximum moves only when
+// a score passes it by 2^kSlack, so most tiles rescale nothing; P is scaled by
+// 2^-kBias, so that sums of values near the type's largest do not leave 32
+// bits. bf16: K's and V's values are exact, P is rounded once, and l sums the
+// rounded P. fp16: K's codes are exact in fp16, their scale is a factor of the
+// scores; V is in bf16, whose range its values need, and P a bf16 pair hi + lo.
+// A row does not see the keys behind its own: where one of these has a NaN in V,
+// it is taken out of the products of the tile and put back into the rows that
+// do see it.
+
+#include "fp8_device.h"
+
+namespace pa {
+namespace {
+
+template <int D>
+struct WideOf {
+  static constexpr int kPerSimd = p16_resident(D);  // a work-group has a wave on each SIMD
+  static constexpr int kQ = D / 16;       // QK products per 32 keys
+  static constexpr int kO = D / 32;       // output tiles
+  static constexpr int kRow = 2 * D;      // bytes of a key row in LDS
+  static constexpr int kCodes = D / 16;   // 16-code pieces of a row in the cache
+  static constexpr int kBuf = kP16WideKeys * kRow;
+  static constexpr int kLoads = D / 64;   // loads of a wave per tile and stream
+  // The place of 16-byte piece c of row t in LDS.
+  static __device__ __forceinline__ int k_piece(int t, int c) {
+    return c ^ (D == 64 ? (t >> 1) & 7 : t & 15);
+  }
+  static __device__ __forceinline__ int v_piece(int t, int c) {
+    return c ^ (D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2);
+  }
+};
+
+template <int D, bool kF16>
+__global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
+    const F8Params p) {
+  using W = WideOf<D>;
+  constexpr int kBM = kP16WideRows, kKT = kP16WideKeys;
+  constexpr float kSlack = 8.0f, kBias = 16.0f;
+  __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
+  __shared__ int32_t s_nan[2][kP16Waves];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r32 = lane & 31, h = lane >> 5;
+  // The work-groups of an XCD (every eighth) take neighbouring shares, so
+  // that the row tiles of one KV head read its keys from one L2.
+  const int per = p.num_wg >> 3;
+  const int wg = per * 8 == p.num_wg
+                     ? static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3)
+                     : static_cast<int>(blockIdx.x);
+  P16Cursor cur;
+  const int64_t tiles = p16_begin<kBM>(p, cur, lane);
+  if (wg == 0) p16_note_groups<kBM, D>(p, cur, lane);
+  const int takers = p16_takers(p, tiles);
+  if (wg >= takers) {
+    if (threadIdx.x == 0) p16_note_none<D>(p, wg);
+    return;
+  }
+  int64_t at = p16_share(tiles, wg, takers);
+  const int64_t end = p16_share(tiles, wg + 1, takers);
+  bool noted = false;
+
+  while (at < end) {
+    const P16Group gr = p16_locate<kBM>(p, cur, at, lane);
+    const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
+    const bool whole = take == gr.req.n_kt;
+    const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
+    const P16Unit u = p16_unit(gr.req, gr.group);
+    const int rows = min(kBM, gr.req.rows - u.rt * kBM);
+    const int row = 32 * wave + r32;
+    const bool live = row < rows;
+    int64_t token, head;
+    p16_row<kBM>(p, gr.req.q0, u, min(row, rows - 1), token, head);
+
+    // Which keys rows see: [row_lo, row_hi) the lane's; the unit's first and last
+    // row; the wave's.
+    const int len = gr.req.len, base = gr.req.base;
+    int row_lo = gr.req.lo, row_hi = len;
+    int unit_lo = row_lo, unit_hi = len, unit_most_lo = row_lo, unit_least_hi = len;
+    int wave_lo = row_lo, wave_hi = len, wave_most_lo = row_lo, wave_least_hi = len;
+    if (p.causal) {
+      const int n = p.qsl == nullptr
+                        ? 1
+                        : static_cast<int>(p.g_div.div(static_cast<uint32_t>(gr.req.rows)));
+      const auto hi_of = [&](int t) { return max(len - (n - 1 - t), 0); };
+      const auto lo_of = [&](int hi) { return p.window > 0 ? max(hi - p.window, 0) : 0; };
+      const auto token_of = [&](int r) {
+        return static_cast<int>(p.g_div.div(
+            static_cast<uint32_t>(u.rt * kBM + min(r, rows - 1))));
+      };
+      row_hi = hi_of(static_cast<int>(token) - gr.req.q0);
+      row_lo = lo_of(row_hi);
+      unit_least_hi = hi_of(token_of(0));
+      unit_hi = hi_of(token_of(kBM - 1));
+      unit_lo = lo_of(unit_least_hi);
+      unit_most_lo = lo_of(unit_hi);
+      wave_least_hi = hi_of(token_of(32 * wave));
+      wave_hi = hi_of(token_of(32 * wave + 31));
+      wave_lo = lo_of(wave_least_hi);
+      wave_most_lo = lo_of(wave_hi);
+    }
+    const bool idle = 32 * wave >= rows;  // a wave without rows only loads
+    // The piece's 64-key tiles [t0, t1) from base on, as far as the unit sees any.
+    const int log = p.key_tile_log2 - 6;
+    const int t_lo = unit_lo > base ? (unit_lo - base) >> 6 : 0;
+    const int t_hi = unit_hi > base ? (unit_hi - base + kKT - 1) >> 6 : 0;
+    const int t0 = __builtin_amdgcn_readfirstlane(max(whole ? 0 : gr.kt << log, t_lo));
+    const int t1 = __builtin_amdgcn_readfirstlane(
+        whole ? t_hi : static_cast<int>(min(static_cast<int64_t>(gr.kt + take) << log,
+                                            static_cast<int64_t>(t_hi))));
+
+    float m = kNegInf, l = 0.0f;
+    f32x16 o[W::kO];
+#pragma unroll
+    for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
+
+    const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
+    // The block of 16 keys that the wave brings of tile t: itself, or the last
+    // one; its entry of the block table.
+    const auto block = [&](int t) { return min(base + kKT * t + 16 * wave, (len - 1) & ~15); };
+    const auto page = [&](int kb) {
+      return mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
+    };
+    u32x4 kc[W::kLoads], vc[W::kLoads];
+    uint32_t ke = 0, ve = 0;
+    int32_t entry = 0;
+    const auto load = [&](int t) {
+      const int kb = block(t);
+      const int64_t id =
+          static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks) ? entry : 0;
+      const int64_t in = kb - static_cast<int32_t>(page(kb) * p.bs_div.d);
+      const char* ks = p.k.base + id * p.k.s_block + in * p.k.s_slot + u.head * p.k.s_head;
+      const char* vs = p.v.base + id * p.v.s_block + in * p.v.s_slot + u.head * p.v.s_head;
+      const int64_t e = (id * p.n_sub + in / kF8Span) * p.num_kv_heads + u.head;
+      ke = ld_ro_byte(p.k_exp + e);
+      ve = ld_ro_byte(p.v_exp + e);
+      const int most = len - 1 - kb;  // keys past the last one repeat it
+#pragma unroll
+      for (int i = 0; i < W::kLoads; ++i) {
+        const int r = (64 * i + lane) / W::kCodes, c = (64 * i + lane) % W::kCodes;
+        const uint32_t from = min(r, most);
+        kc[i] = *reinterpret_cast<const u32x4*>(
+            ks + (__umul24(from, static_cast<uint32_t>(p.k.s_slot)) + 16 * c));
+        vc[i] = *reinterpret_cast<const u32x4*>(
+            vs + (__umul24(from, static_cast<uint32_t>(p.v.s_slot)) + 16 * c));
+      }
+    };
+    const auto masked = [&](int t) {  // some row of the unit does not see all of it
+      const int k0 = base + kKT * t;
+      return k0 < unit_most_lo || k0 + kKT > unit_least_hi;
+    };
+    // The loaded tile t into buffer `buf`; the scales of K's blocks, in fp16.
+    __shared__ float s_scale[2][kP16Waves];
+    const auto store = [&](int t, int buf) {
+      char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
+      char* vd = kd + 2 * W::kBuf;
+      const float k_scale = f8_scale(ke), v_scale = f8_scale(ve);
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < W::kLoads; ++i) {
+        const int r = (64 * i + lane) / W::kCodes, c = (64 * i + lane) % W::kCodes;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          *reinterpret_cast<u32x4*>(kd + r * W::kRow + 16 * W::k_piece(r, 2 * c + e)) =
+              f8_eight<kF16>(kc[i][2 * e], kc[i][2 * e + 1], kF16 ? 1.0f : k_scale);
+          *reinterpret_cast<u32x4*>(vd + r * W::kRow + 16 * W::v_piece(r, 2 * c + e)) =
+              f8_eight<false>(vc[i][2 * e], vc[i][2 * e + 1], v_scale);
+        }
+      }
+      if (masked(t)) {
+#pragma unroll
+        for (int i = 0; i < W::kLoads; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) any |= f8_has_nan(vc[i][e]);
+        const bool nan = __ballot(any) != 0;
+        if (lane == 0) s_nan[buf][wave] = nan;
+      }
+      if (kF16 && lane == 0) s_scale[buf][wave] = k_scale;
+    };
+
+    int buf = 0;
+    lds_barrier();  // the last unit's reads of both buffers are done
+    if (t0 < t1) {
+      entry = ld_ro(table, page(block(t0)));
+      load(t0);
+      entry = ld_ro(table, page(block(min(t0 + 1, t1 - 1))));
+    }
+    u32x4 q[W::kQ];
+    {
+      const char* src = p.q + token * p.s_q_tok + head * p.s_q_head + 16 * h;
+#pragma unroll
+      for (int j = 0; j < W::kQ; ++j) {
+        q[j] = *reinterpret_cast<const u32x4*>(src + 32 * j);
+        if (!live) q[j] = (u32x4){0u, 0u, 0u, 0u};
+      }
+    }
+    if (gr.kt == 0 && (!whole || p.notes > 0)) {
+      noted |= !whole;
+      if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
+    }
+    at += take;
+    if (t0 < t1) store(t0, 0);
+
+    for (int t = t0; t < t1; ++t, buf ^= 1) {
+      lds_barrier();  // tile t is in LDS, and nobody reads tile t - 1 any more
+      const bool more = t + 1 < t1;
+      if (more) {
+        load(t + 1);
+        entry = ld_ro(table, page(block(min(t + 2, t1 - 1))));
+      }
+      const int k0 = base + kKT * t;
+      if (!idle && k0 < wave_hi && k0 + kKT > wave_lo) {
+        const char* kt = lds + buf * W::kBuf;
+        const char* vt = kt + 2 * W::kBuf;
+        // Scores: K operands four products ahead.
+        f32x16 s[2];
+        u32x4 kf[2][4];
+        const auto read_k = [&](int n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int b = e & 1, j = 2 * n + (e >> 1);
+            kf[n & 1][e] = *reinterpret_cast<const u32x4*>(kt + (32 * b + r32) * W::kRow +
+                                                           16 * W::k_piece(r32, 2 * j + h));
+          }
+        };
+        read_k(0);
+#pragma unroll
+        for (int n = 0; n < W::kQ / 2; ++n) {
+          if (n + 1 < W::kQ / 2) read_k(n + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int b = e & 1, j = 2 * n + (e >> 1);
+            if (j == 0)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+            s[b] = mfma32<kF16>(kf[n & 1][e], q[j], s[b]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // V operands of 16 keys: rows 16 i + 4 h + 0..3 and 8 further on, columns
+        // 32 j + l % 32.
+        u32x4 vf[2][W::kO];
+        const auto read_v = [&](int i) {
+          const int r0 = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+          for (int j = 0; j < W::kO; ++j) {
+            const int byte = 64 * j + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+            const char* a =
+                vt + (16 * i + r0) * W::kRow + 16 * W::v_piece(r0, byte >> 4) + (byte & 15);
+            const u32x2 x = column4(a), y = column4(a + 8 * W::kRow);
+            vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
+          }
+        };
+        // The softmax goes before the products of the SIMD's other waves.
+        __builtin_amdgcn_s_setprio(2);
+        read_v(0);
+        if constexpr (kF16) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] *= s_scale[buf][2 * b + (i >> 3)];
+        }
+        if (k0 < wave_most_lo || k0 + kKT > wave_least_hi) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * h + (i & 3);
+              s[b][i] = key >= row_lo && key < row_hi ? s[b][i] : kNegInf;
+            }
+        }
+        float top = fmaxf(s[1][15], s[0][15]);
+#pragma unroll
+        for (int i = 0; i < 15; ++i) top = max3_raw(top, s[0][i], s[1][i]);
+        {
+          const SwapPair sw = swap_halves(top);
+          top = max_raw(sw.a, sw.b) * p.scale_log2;
+        }
+        if (__ballot(top > m + kSlack) != 0) {
+          const float next = fmaxf(m, top);
+          const float ref = next == kNegInf ? 0.0f : next;
+          float alpha = __builtin_amdgcn_exp2f(m - ref);
+          m = next;
+          // In place, as p16_wide.hip: otherwise the branch costs a copy of O in
+          // every tile. The first product needs a wait after the exp2; O's own
+          // products were issued before the scores'.
+          asm volatile("s_nop 3" : "+v"(alpha));
+          l *= alpha;
+#pragma unroll
+          for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x = o[j][i];
+              asm volatile("v_mul_f32 %0, %0, %1" : "+v"(x) : "v"(alpha));
+              o[j][i] = x;
+            }
+        }
+        const float shift = (m == kNegInf ? 0.0f : m) + kBias;
+        u32x4 pf[4], pl[kF16 ? 4 : 1];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float x0 = __builtin_amdgcn_exp2f(s[b][i] * p.scale_log2 - shift);
+            const float x1 = __builtin_amdgcn_exp2f(s[b][i + 1] * p.scale_log2 - shift);
+            const uint32_t w = pack16<false>(x0, x1);
+            pf[2 * b + (i >> 3)][(i & 7) >> 1] = w;
+            if constexpr (kF16) {
+              l += x0;
+              l += x1;
+              pl[2 * b + (i >> 3)][(i & 7) >> 1] =
+                  pack16<false>(x0 - __builtin_bit_cast(float, w << 16),
+                                x1 - __builtin_bit_cast(float, w & 0xffff0000u));
+            } else {
+              l = add_pair<false>(w, l);
+            }
+          }
+        __builtin_amdgcn_s_setprio(0);
+        bool nan = false;
+        if (masked(t)) {
+          nan = (s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3]) != 0;
+          nan = __ballot(nan) != 0;
+        }
+        if (nan) {
+#pragma unroll 1
+          for (int k = 0; k < kKT; ++k) {
+            const bool sees = k0 + k >= row_lo && k0 + k < row_hi;
+#pragma unroll
+            for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int col = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
+                const uint16_t w = *reinterpret_cast<const uint16_t*>(
+                    vt + k * W::kRow + 16 * W::v_piece(k & 15, col >> 3) + 2 * (col & 7));
+                o[j][i] = sees && (w & 0x7fffu) > 0x7f80u ? __builtin_nanf("") : o[j][i];
+              }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (i < 3) read_v(i + 1);
+          if (nan) {
+#pragma unroll
+            for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vf[i & 1][j][e] = f8_without_nan(vf[i & 1][j][e]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < W::kO; ++j) {
+            o[j] = mfma32<false>(vf[i & 1][j], pf[i], o[j]);
+            if constexpr (kF16) o[j] = mfma32<false>(vf[i & 1][j], pl[i], o[j]);
+          }
+        }
+        __builtin_amdgcn_s_setprio(1);
+      }
+      if (more) store(t + 1, buf ^ 1);
+    }
+
+    const SwapPair ls = swap_halves(l);
+    const float sum = ls.a + ls.b;
+    if (live && !whole) {
+      float* dst = p16_slot_o<D>(p, slot, 0, row) + 4 * h;
+#pragma unroll
+      for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<f32x4*>(dst + 32 * j + 8 * b) =
+              (f32x4){o[j][4 * b], o[j][4 * b + 1], o[j][4 * b + 2], o[j][4 * b + 3]};
+      if (h == 0) *reinterpret_cast<f32x2*>(p16_slot_ml<D>(p, slot, 0, row)) = (f32x2){m, sum};
+    } else if (live) {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      char* dst = p.out + token * p.s_out_tok + head * p.s_out_head + 8 * h;
+#pragma unroll
+      for (int j = 0; j < W::kO; ++j)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *reinterpret_cast<u32x2*>(dst + 64 * j + 16 * b) =
+              (u32x2){pack16<kF16>(o[j][4 * b] * inv, o[j][4 * b + 1] * inv),
+                      pack16<kF16>(o[j][4 * b + 2] * inv, o[j][4 * b + 3] * inv)};
+    }
+  }
+  if (!noted && threadIdx.x == 0) p16_note_none<D>(p, wg);
+}
+
+}  // namespace
+
+hipError_t launch_f8_wide_kernel(const F8Params& p, bool f16, int head_size, hipStream_t stream) {
+  note_kernel("f8_wide");
+  const dim3 grid(static_cast<unsigned>(p.num_wg)), block(64 * kP16Waves);
+  switch (head_size) {
+    case 64:
+      if (f16) f8_wide<64, true><<<grid, block, 0, stream>>>(p);
+      else f8_wide<64, false><<<grid, block, 0, stream>>>(p);
+      break;
+    case 256:
+      if (f16) f8_wide<256, true><<<grid, block, 0, stream>>>(p);
+      else f8_wide<256, false><<<grid, block, 0, stream>>>(p);
+      break;
+    default:
+      if (f16) f8_wide<128, true><<<grid, block, 0, stream>>>(p);
+      else f8_wide<128, false><<<grid, block, 0, stream>>>(p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace pa

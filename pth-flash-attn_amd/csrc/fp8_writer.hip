@@ -1,0 +1,502 @@
+// fp8_writer.hip -- keys and values into a paged cache in 8-bit floating point,
+// and back (fp8.h has the format).
+//
+// The writer. A block's scale depends on all its tokens of the call, which may
+// stand anywhere in slot_mapping. A work-group takes a run of tokens and one
+// KV head, puts the blocks of its tokens into a table in LDS, and reads the
+// whole of slot_mapping against it: then it knows of each of its blocks the
+// first token of the call and the last token of every slot. It takes the
+// blocks whose first token is its own, one for each wave at a time and for K
+// and V apart: the rows of up to 16 tokens in registers, their largest value
+// over the wave, the scale, the codes. So a value is read once and a code
+// written once, whatever the order of the tokens, in one launch and without
+// an atomic in memory. Rows that the block holds already are touched only if
+// its scale grows.
+//
+// The reader: a work-group finds the pages of 16 rows in LDS, then each thread
+// takes 16 codes at a time.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <string>
+
+#include "fp8_device.h"
+
+namespace pa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kWriteTokens = 128;       // of a work-group, at most
+constexpr int kTable = 2 * kWriteTokens;  // entries, a power of two, one per thread
+static_assert(kTable == kThreads, "a thread looks at each entry");
+
+struct WriteF8Params {
+  const char* src[2];  // keys, values
+  int64_t s_tok[2], s_head[2];
+  CacheStream cache[2];
+  uint8_t* scale[2];
+  const int64_t* slot_mapping;
+  int64_t num_slots;
+  Div32 sub_div;  // blocks of a page
+  int32_t n_sub;
+  int32_t num_kv_heads;
+  int32_t num_tokens;
+  int32_t tokens;  // of a work-group
+};
+
+// Eight values of a source row as 32-bit ones. kWide: on a 16-byte address.
+template <class T, bool kWide>
+__device__ __forceinline__ void load_eight(const char* src, float (&x)[8]) {
+  T y[8];
+  if constexpr (kWide) {
+    u32x4 w[sizeof(T) / 2];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const u32x4*>(src)[i];
+    __builtin_memcpy(y, w, sizeof(y));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = reinterpret_cast<const T*>(src)[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(y[i]);
+}
+
+// The smallest exponent whose scale brings the value with these bits (not
+// negative, finite) within 448 = 1.75 x 2^8; 0 for 0.
+__device__ __forceinline__ uint32_t exponent_for(uint32_t bits) {
+  if (bits == 0) return 0;
+  const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return static_cast<uint32_t>(min(max(e, 1), kF8MostExp));
+}
+
+// Four 32-bit values, within the codes' range or NaN, as codes.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  return static_cast<uint32_t>(w);
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+#pragma unroll
+  for (int i = 32; i > 0; i >>= 1) x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), i)));
+  return x;
+}
+
+template <int D, class T, bool kWide>
+__global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes, kPasses = kF8Span / kRows;
+  __shared__ int32_t s_block[kTable], s_first[kTable], s_row[kTable][kF8Span];
+  __shared__ int32_t s_list[kTable];
+  __shared__ int32_t s_count;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t0 = static_cast<int>(blockIdx.x) * p.tokens;
+  const int t1 = min(t0 + p.tokens, p.num_tokens);
+  const int head = blockIdx.y;
+
+  s_block[threadIdx.x] = -1;
+  s_first[threadIdx.x] = INT32_MAX;
+#pragma unroll
+  for (int i = 0; i < kF8Span; ++i) s_row[threadIdx.x][i] = -1;
+  if (threadIdx.x == 0) s_count = 0;
+  __syncthreads();
+  const auto place = [](int32_t block) {
+    return static_cast<int>(static_cast<uint32_t>(block) * 0x9e3779b1u >> 24) & (kTable - 1);
+  };
+  // At most half of the entries are taken: every search ends at an empty one.
+  for (int t = t0 + static_cast<int>(threadIdx.x); t < t1; t += kThreads) {
+    const int64_t slot = p.slot_mapping[t];
+    if (slot < 0 || slot >= p.num_slots) continue;
+    const int32_t block = static_cast<int32_t>(slot / kF8Span);
+    for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
+      const int32_t was = atomicCAS(&s_block[i], -1, block);
+      if (was == -1 || was == block) break;
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < p.num_tokens; t += kThreads) {
+    const int64_t slot = p.slot_mapping[t];
+    if (slot < 0 || slot >= p.num_slots) continue;
+    const int32_t block = static_cast<int32_t>(slot / kF8Span);
+    for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
+      const int32_t is = s_block[i];
+      if (is == block) {
+        atomicMin(&s_first[i], t);
+        atomicMax(&s_row[i][slot % kF8Span], t);
+      }
+      if (is == block || is == -1) break;
+    }
+  }
+  __syncthreads();
+  if (s_first[threadIdx.x] >= t0 && s_first[threadIdx.x] < t1)
+    s_list[atomicAdd(&s_count, 1)] = threadIdx.x;
+  __syncthreads();
+
+  const int c = lane % kLanes, r = lane / kLanes;
+  const int units = 2 * s_count;
+  for (int u = wave; u < units; u += kWaves) {
+    const int kv = u & 1;
+    const int entry = __builtin_amdgcn_readfirstlane(s_list[u >> 1]);
+    const int32_t block = __builtin_amdgcn_readfirstlane(s_block[entry]);
+    const int32_t page = static_cast<int32_t>(p.sub_div.div(static_cast<uint32_t>(block)));
+    const int32_t sub = block - page * p.n_sub;
+    uint8_t* exponent = p.scale[kv] + static_cast<int64_t>(block) * p.num_kv_heads + head;
+    const uint32_t had = *exponent;
+    int32_t token[kPasses];
+    float x[kPasses][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      token[i] = s_row[entry][kRows * i + r];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+      if (token[i] >= 0)
+        load_eight<T, kWide>(p.src[kv] + static_cast<int64_t>(token[i]) * p.s_tok[kv] +
+                                 static_cast<int64_t>(head) * p.s_head[kv] + 8 * sizeof(T) * c,
+                             x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
+        top = max(top, b < 0x7f800000u ? b : 0u);
+      }
+    top = wave_max(top);
+    const bool begun = s_row[entry][0] >= 0;
+    const uint32_t old = begun ? 0u : min(had, static_cast<uint32_t>(kF8MostExp));
+    const uint32_t e = max(old, exponent_for(top));
+    const float unit = e ? __builtin_bit_cast(float, (254u - e) << 23) : 0.0f;
+    const CacheStream& s = p.cache[kv];
+    char* cell = const_cast<char*>(s.base) + static_cast<int64_t>(page) * s.s_block +
+                 static_cast<int64_t>(kF8Span * sub + r) * s.s_slot +
+                 static_cast<int64_t>(head) * s.s_head + 8 * c;
+    const bool grown = !begun && e > old;
+    const float move = old && old + 127 > e ? __builtin_bit_cast(float, (old + 127u - e) << 23) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      u32x2* dst = reinterpret_cast<u32x2*>(cell + static_cast<int64_t>(kRows * i) * s.s_slot);
+      if (token[i] >= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
+          const float y = fminf(fmaxf(x[i][j] * unit, -448.0f), 448.0f);
+          x[i][j] = b < 0x7f800000u ? y : __builtin_nanf("");
+        }
+        *dst = (u32x2){codes4(x[i][0], x[i][1], x[i][2], x[i][3]),
+                       codes4(x[i][4], x[i][5], x[i][6], x[i][7])};
+      } else if (grown) {
+        const u32x2 w = *dst;
+        u32x2 y;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false);
+          const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+          y[j] = codes4(a[0] * move, a[1] * move, b[0] * move, b[1] * move);
+        }
+        *dst = y;
+      }
+    }
+    if (lane == 0 && e != had) *exponent = static_cast<uint8_t>(e);
+  }
+}
+
+struct GatherF8Params {
+  char* dst[2];
+  int64_t s_tok[2], s_head[2];
+  CacheStream cache[2];
+  const uint8_t* scale[2];
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* starts;
+  const int32_t* first;
+  int64_t reach;  // tokens that a row of the block table holds
+  Div32 bs_div, item_div;
+  int32_t n_sub, num_blocks, num_reqs, num_tokens, num_kv_heads;
+  int32_t row_items;  // 16-code pieces of a row's heads
+};
+
+constexpr int kGatherTokens = 16;
+
+template <int D, int kType>  // kType: PTH_ATTN_F32, F16 or BF16
+__global__ __launch_bounds__(kThreads) void gather_kv_f8(const GatherF8Params p) {
+  constexpr int kPieces = D / 16;
+  __shared__ int64_t s_k[kGatherTokens], s_v[kGatherTokens], s_e[kGatherTokens];
+  const int t0 = static_cast<int>(blockIdx.x) * kGatherTokens;
+  if (threadIdx.x < kGatherTokens) {
+    const int t = t0 + static_cast<int>(threadIdx.x);
+    // The last request that begins at or before the row, if it ends behind it.
+    int lo = 0, hi = p.num_reqs;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (p.starts[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    int64_t e = -2;  // -2: no request's; -1: no page
+    int64_t k = 0, v = 0;
+    if (t < p.num_tokens && lo < p.num_reqs && p.starts[lo] <= t) {
+      e = -1;
+      const int64_t pos = static_cast<int64_t>(p.first ? p.first[lo] : 0) + t -
+                          static_cast<int64_t>(p.starts[lo]);
+      if (pos >= 0 && pos < p.reach) {
+        const uint32_t entry = p.bs_div.div(static_cast<uint32_t>(pos));
+        const int32_t page = p.block_table[lo * p.bt_stride + entry];
+        if (page >= 0 && page < p.num_blocks) {
+          const int64_t in = pos - static_cast<int64_t>(entry) * p.bs_div.d;
+          k = page * p.cache[0].s_block + in * p.cache[0].s_slot;
+          v = page * p.cache[1].s_block + in * p.cache[1].s_slot;
+          e = (static_cast<int64_t>(page) * p.n_sub + in / kF8Span) * p.num_kv_heads;
+        }
+      }
+    }
+    s_k[threadIdx.x] = k;
+    s_v[threadIdx.x] = v;
+    s_e[threadIdx.x] = e;
+  }
+  __syncthreads();
+  const int items = 2 * kGatherTokens * p.row_items;
+  for (int i = threadIdx.x; i < items; i += kThreads) {
+    const int row = static_cast<int>(p.item_div.div(static_cast<uint32_t>(i)));
+    const int item = i - row * p.row_items;
+    const int kv = row & 1, t = row >> 1;
+    const int64_t e = s_e[t];
+    if (e == -2) continue;
+    const int head = item / kPieces, c = item % kPieces;
+    u32x4 w = {0u, 0u, 0u, 0u};
+    float scale = 0.0f;
+    if (e >= 0) {
+      w = *reinterpret_cast<const u32x4*>(p.cache[kv].base + (kv ? s_v[t] : s_k[t]) +
+                                          head * p.cache[kv].s_head + 16 * c);
+      scale = f8_scale(p.scale[kv][e + head]);
+    }
+    char* dst = p.dst[kv] + static_cast<int64_t>(t0 + t) * p.s_tok[kv] +
+                head * p.s_head[kv] + 16 * (kType == PTH_ATTN_F32 ? 4 : 2) * c;
+    float x[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false);
+      const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+      x[4 * j] = a[0] * scale;
+      x[4 * j + 1] = a[1] * scale;
+      x[4 * j + 2] = b[0] * scale;
+      x[4 * j + 3] = b[1] * scale;
+    }
+    if constexpr (kType == PTH_ATTN_F32) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        reinterpret_cast<f32x4*>(dst)[j] = (f32x4){x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
+    } else {
+      constexpr bool kF16 = kType == PTH_ATTN_F16;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        reinterpret_cast<u32x4*>(dst)[j] = (u32x4){
+            pack16<kF16>(x[8 * j], x[8 * j + 1]), pack16<kF16>(x[8 * j + 2], x[8 * j + 3]),
+            pack16<kF16>(x[8 * j + 4], x[8 * j + 5]), pack16<kF16>(x[8 * j + 6], x[8 * j + 7])};
+    }
+  }
+}
+
+CacheStream stream_of(const PthAttnStream& s) {
+  return CacheStream{static_cast<const char*>(s.data), s.stride_block, s.stride_slot,
+                     s.stride_head};
+}
+bool on16(const void* p, int64_t tok, int64_t n_tok, int64_t head, int64_t n_head) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && used_stride(tok, n_tok) % 16 == 0 &&
+         used_stride(head, n_head) % 16 == 0;
+}
+
+template <int D, class T>
+void write_as(const WriteF8Params& w, bool wide, dim3 grid, hipStream_t stream) {
+  if (wide) write_kv_f8<D, T, true><<<grid, kThreads, 0, stream>>>(w);
+  else write_kv_f8<D, T, false><<<grid, kThreads, 0, stream>>>(w);
+}
+template <int D>
+void write_d(const WriteF8Params& w, int dtype, bool wide, dim3 grid, hipStream_t stream) {
+  if (dtype == PTH_ATTN_F32) write_as<D, float>(w, wide, grid, stream);
+  else if (dtype == PTH_ATTN_F16) write_as<D, _Float16>(w, wide, grid, stream);
+  else write_as<D, __bf16>(w, wide, grid, stream);
+}
+template <int D>
+void gather_d(const GatherF8Params& g, int dtype, dim3 grid, hipStream_t stream) {
+  if (dtype == PTH_ATTN_F32) gather_kv_f8<D, PTH_ATTN_F32><<<grid, kThreads, 0, stream>>>(g);
+  else if (dtype == PTH_ATTN_F16) gather_kv_f8<D, PTH_ATTN_F16><<<grid, kThreads, 0, stream>>>(g);
+  else gather_kv_f8<D, PTH_ATTN_BF16><<<grid, kThreads, 0, stream>>>(g);
+}
+
+}  // namespace
+
+std::string f8_cache_sizes(const PthAttnCacheF8& c) {
+  if (c.head_size != 64 && c.head_size != 128 && c.head_size != 256)
+    return "head_size must be 64, 128 or 256";
+  if (c.num_blocks < 1 || c.num_kv_heads < 1 || c.num_kv_heads > 65535)
+    return "num_blocks >= 1, num_kv_heads 1 .. 65535";
+  if (c.block_size < kF8Span || c.block_size % kF8Span != 0)
+    return "block_size must be a positive multiple of 16";
+  if (static_cast<int64_t>(c.num_blocks) * (c.block_size / kF8Span) > INT32_MAX)
+    return "num_blocks x block_size must be less than 2^35";
+  return "";
+}
+
+std::string f8_cache_rows(const PthAttnCacheF8& c) {
+  if (!c.k_cache.data || !c.v_cache.data || !c.k_scale || !c.v_scale)
+    return "the cache's codes and scales must be non-NULL";
+  for (const PthAttnStream* s : {&c.k_cache, &c.v_cache}) {
+    const int64_t block = used_stride(s->stride_block, c.num_blocks);
+    const int64_t head = used_stride(s->stride_head, c.num_kv_heads);
+    if (reinterpret_cast<uintptr_t>(s->data) % 16 != 0 || block % 16 != 0 ||
+        s->stride_slot % 16 != 0 || head % 16 != 0 || block < 0 || head < 0 ||
+        s->stride_slot < 0 || s->stride_slot >= 1 << 24)
+      return "k_cache and v_cache must have 16-byte aligned rows, strides >= 0 and less than 2^24 "
+             "bytes between slots";
+  }
+  return "";
+}
+
+int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
+  clear_error();
+  PA_REQUIRE(a.abi_version == PTH_ATTN_ABI_VERSION,
+             "abi_version " + std::to_string(a.abi_version) + " != library ABI " +
+                 std::to_string(PTH_ATTN_ABI_VERSION));
+  PA_REQUIRE(a.struct_bytes == static_cast<int32_t>(sizeof(PthAttnWriteF8Args)),
+             "struct_bytes " + std::to_string(a.struct_bytes) + " != sizeof(PthAttnWriteF8Args) " +
+                 std::to_string(sizeof(PthAttnWriteF8Args)));
+  const std::string sizes = f8_cache_sizes(a.cache);
+  PA_REQUIRE(sizes.empty(), sizes);
+  PA_REQUIRE(a.kv_dtype == PTH_ATTN_F32 || a.kv_dtype == PTH_ATTN_F16 || a.kv_dtype == PTH_ATTN_BF16,
+             "kv_dtype must be PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16");
+  PA_REQUIRE(a.num_tokens >= 0 && a.num_tokens < 1 << 30, "num_tokens must be 0 .. 2^30 - 1");
+  if (a.num_tokens == 0) return PTH_ATTN_OK;
+  PA_REQUIRE(a.key && a.value && a.slot_mapping, "key, value and slot_mapping must be non-NULL");
+  const std::string rows = f8_cache_rows(a.cache);
+  PA_REQUIRE(rows.empty(), rows);
+  const PthAttnCacheF8& c = a.cache;
+  const int64_t elt = a.kv_dtype == PTH_ATTN_F32 ? 4 : 2;
+  PA_REQUIRE(reinterpret_cast<uintptr_t>(a.key) % elt == 0 &&
+                 reinterpret_cast<uintptr_t>(a.value) % elt == 0 &&
+                 a.key_stride_token % elt == 0 && a.key_stride_head % elt == 0 &&
+                 a.value_stride_token % elt == 0 && a.value_stride_head % elt == 0,
+             "key and value must be aligned to their element");
+  WriteF8Params w{};
+  w.src[0] = static_cast<const char*>(a.key);
+  w.src[1] = static_cast<const char*>(a.value);
+  w.s_tok[0] = a.key_stride_token;
+  w.s_tok[1] = a.value_stride_token;
+  w.s_head[0] = a.key_stride_head;
+  w.s_head[1] = a.value_stride_head;
+  w.cache[0] = stream_of(c.k_cache);
+  w.cache[1] = stream_of(c.v_cache);
+  w.scale[0] = c.k_scale;
+  w.scale[1] = c.v_scale;
+  w.slot_mapping = a.slot_mapping;
+  w.num_slots = static_cast<int64_t>(c.num_blocks) * c.block_size;
+  w.n_sub = c.block_size / kF8Span;
+  w.sub_div = Div32::make(static_cast<uint32_t>(w.n_sub));
+  w.num_kv_heads = c.num_kv_heads;
+  w.num_tokens = a.num_tokens;
+  const int32_t cus = resident_workgroups();
+  PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
+  // Fewer tokens of a work-group while that leaves compute units idle.
+  w.tokens = kWriteTokens;
+  while (w.tokens > 2 && static_cast<int64_t>(a.num_tokens) * c.num_kv_heads < int64_t{4} * cus * w.tokens)
+    w.tokens /= 2;
+  const bool wide = on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
+                    on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head, c.num_kv_heads);
+  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + w.tokens - 1) / w.tokens),
+                  static_cast<unsigned>(c.num_kv_heads));
+  switch (c.head_size) {
+    case 64: write_d<64>(w, a.kv_dtype, wide, grid, stream); break;
+    case 256: write_d<256>(w, a.kv_dtype, wide, grid, stream); break;
+    default: write_d<128>(w, a.kv_dtype, wide, grid, stream);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess)
+    return fail(PTH_ATTN_ECUDA, std::string("8-bit cache writer launch: ") + hipGetErrorString(err));
+  return PTH_ATTN_OK;
+}
+
+int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream) {
+  clear_error();
+  PA_REQUIRE(a.abi_version == PTH_ATTN_ABI_VERSION,
+             "abi_version " + std::to_string(a.abi_version) + " != library ABI " +
+                 std::to_string(PTH_ATTN_ABI_VERSION));
+  PA_REQUIRE(a.struct_bytes == static_cast<int32_t>(sizeof(PthAttnGatherF8Args)),
+             "struct_bytes " + std::to_string(a.struct_bytes) +
+                 " != sizeof(PthAttnGatherF8Args) " + std::to_string(sizeof(PthAttnGatherF8Args)));
+  const std::string sizes = f8_cache_sizes(a.cache);
+  PA_REQUIRE(sizes.empty(), sizes);
+  PA_REQUIRE(a.kv_dtype == PTH_ATTN_F32 || a.kv_dtype == PTH_ATTN_F16 || a.kv_dtype == PTH_ATTN_BF16,
+             "kv_dtype must be PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16");
+  PA_REQUIRE(a.num_tokens >= 0 && a.num_reqs >= 0 && a.block_table_width >= 0,
+             "num_tokens, num_reqs and block_table_width must be >= 0");
+  if (a.num_tokens == 0 || a.num_reqs == 0) return PTH_ATTN_OK;
+  PA_REQUIRE(a.key && a.value && a.row_start_loc, "key, value and row_start_loc must be non-NULL");
+  PA_REQUIRE(a.block_table || a.block_table_width == 0, "block_table must be non-NULL");
+  const std::string rows = f8_cache_rows(a.cache);
+  PA_REQUIRE(rows.empty(), rows);
+  const PthAttnCacheF8& c = a.cache;
+  PA_REQUIRE(on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
+                 on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head,
+                      c.num_kv_heads),
+             "key and value must have 16-byte aligned rows");
+  GatherF8Params g{};
+  g.dst[0] = static_cast<char*>(a.key);
+  g.dst[1] = static_cast<char*>(a.value);
+  g.s_tok[0] = a.key_stride_token;
+  g.s_tok[1] = a.value_stride_token;
+  g.s_head[0] = a.key_stride_head;
+  g.s_head[1] = a.value_stride_head;
+  g.cache[0] = stream_of(c.k_cache);
+  g.cache[1] = stream_of(c.v_cache);
+  g.scale[0] = c.k_scale;
+  g.scale[1] = c.v_scale;
+  g.block_table = a.block_table;
+  g.bt_stride = a.block_table_row_stride;
+  g.starts = a.row_start_loc;
+  g.first = a.first;
+  // A position is divided as 31 bits.
+  g.reach = std::min<int64_t>(int64_t{a.block_table_width} * c.block_size, INT32_MAX);
+  g.bs_div = Div32::make(static_cast<uint32_t>(c.block_size));
+  g.n_sub = c.block_size / kF8Span;
+  g.num_blocks = c.num_blocks;
+  g.num_reqs = a.num_reqs;
+  g.num_tokens = a.num_tokens;
+  g.num_kv_heads = c.num_kv_heads;
+  g.row_items = c.num_kv_heads * (c.head_size / 16);
+  g.item_div = Div32::make(static_cast<uint32_t>(g.row_items));
+  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + kGatherTokens - 1) / kGatherTokens));
+  switch (c.head_size) {
+    case 64: gather_d<64>(g, a.kv_dtype, grid, stream); break;
+    case 256: gather_d<256>(g, a.kv_dtype, grid, stream); break;
+    default: gather_d<128>(g, a.kv_dtype, grid, stream);
+  }
+  const hipError_t err = hipGetLastError();
+  if (err != hipSuccess)
+    return fail(PTH_ATTN_ECUDA, std::string("8-bit cache reader launch: ") + hipGetErrorString(err));
+  return PTH_ATTN_OK;
+}
+
+}  // namespace pa
+
+extern "C" {
+
+int32_t pth_attn_write_f8_args_bytes(void) {
+  return static_cast<int32_t>(sizeof(PthAttnWriteF8Args));
+}
+int32_t pth_attn_gather_f8_args_bytes(void) {
+  return static_cast<int32_t>(sizeof(PthAttnGatherF8Args));
+}
+
+int32_t pth_attn_write_f8(const PthAttnWriteF8Args* args, void* stream) {
+  if (args == nullptr) return pa::fail(PTH_ATTN_EINVAL, "args is NULL");
+  return pa::launch_write_f8(*args, static_cast<hipStream_t>(stream));
+}
+
+int32_t pth_attn_gather_f8(const PthAttnGatherF8Args* args, void* stream) {
+  if (args == nullptr) return pa::fail(PTH_ATTN_EINVAL, "args is NULL");
+  return pa::launch_gather_f8(*args, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

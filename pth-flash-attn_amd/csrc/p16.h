@@ -30,6 +30,7 @@
 namespace pa {
 
 struct P16Params {
+  static constexpr bool kF8 = false;
   const char* q;
   int64_t s_q_tok, s_q_head;
   char* out;
@@ -59,6 +60,16 @@ struct P16Params {
   float scale_log2;       // softmax_scale * log2(e)
 };
 
+// The same of a cache in 8-bit floating point (fp8.h): its exponents, the blocks
+// of a page, and whether a query token sees the keys up to its own alone. A row
+// without weights is 0 there (NaN over a 16-bit cache).
+struct F8Params : P16Params {
+  static constexpr bool kF8 = true;
+  const uint8_t *k_exp, *v_exp;
+  int32_t n_sub;
+  int32_t causal;
+};
+
 // A cut group: the slots that hold it (0: none is cut) and, above kP16CutShift,
 // the work-group that begins it; its request's first query token and rows, its
 // place among the request's groups.
@@ -84,8 +95,8 @@ struct P16Req {
   int32_t n_kt;  // key tiles, >= 1
 };
 
-template <int kRows>
-__device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int q0, int q1,
+template <int kRows, class P>
+__device__ __forceinline__ P16Req p16_request_of(const P& p, int r, int q0, int q1,
                                                  int len) {
   P16Req x;
   if (p.qsl == nullptr) {
@@ -97,6 +108,8 @@ __device__ __forceinline__ P16Req p16_request_of(const P16Params& p, int r, int 
   x.rows = t.count * p.group;
   x.len = min(max(len, 0), p.max_keys);
   x.lo = p.window > 0 ? max(x.len - p.window, 0) : 0;
+  if constexpr (P::kF8)
+    if (p.causal) x.lo = max(x.lo - max(t.count - 1, 0), 0);  // of the first token
   x.base = x.lo & ~15;
   x.n_rt = (x.rows + kRows - 1) / kRows;
   x.n_gr = (p.num_kv_heads * x.n_rt + p.team - 1) >> (p.team >> 1);  // / team
@@ -125,8 +138,8 @@ struct P16Count {
   int64_t tiles;
   int32_t groups;
 };
-template <int kRows>
-__device__ __forceinline__ P16Count p16_count(const P16Params& p, const P16Lane& n, int r) {
+template <int kRows, class P>
+__device__ __forceinline__ P16Count p16_count(const P& p, const P16Lane& n, int r) {
   if (r >= p.num_reqs) return {0, 0};
   const P16Req x = p16_request_of<kRows>(p, r, n.q0, n.q1, n.len);
   return {static_cast<int64_t>(x.n_gr) * x.n_kt, x.n_gr};
@@ -152,8 +165,8 @@ __device__ __forceinline__ bool p16_counted(const P16Params& p) {
 }
 
 // The cursor at the 64 requests from r0 on.
-template <int kRows>
-__device__ __forceinline__ void p16_window(const P16Params& p, P16Cursor& c, int lane) {
+template <int kRows, class P>
+__device__ __forceinline__ void p16_window(const P& p, P16Cursor& c, int lane) {
   c.of = p16_lane(p, c.r0 + lane);
   const P16Count n = p16_count<kRows>(p, c.of, c.r0 + lane);
   c.incl = wave_scan64(n.tiles, lane);
@@ -162,8 +175,8 @@ __device__ __forceinline__ void p16_window(const P16Params& p, P16Cursor& c, int
 }
 
 // All tiles of the launch; the cursor at its first window.
-template <int kRows>
-__device__ __forceinline__ int64_t p16_begin(const P16Params& p, P16Cursor& c, int lane) {
+template <int kRows, class P>
+__device__ __forceinline__ int64_t p16_begin(const P& p, P16Cursor& c, int lane) {
   c.r0 = 0;
   c.base = 0;
   c.groups = 0;
@@ -196,8 +209,8 @@ struct P16Group {
 };
 
 // The group of tile `at` (not before the cursor, and less than all tiles).
-template <int kRows>
-__device__ __forceinline__ P16Group p16_locate(const P16Params& p, P16Cursor& c, int64_t at,
+template <int kRows, class P>
+__device__ __forceinline__ P16Group p16_locate(const P& p, P16Cursor& c, int64_t at,
                                                int lane) {
   if (at >= c.end && p.num_reqs > 64) {
     // Past the 64th window, which says what all after it hold, one by one.
@@ -302,8 +315,8 @@ __device__ __forceinline__ void p16_note_none(const P16Params& p, int wg) {
 }
 // The note before the first group's: how many groups there are. By the first
 // work-group, in any case.
-template <int kRows, int D>
-__device__ __forceinline__ void p16_note_groups(const P16Params& p, const P16Cursor& c, int lane) {
+template <int kRows, int D, class P>
+__device__ __forceinline__ void p16_note_groups(const P& p, const P16Cursor& c, int lane) {
   if (!p16_counted(p)) return;
   int32_t n = __builtin_amdgcn_readlane(c.group_incl, 63);
   for (int r0 = 64; r0 < p.num_reqs; r0 += 64)
@@ -332,6 +345,8 @@ hipError_t launch_p16_wide_kernel(const P16Params& p, bool f16, bool page16, int
                                   hipStream_t stream);
 hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
                                      int y, hipStream_t stream);
+hipError_t launch_f8_combine_kernel(const F8Params& p, bool f16, bool wide, int head_size, int y,
+                                    hipStream_t stream);
 int32_t launch_write_kv16(const PthAttnWrite16Args& a, hipStream_t stream);
 int32_t launch_step_tables(const PthAttnTablesArgs& a, hipStream_t stream);
 

@@ -18,8 +18,8 @@
 namespace pa {
 namespace {
 
-template <int D, bool kF16, int kBM, int kThreads>
-__global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
+template <int D, bool kF16, int kBM, int kThreads, class P>
+__global__ __launch_bounds__(kThreads) void p16_combine(const P p) {
   constexpr int kVec = D / 4, kCrews = kThreads / kVec, kAhead = kThreads > 256 ? 8 : 4;
   __shared__ f32x4 s_o[kCrews][kVec];
   __shared__ float s_m[kCrews], s_l[kCrews];
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
         o += w * s_o[v][col];
       }
     }
-    const float inv = 1.0f / l;
+    const float inv = P::kF8 && l == 0.0f ? 0.0f : 1.0f / l;
     int64_t token, head;
     p16_row<kBM>(p, cut.q0, u, row, token, head);
     *reinterpret_cast<u32x2*>(p.out + token * p.s_out_tok + head * p.s_out_head + 8 * col) =
@@ -104,22 +104,20 @@ __global__ __launch_bounds__(kThreads) void p16_combine(const P16Params p) {
   }
 }
 
-template <int D, bool kF16>
-void combine_of(const P16Params& p, bool wide, dim3 grid, hipStream_t stream) {
+template <int D, bool kF16, class P>
+void combine_of(const P& p, bool wide, dim3 grid, hipStream_t stream) {
   if (wide) p16_combine<D, kF16, kP16WideRows, 256><<<grid, 256, 0, stream>>>(p);
   else if (p.notes > 0) p16_combine<D, kF16, kP16RowsRows, 512><<<grid, 512, 0, stream>>>(p);
   else p16_combine<D, kF16, kP16RowsRows, 256><<<grid, 256, 0, stream>>>(p);
 }
-template <int D>
-void combine(const P16Params& p, bool f16, bool wide, dim3 grid, hipStream_t stream) {
+template <int D, class P>
+void combine(const P& p, bool f16, bool wide, dim3 grid, hipStream_t stream) {
   if (f16) combine_of<D, true>(p, wide, grid, stream);
   else combine_of<D, false>(p, wide, grid, stream);
 }
-
-}  // namespace
-
-hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
-                                     int y, hipStream_t stream) {
+template <class P>
+hipError_t launch_combine(const P& p, bool f16, bool wide, int head_size, int y,
+                          hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.notes > 0 ? p.notes : p.num_wg),
                   static_cast<unsigned>(y));
   switch (head_size) {
@@ -128,6 +126,17 @@ hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, in
     default: combine<128>(p, f16, wide, grid, stream);
   }
   return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_p16_combine_kernel(const P16Params& p, bool f16, bool wide, int head_size,
+                                     int y, hipStream_t stream) {
+  return launch_combine(p, f16, wide, head_size, y, stream);
+}
+hipError_t launch_f8_combine_kernel(const F8Params& p, bool f16, bool wide, int head_size, int y,
+                                    hipStream_t stream) {
+  return launch_combine(p, f16, wide, head_size, y, stream);
 }
 
 }  // namespace pa

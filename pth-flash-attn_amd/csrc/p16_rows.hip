@@ -39,8 +39,7 @@
 
 #include <type_traits>
 
-#include "attn_device.h"
-#include "p16.h"
+#include "p16_device.h"
 
 namespace pa {
 namespace {
@@ -62,16 +61,6 @@ template <>
 struct VRun<4> { typedef u32x2 type; };
 template <>
 struct VRun<8> { typedef u32x4 type; };
-
-template <bool kF16>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (kF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
-                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 
 template <bool kF16>
 __device__ __forceinline__ float low16(uint32_t w) {

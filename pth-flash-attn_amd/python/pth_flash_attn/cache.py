@@ -145,6 +145,25 @@ def paged16_views(kv: torch.Tensor, *, layout: str = "NHD") -> tuple[torch.Tenso
     return nhd[:, 0], nhd[:, 1]
 
 
+def fp8_cache(
+    num_blocks: int, block_size: int, Hkv: int, D: int, *, layout: str = "NHD",
+    device: str | torch.device = "cuda",
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """An empty paged 8-bit cache for the ops of ``ops8``: (k_cache, v_cache,
+    k_scale, v_scale), views of one storage of codes (keys and values of a page side
+    by side) and one of scales; all values 0."""
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}")
+    if block_size < 16 or block_size % 16:
+        raise ValueError(f"block_size must be a positive multiple of 16, got {block_size}")
+    inner = (block_size, Hkv) if layout == "NHD" else (Hkv, block_size)
+    codes = torch.zeros((num_blocks, 2, *inner, D), dtype=torch.uint8, device=device)
+    codes = codes.view(torch.float8_e4m3fn)
+    nhd = codes if layout == "NHD" else codes.transpose(2, 3)
+    scale = torch.zeros((2, num_blocks, block_size // 16, Hkv), dtype=torch.uint8, device=device)
+    return nhd[:, 0], nhd[:, 1], scale[0], scale[1]
+
+
 @dataclass
 class PagedCache:
     """A filled cache plus the per-request metadata the op needs."""

@@ -47,6 +47,15 @@ EXPORTED_SYMBOLS = (
     "pth_attn_write16_args_bytes",
     "pth_attn_step_tables",
     "pth_attn_tables_args_bytes",
+    "pth_attn_rotary",
+    "pth_attn_rotary_args_bytes",
+    "pth_attn_write_f8",
+    "pth_attn_write_f8_args_bytes",
+    "pth_attn_gather_f8",
+    "pth_attn_gather_f8_args_bytes",
+    "pth_attn_paged_f8",
+    "pth_attn_paged_f8_args_bytes",
+    "pth_attn_paged_f8_workspace_floats",
 )
 
 
@@ -240,6 +249,119 @@ class PthAttnTablesArgs(ctypes.Structure):
     ]
 
 
+class PthAttnRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p),
+        ("k_out_stride_token", ctypes.c_int64),
+        ("k_out_stride_head", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("turns", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("rot_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class PthAttnCacheF8(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+    ]
+
+
+class PthAttnWriteF8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("cache", PthAttnCacheF8),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("slot_mapping", ctypes.c_void_p),
+        ("kv_dtype", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+    ]
+
+
+class PthAttnGatherF8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("cache", PthAttnCacheF8),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("row_start_loc", ctypes.c_void_p),
+        ("first", ctypes.c_void_p),
+        ("block_table_width", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("kv_dtype", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+    ]
+
+
+class PthAttnPagedF8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("cache", PthAttnCacheF8),
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("block_table_width", ctypes.c_int32),
+        ("max_kv_len", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("max_query_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("ws", ctypes.c_void_p),
+        ("ws_floats", ctypes.c_int64),
+    ]
+
+
 class AttnLib:
     """The loaded libpth_attn.so with typed entry points."""
 
@@ -262,6 +384,10 @@ class AttnLib:
             "pth_attn_paged16_args_bytes",
             "pth_attn_write16_args_bytes",
             "pth_attn_tables_args_bytes",
+            "pth_attn_rotary_args_bytes",
+            "pth_attn_write_f8_args_bytes",
+            "pth_attn_gather_f8_args_bytes",
+            "pth_attn_paged_f8_args_bytes",
         ):
             getattr(lib, name).restype = i32
             getattr(lib, name).argtypes = []
@@ -293,11 +419,16 @@ class AttnLib:
         lib.pth_attn_write_kv.argtypes = [ctypes.POINTER(PthAttnWriteArgs), vp]
         for name, args in (("pth_attn_paged16", PthAttnP16Args),
                            ("pth_attn_write_kv16", PthAttnWrite16Args),
-                           ("pth_attn_step_tables", PthAttnTablesArgs)):
+                           ("pth_attn_step_tables", PthAttnTablesArgs),
+                           ("pth_attn_rotary", PthAttnRotaryArgs),
+                           ("pth_attn_write_f8", PthAttnWriteF8Args),
+                           ("pth_attn_gather_f8", PthAttnGatherF8Args),
+                           ("pth_attn_paged_f8", PthAttnPagedF8Args)):
             getattr(lib, name).restype = i32
             getattr(lib, name).argtypes = [ctypes.POINTER(args), vp]
-        lib.pth_attn_paged16_workspace_floats.restype = ctypes.c_int64
-        lib.pth_attn_paged16_workspace_floats.argtypes = [i32]
+        for name in ("pth_attn_paged16_workspace_floats", "pth_attn_paged_f8_workspace_floats"):
+            getattr(lib, name).restype = ctypes.c_int64
+            getattr(lib, name).argtypes = [i32]
         self.lib = lib
 
     def paged16(self, args: PthAttnP16Args, stream: int | None = None) -> int:
@@ -311,6 +442,22 @@ class AttnLib:
     def step_tables(self, args: PthAttnTablesArgs, stream: int | None = None) -> int:
         """A step's block tables and slot map (see the header)."""
         return self.lib.pth_attn_step_tables(ctypes.byref(args), stream)
+
+    def rotary(self, args: PthAttnRotaryArgs, stream: int | None = None) -> int:
+        """Rotary positions of queries and keys (see the header)."""
+        return self.lib.pth_attn_rotary(ctypes.byref(args), stream)
+
+    def write_f8(self, args: PthAttnWriteF8Args, stream: int | None = None) -> int:
+        """The 8-bit cache's writer (see the header)."""
+        return self.lib.pth_attn_write_f8(ctypes.byref(args), stream)
+
+    def gather_f8(self, args: PthAttnGatherF8Args, stream: int | None = None) -> int:
+        """The 8-bit cache's reader (see the header)."""
+        return self.lib.pth_attn_gather_f8(ctypes.byref(args), stream)
+
+    def paged_f8(self, args: PthAttnPagedF8Args, stream: int | None = None) -> int:
+        """Attention over a paged 8-bit cache (see the header)."""
+        return self.lib.pth_attn_paged_f8(ctypes.byref(args), stream)
 
     def write_kv(self, args: PthAttnWriteArgs, stream: int | None = None) -> int:
         """The int8 cache writer (see include/pth_attn.h)."""
@@ -542,4 +689,94 @@ def tables_args(*, block_table: Any, slot_mapping: Any, seq_lens: Any, query_sta
     a.context_lens, a.query_lens = context_lens.data_ptr(), query_lens.data_ptr()
     a.free_pages, a.num_free = free_pages.data_ptr(), int(free_pages.numel())
     a.num_reqs = int(context_lens.shape[0])
+    return a
+
+
+def rotary_args(*, q_out: Any, k_out: Any, q: Any, k: Any, positions: Any, turns: Any,
+                interleaved: bool = False, scale: float = 1.0,
+                inverse: bool = False) -> PthAttnRotaryArgs:
+    """PthAttnRotaryArgs of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnRotaryArgs()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(PthAttnRotaryArgs)
+    for name, t in (("q", q), ("k", k), ("q_out", q_out), ("k_out", k_out)):
+        setattr(a, name, t.data_ptr())
+        setattr(a, f"{name}_stride_token", _bstride(t, 0))
+        setattr(a, f"{name}_stride_head", _bstride(t, 1))
+    a.positions, a.turns = positions.data_ptr(), turns.data_ptr()
+    a.dtype = _dtype_code(q.dtype)
+    a.num_tokens, a.num_q_heads, a.head_size = (int(x) for x in q.shape)
+    a.num_kv_heads = int(k.shape[1])
+    a.rot_dim = 2 * int(turns.shape[0])
+    a.interleaved, a.inverse, a.scale = int(interleaved), int(inverse), scale
+    return a
+
+
+def cache_f8(*, k_cache: Any, v_cache: Any, k_scale: Any, v_scale: Any) -> PthAttnCacheF8:
+    """PthAttnCacheF8 of torch tensors (raw pointers: keep the tensors alive)."""
+    c = PthAttnCacheF8()
+    c.k_cache, c.v_cache = _stream(k_cache), _stream(v_cache)
+    c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    c.num_blocks, c.block_size, c.num_kv_heads, c.head_size = (int(x) for x in k_cache.shape)
+    return c
+
+
+def _rows_f8(a: Any, key: Any, value: Any) -> None:
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(type(a))
+    a.key, a.value = key.data_ptr(), value.data_ptr()
+    a.key_stride_token, a.key_stride_head = _bstride(key, 0), _bstride(key, 1)
+    a.value_stride_token, a.value_stride_head = _bstride(value, 0), _bstride(value, 1)
+    a.kv_dtype = _dtype_code(key.dtype)
+    a.num_tokens = int(key.shape[0])
+
+
+def write_f8_args(*, key: Any, value: Any, slot_mapping: Any, **cache: Any) -> PthAttnWriteF8Args:
+    """PthAttnWriteF8Args of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnWriteF8Args()
+    _rows_f8(a, key, value)
+    a.cache = cache_f8(**cache)
+    a.slot_mapping = slot_mapping.data_ptr()
+    return a
+
+
+def gather_f8_args(*, key: Any, value: Any, block_table: Any, row_start_loc: Any,
+                   first: Any = None, **cache: Any) -> PthAttnGatherF8Args:
+    """PthAttnGatherF8Args of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnGatherF8Args()
+    _rows_f8(a, key, value)
+    a.cache = cache_f8(**cache)
+    a.block_table = block_table.data_ptr()
+    a.block_table_row_stride = int(block_table.stride(0))
+    a.block_table_width = int(block_table.shape[1])
+    a.row_start_loc = row_start_loc.data_ptr()
+    a.first = None if first is None else first.data_ptr()
+    a.num_reqs = int(row_start_loc.shape[0]) - 1
+    return a
+
+
+def paged_f8_args(*, q: Any, out: Any, block_table: Any, kv_lens: Any, max_kv_len: int,
+                  softmax_scale: float, ws: Any, query_start_loc: Any = None,
+                  max_query_len: int = 1, window: int = 0, causal: bool = True,
+                  **cache: Any) -> PthAttnPagedF8Args:
+    """PthAttnPagedF8Args of torch tensors (raw pointers: keep the tensors alive)."""
+    a = PthAttnPagedF8Args()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(PthAttnPagedF8Args)
+    a.cache = cache_f8(**cache)
+    a.q, a.out = q.data_ptr(), out.data_ptr()
+    a.q_stride_token, a.q_stride_head = _bstride(q, 0), _bstride(q, 1)
+    a.out_stride_token, a.out_stride_head = _bstride(out, 0), _bstride(out, 1)
+    a.block_table = block_table.data_ptr()
+    a.block_table_row_stride = int(block_table.stride(0))
+    a.block_table_width = int(block_table.shape[1])
+    a.max_kv_len = max_kv_len
+    a.kv_lens = kv_lens.data_ptr()
+    a.query_start_loc = None if query_start_loc is None else query_start_loc.data_ptr()
+    a.dtype = _dtype_code(q.dtype)
+    a.num_reqs = int(kv_lens.shape[0])
+    a.num_tokens, a.num_q_heads = int(q.shape[0]), int(q.shape[1])
+    a.max_query_len, a.window, a.causal = max_query_len, window, int(causal)
+    a.softmax_scale = softmax_scale
+    a.ws, a.ws_floats = ws.data_ptr(), int(ws.numel())
     return a

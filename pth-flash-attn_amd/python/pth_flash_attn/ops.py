@@ -21,7 +21,13 @@ from pathlib import Path
 
 import torch
 
-from pth_flash_attn import ops16
+from pth_flash_attn import ops8, ops16
+from pth_flash_attn.ops8 import (  # noqa: F401  (rotary positions, the ops of an 8-bit cache)
+    gather_cache_fp8,
+    paged_attn_fp8_fwd,
+    reshape_and_cache_fp8,
+    rotary_embedding,
+)
 from pth_flash_attn.ops16 import (  # noqa: F401  (the ops of a 16-bit cache)
     build_step_tables,
     cross_attn_fwd,
@@ -284,7 +290,7 @@ def _load_library() -> bool:
     torch.ops.load_library(str(LIBRARY_PATH))
     torch.library.register_fake(OP_QUALNAME)(pth_flash_attn_fwd_fake)
     torch.library.register_fake(WRITER_QUALNAME)(reshape_and_cache_int8_fake)
-    for name, fake in ops16.FAKES.items():
+    for name, fake in (*ops16.FAKES.items(), *ops8.FAKES.items()):
         torch.library.register_fake(f"{OP_NAMESPACE}::{name}")(fake)
     return True
 

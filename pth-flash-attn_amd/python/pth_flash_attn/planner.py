@@ -311,3 +311,10 @@ def paged16_workspace_floats(*, D: int, num_sms: int) -> int:
     d = _head_size(D)
     per_cu = PAGED16_ROWS_PER_CU[d] * (d + 2) + PAGED16_NOTE_WORDS_PER_CU
     return _host_int("num_sms", num_sms, 1) * per_cu
+
+
+def fp8_workspace_floats(*, D: int, num_sms: int) -> int:
+    """fp32 elements of the workspace of ``paged_attn_fp8_fwd``: as many as the 16-bit
+    cache's ops take at this head size, so that one workspace serves both (no
+    counterpart in the reference)."""
+    return paged16_workspace_floats(D=D, num_sms=num_sms)
