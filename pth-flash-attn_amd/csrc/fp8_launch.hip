@@ -169,7 +169,8 @@ int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
       a.query_start_loc == nullptr
           ? a.num_reqs * ((row_tiles / a.num_reqs * c.num_kv_heads + p.team - 1) / p.team)
           : units / p.team + (p.team > 1 ? a.num_reqs : 0);
-  PA_REQUIRE(units < INT32_MAX / key_tiles, "the launch exceeds 2^31 tiles");
+  // A causal unit's share is up to five tiles more than its keys (f8_tiles).
+  PA_REQUIRE(units < INT32_MAX / (key_tiles + 6), "the launch exceeds 2^31 tiles");
   const int64_t fill =
       cus * (wide ? p16_resident(c.head_size) : rows_per_cu(c.head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));

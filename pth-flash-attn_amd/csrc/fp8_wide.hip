@@ -52,6 +52,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
   constexpr float kSlack = 8.0f, kBias = 16.0f;
   __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
   __shared__ int32_t s_nan[2][kP16Waves];
+  __shared__ float s_scale[2][kP16Waves];
+  __shared__ uint16_t s_bad[W::kO][64 * kP16Waves];  // columns that a row's NaN is in
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -86,17 +88,19 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     int64_t token, head;
     p16_row<kBM>(p, gr.req.q0, u, min(row, rows - 1), token, head);
 
-    // Which keys rows see: [row_lo, row_hi) the lane's; the unit's first and last
-    // row; the wave's.
+    // The keys [row_lo, row_hi) that the lane's row sees. The piece's 64-key tiles
+    // [t0, t1) from base on, of those that the unit sees any key of; those of them in
+    // [full0, full1) are seen whole by all rows of the unit, those outside of
+    // [w0, w1) by none of the wave's, and those in [wf0, wf1) whole by all of these.
     const int len = gr.req.len, base = gr.req.base;
+    const bool idle = 32 * wave >= rows;  // a wave without rows only loads
     int row_lo = gr.req.lo, row_hi = len;
-    int unit_lo = row_lo, unit_hi = len, unit_most_lo = row_lo, unit_least_hi = len;
-    int wave_lo = row_lo, wave_hi = len, wave_most_lo = row_lo, wave_least_hi = len;
-    if (p.causal) {
+    int t0 = 0, t1, full0, full1, w0, w1, wf0, wf1;
+    {
       const int n = p.qsl == nullptr
                         ? 1
                         : static_cast<int>(p.g_div.div(static_cast<uint32_t>(gr.req.rows)));
-      const auto hi_of = [&](int t) { return max(len - (n - 1 - t), 0); };
+      const auto hi_of = [&](int t) { return p.causal ? max(len - (n - 1 - t), 0) : len; };
       const auto lo_of = [&](int hi) { return p.window > 0 ? max(hi - p.window, 0) : 0; };
       const auto token_of = [&](int r) {
         return static_cast<int>(p.g_div.div(
@@ -104,26 +108,27 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       };
       row_hi = hi_of(static_cast<int>(token) - gr.req.q0);
       row_lo = lo_of(row_hi);
-      unit_least_hi = hi_of(token_of(0));
-      unit_hi = hi_of(token_of(kBM - 1));
-      unit_lo = lo_of(unit_least_hi);
-      unit_most_lo = lo_of(unit_hi);
-      wave_least_hi = hi_of(token_of(32 * wave));
-      wave_hi = hi_of(token_of(32 * wave + 31));
-      wave_lo = lo_of(wave_least_hi);
-      wave_most_lo = lo_of(wave_hi);
+      // First tile of the keys from `key` on, and one past the last of those before.
+      const auto down = [&](int key) { return key > base ? (key - base) >> 6 : 0; };
+      const auto up = [&](int key) { return key > base ? (key - base + kKT - 1) >> 6 : 0; };
+      const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+      const int u_first = hi_of(token_of(0)), u_last = hi_of(token_of(kBM - 1));
+      const int w_first = hi_of(token_of(32 * wave)), w_last = hi_of(token_of(32 * wave + 31));
+      const int log = p.key_tile_log2 - 6;
+      // A piece is tiles of those that the unit sees; whole ones are one "tile".
+      const int first = down(lo_of(u_first)), last = up(u_last);
+      t0 = uniform(first + (whole ? 0 : gr.kt << log));
+      t1 = uniform(whole ? last : min(first + ((gr.kt + take) << log), last));
+      full0 = uniform(up(lo_of(u_last)));
+      full1 = uniform(down(u_first));
+      w0 = uniform(idle ? INT32_MAX : down(lo_of(w_first)));
+      w1 = uniform(up(w_last));
+      wf0 = uniform(up(lo_of(w_last)));
+      wf1 = uniform(down(w_first));
     }
-    const bool idle = 32 * wave >= rows;  // a wave without rows only loads
-    // The piece's 64-key tiles [t0, t1) from base on, as far as the unit sees any.
-    const int log = p.key_tile_log2 - 6;
-    const int t_lo = unit_lo > base ? (unit_lo - base) >> 6 : 0;
-    const int t_hi = unit_hi > base ? (unit_hi - base + kKT - 1) >> 6 : 0;
-    const int t0 = __builtin_amdgcn_readfirstlane(max(whole ? 0 : gr.kt << log, t_lo));
-    const int t1 = __builtin_amdgcn_readfirstlane(
-        whole ? t_hi : static_cast<int>(min(static_cast<int64_t>(gr.kt + take) << log,
-                                            static_cast<int64_t>(t_hi))));
 
     float m = kNegInf, l = 0.0f;
+    bool bad = false;
     f32x16 o[W::kO];
 #pragma unroll
     for (int j = 0; j < W::kO; ++j)
@@ -132,58 +137,64 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 
     const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
     // The block of 16 keys that the wave brings of tile t: itself, or the last
-    // one; its entry of the block table.
+    // one. Lane i knows that of tile window + i.
     const auto block = [&](int t) { return min(base + kKT * t + 16 * wave, (len - 1) & ~15); };
-    const auto page = [&](int kb) {
-      return mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
+    int window = t0;
+    F8Window w;
+    const auto refill = [&](int t) {
+      window = t;
+      w = f8_window(p, table, u.head, block(t + lane));
     };
+    // Lane: 16 codes from column 16 c on of row r and of every kStep-th after it.
+    constexpr int kStep = 64 / W::kCodes;
+    const int r0 = lane / W::kCodes, c0 = lane % W::kCodes;
     u32x4 kc[W::kLoads], vc[W::kLoads];
     uint32_t ke = 0, ve = 0;
-    int32_t entry = 0;
     const auto load = [&](int t) {
-      const int kb = block(t);
-      const int64_t id =
-          static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks) ? entry : 0;
-      const int64_t in = kb - static_cast<int32_t>(page(kb) * p.bs_div.d);
-      const char* ks = p.k.base + id * p.k.s_block + in * p.k.s_slot + u.head * p.k.s_head;
-      const char* vs = p.v.base + id * p.v.s_block + in * p.v.s_slot + u.head * p.v.s_head;
-      const int64_t e = (id * p.n_sub + in / kF8Span) * p.num_kv_heads + u.head;
-      ke = ld_ro_byte(p.k_exp + e);
-      ve = ld_ro_byte(p.v_exp + e);
-      const int most = len - 1 - kb;  // keys past the last one repeat it
+      const int kb = block(t), at_lane = t - window;
+      const char* ks = f8_lane_address(w.k_lo, w.k_hi, at_lane);
+      const char* vs = f8_lane_address(w.v_lo, w.v_hi, at_lane);
+      const uint32_t e = __builtin_amdgcn_readlane(w.e, at_lane);
+      ke = e & 0xffu;
+      ve = e >> 8;
+      const uint32_t k_slot = static_cast<uint32_t>(p.k.s_slot);
+      const uint32_t v_slot = static_cast<uint32_t>(p.v.s_slot);
+      if (kb + kF8Span <= len) {
+        const uint32_t ko = __umul24(r0, k_slot) + 16 * c0, vo = __umul24(r0, v_slot) + 16 * c0;
 #pragma unroll
-      for (int i = 0; i < W::kLoads; ++i) {
-        const int r = (64 * i + lane) / W::kCodes, c = (64 * i + lane) % W::kCodes;
-        const uint32_t from = min(r, most);
-        kc[i] = *reinterpret_cast<const u32x4*>(
-            ks + (__umul24(from, static_cast<uint32_t>(p.k.s_slot)) + 16 * c));
-        vc[i] = *reinterpret_cast<const u32x4*>(
-            vs + (__umul24(from, static_cast<uint32_t>(p.v.s_slot)) + 16 * c));
+        for (int i = 0; i < W::kLoads; ++i) {
+          kc[i] = *reinterpret_cast<const u32x4*>(ks + static_cast<int64_t>(i * kStep) * k_slot + ko);
+          vc[i] = *reinterpret_cast<const u32x4*>(vs + static_cast<int64_t>(i * kStep) * v_slot + vo);
+        }
+      } else {  // keys past the last one repeat it
+#pragma unroll
+        for (int i = 0; i < W::kLoads; ++i) {
+          const uint32_t from = min(r0 + i * kStep, len - 1 - kb);
+          kc[i] = *reinterpret_cast<const u32x4*>(ks + (__umul24(from, k_slot) + 16 * c0));
+          vc[i] = *reinterpret_cast<const u32x4*>(vs + (__umul24(from, v_slot) + 16 * c0));
+        }
       }
     };
-    const auto masked = [&](int t) {  // some row of the unit does not see all of it
-      const int k0 = base + kKT * t;
-      return k0 < unit_most_lo || k0 + kKT > unit_least_hi;
-    };
-    // The loaded tile t into buffer `buf`; the scales of K's blocks, in fp16.
-    __shared__ float s_scale[2][kP16Waves];
+    // The loaded tile t into buffer `buf`; the scales of K's blocks, in fp16. The
+    // pieces' places differ in bits that an exclusive or or an addition sets.
     const auto store = [&](int t, int buf) {
       char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
       char* vd = kd + 2 * W::kBuf;
+      const uint32_t ka = r0 * W::kRow + 16 * W::k_piece(r0, 2 * c0);
+      const uint32_t va = r0 * W::kRow + 16 * W::v_piece(r0, 2 * c0);
       const float k_scale = f8_scale(ke), v_scale = f8_scale(ve);
-      bool any = false;
 #pragma unroll
-      for (int i = 0; i < W::kLoads; ++i) {
-        const int r = (64 * i + lane) / W::kCodes, c = (64 * i + lane) % W::kCodes;
+      for (int i = 0; i < W::kLoads; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          *reinterpret_cast<u32x4*>(kd + r * W::kRow + 16 * W::k_piece(r, 2 * c + e)) =
+          static_assert(kStep % 4 == 0 && (D == 64 || kStep * W::kLoads == 16), "bits of a row");
+          *reinterpret_cast<u32x4*>(kd + (ka ^ (16u * e) ^ (16u * (kStep * i))) + kStep * i * W::kRow) =
               f8_eight<kF16>(kc[i][2 * e], kc[i][2 * e + 1], kF16 ? 1.0f : k_scale);
-          *reinterpret_cast<u32x4*>(vd + r * W::kRow + 16 * W::v_piece(r, 2 * c + e)) =
+          *reinterpret_cast<u32x4*>(vd + va + 16 * e + kStep * i * W::kRow) =
               f8_eight<false>(vc[i][2 * e], vc[i][2 * e + 1], v_scale);
         }
-      }
-      if (masked(t)) {
+      if (t < full0 || t >= full1) {
+        bool any = false;
 #pragma unroll
         for (int i = 0; i < W::kLoads; ++i)
 #pragma unroll
@@ -197,9 +208,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     int buf = 0;
     lds_barrier();  // the last unit's reads of both buffers are done
     if (t0 < t1) {
-      entry = ld_ro(table, page(block(t0)));
+      refill(t0);
       load(t0);
-      entry = ld_ro(table, page(block(min(t0 + 1, t1 - 1))));
     }
     u32x4 q[W::kQ];
     {
@@ -220,14 +230,44 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     for (int t = t0; t < t1; ++t, buf ^= 1) {
       lds_barrier();  // tile t is in LDS, and nobody reads tile t - 1 any more
       const bool more = t + 1 < t1;
-      if (more) {
-        load(t + 1);
-        entry = ld_ro(table, page(block(min(t + 2, t1 - 1))));
-      }
       const int k0 = base + kKT * t;
-      if (!idle && k0 < wave_hi && k0 + kKT > wave_lo) {
-        const char* kt = lds + buf * W::kBuf;
-        const char* vt = kt + 2 * W::kBuf;
+      const char* kt = lds + buf * W::kBuf;
+      const char* vt = kt + 2 * W::kBuf;
+      if ((t < full0 || t >= full1) &&
+          (s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3]) != 0) {
+        // A NaN in V that not all rows see: the lane's columns of which its row sees
+        // one are noted, and the tile is rid of them.
+#pragma unroll 1
+        for (int j = 0; j < W::kO; ++j) {
+          uint32_t bits = 0;
+#pragma unroll 1
+          for (int k = max(row_lo - k0, 0); k < min(row_hi - k0, kKT); ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int col = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
+              const uint16_t w = *reinterpret_cast<const uint16_t*>(
+                  vt + k * W::kRow + 16 * W::v_piece(k & 15, col >> 3) + 2 * (col & 7));
+              bits |= (w & 0x7fffu) > 0x7f80u ? 1u << i : 0u;
+            }
+          s_bad[j][threadIdx.x] = static_cast<uint16_t>(bits | (bad ? s_bad[j][threadIdx.x] : 0u));
+        }
+        bad = true;
+        lds_barrier();
+        char* vd = lds + (buf + 2) * W::kBuf + 16 * wave * W::kRow;
+#pragma unroll
+        for (int i = 0; i < W::kRow / 64; ++i) {
+          u32x4* x = reinterpret_cast<u32x4*>(vd + 1024 * i + 16 * lane);
+          u32x4 y = *x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = f8_without_nan(y[e]);
+          *x = y;
+        }
+        lds_barrier();
+      }
+      const bool mine = t >= w0 && t < w1;
+      if (more && t + 1 - window == 64) refill(t + 1);
+      if (more && !mine) load(t + 1);
+      if (mine) {
         // Scores: K operands four products ahead.
         f32x16 s[2];
         u32x4 kf[2][4];
@@ -268,6 +308,9 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             vf[i & 1][j] = (u32x4){x[0], x[1], y[0], y[1]};
           }
         };
+        // The next tile is on its way during the softmax and the PV products, in the
+        // registers that K's operands had.
+        if (more) load(t + 1);
         // The softmax goes before the products of the SIMD's other waves.
         __builtin_amdgcn_s_setprio(2);
         read_v(0);
@@ -277,7 +320,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] *= s_scale[buf][2 * b + (i >> 3)];
         }
-        if (k0 < wave_most_lo || k0 + kKT > wave_least_hi) {
+        if (t < wf0 || t >= wf1) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -333,36 +376,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             }
           }
         __builtin_amdgcn_s_setprio(0);
-        bool nan = false;
-        if (masked(t)) {
-          nan = (s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3]) != 0;
-          nan = __ballot(nan) != 0;
-        }
-        if (nan) {
-#pragma unroll 1
-          for (int k = 0; k < kKT; ++k) {
-            const bool sees = k0 + k >= row_lo && k0 + k < row_hi;
-#pragma unroll
-            for (int j = 0; j < W::kO; ++j)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int col = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
-                const uint16_t w = *reinterpret_cast<const uint16_t*>(
-                    vt + k * W::kRow + 16 * W::v_piece(k & 15, col >> 3) + 2 * (col & 7));
-                o[j][i] = sees && (w & 0x7fffu) > 0x7f80u ? __builtin_nanf("") : o[j][i];
-              }
-          }
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __builtin_amdgcn_sched_barrier(0);
           if (i < 3) read_v(i + 1);
-          if (nan) {
-#pragma unroll
-            for (int j = 0; j < W::kO; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) vf[i & 1][j][e] = f8_without_nan(vf[i & 1][j][e]);
-          }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int j = 0; j < W::kO; ++j) {
@@ -375,6 +392,14 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       if (more) store(t + 1, buf ^ 1);
     }
 
+    if (bad) {
+#pragma unroll
+      for (int j = 0; j < W::kO; ++j) {
+        const uint32_t bits = s_bad[j][threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[j][i] = bits >> i & 1u ? __builtin_nanf("") : o[j][i];
+      }
+    }
     const SwapPair ls = swap_halves(l);
     const float sum = ls.a + ls.b;
     if (live && !whole) {

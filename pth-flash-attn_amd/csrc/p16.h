@@ -117,6 +117,47 @@ __device__ __forceinline__ P16Req p16_request_of(const P& p, int r, int q0, int 
   return x;
 }
 
+// Causal 128-row units see a different number of key tiles each: in tokens, unit
+// u's last row sees c + (128 u + 127) / G + 1 keys at most, c being the request's
+// keys before its tokens. Its share of the stream is an upper bound of that
+// whose sums over the units before m have a closed form,
+//   F(m) = floor((m G (c + 128) + 64 m (m + 1)) / 64 G),
+// within two tiles of the unit's need: F's steps are at least what the sum under
+// the floor grows by, less 1, and that leaves the need and the 63 / 64 that it is
+// rounded up by. With a window, units from the first that a bound C of what a
+// window and a unit's tokens cover is no more for have C each.
+struct F8Steps {
+  int32_t units;   // row tiles
+  int32_t linear;  // of these, the first ones that F holds for
+  int32_t cap;     // of each behind them
+  int32_t before;  // c; -1: `cap` tiles each
+};
+__device__ __forceinline__ F8Steps f8_steps(const F8Params& p, const P16Req& x) {
+  F8Steps s = {x.n_rt, 0, x.n_kt, -1};
+  if (!p.causal || p.qsl == nullptr || p.key_tile_log2 != 6) return s;
+  const int n = static_cast<int>(p.g_div.div(static_cast<uint32_t>(x.rows)));
+  s.before = max(x.len - n, 0);
+  s.linear = x.n_rt;
+  if (p.window > 0) {
+    const int per = 128 / p.group + 2;  // tokens of a unit
+    s.cap = ((p.window + per + 63) >> 6) + 2;
+    const int64_t from =
+        (static_cast<int64_t>(64 * static_cast<int64_t>(s.cap) - s.before - 128) * p.group) >> 7;
+    s.linear = static_cast<int32_t>(min(max(from, int64_t{0}), static_cast<int64_t>(x.n_rt)));
+  }
+  return s;
+}
+// Tiles of a head's units before m.
+__device__ __forceinline__ int32_t f8_tiles(const F8Params& p, const F8Steps& s, int32_t m) {
+  if (s.before < 0) return m * s.cap;
+  const int64_t l = min(m, s.linear);
+  const uint64_t sum = static_cast<uint64_t>(l * (static_cast<int64_t>(p.group) * (s.before + 128)) +
+                                             64 * l * (l + 1)) >> 6;
+  const uint32_t f = sum >> 31 == 0 ? p.g_div.div(static_cast<uint32_t>(sum))
+                                    : static_cast<uint32_t>(sum / static_cast<uint32_t>(p.group));
+  return static_cast<int32_t>(f) + max(m - s.linear, 0) * s.cap;
+}
+
 // Length and first and last query token of request `r` (r differs from lane to
 // lane; none behind the last request).
 struct P16Lane {
@@ -142,6 +183,8 @@ template <int kRows, class P>
 __device__ __forceinline__ P16Count p16_count(const P& p, const P16Lane& n, int r) {
   if (r >= p.num_reqs) return {0, 0};
   const P16Req x = p16_request_of<kRows>(p, r, n.q0, n.q1, n.len);
+  if constexpr (P::kF8 && kRows == kP16WideRows)
+    return {static_cast<int64_t>(p.num_kv_heads) * f8_tiles(p, f8_steps(p, x), x.n_rt), x.n_gr};
   return {static_cast<int64_t>(x.n_gr) * x.n_kt, x.n_gr};
 }
 
@@ -241,6 +284,27 @@ __device__ __forceinline__ P16Group p16_locate(const P& p, P16Cursor& c, int64_t
                                 __builtin_amdgcn_readlane(c.of.len, j));
   // Within a request: less than 2^31 tiles, by the launcher's check.
   const uint32_t in_req = static_cast<uint32_t>(local - before);
+  if constexpr (P::kF8 && kRows == kP16WideRows) {
+    const F8Steps s = f8_steps(p, u.req);
+    const uint32_t per_head = static_cast<uint32_t>(f8_tiles(p, s, s.units));
+    const int32_t head =
+        __builtin_amdgcn_readfirstlane(static_cast<int32_t>(in_req / max(per_head, 1u)));
+    const int32_t pos = static_cast<int32_t>(in_req) - head * static_cast<int32_t>(per_head);
+    // The last unit that begins at or before it, among 64 at a time.
+    int32_t unit = 0;
+    for (int32_t step = (s.units + 63) >> 6;; step = (step + 63) >> 6) {
+      const int32_t at_lane = min(unit + lane * step, s.units);
+      const bool begun = at_lane < s.units && f8_tiles(p, s, at_lane) <= pos;
+      unit = __builtin_amdgcn_readfirstlane(
+          unit + (static_cast<int32_t>(__popcll(__ballot(begun))) - 1) * step);
+      if (step == 1) break;
+    }
+    const int32_t first = f8_tiles(p, s, unit);
+    u.group = head * u.req.n_rt + unit;
+    u.kt = __builtin_amdgcn_readfirstlane(pos - first);
+    u.req.n_kt = __builtin_amdgcn_readfirstlane(f8_tiles(p, s, unit + 1) - first);
+    return u;
+  }
   const uint32_t n_kt = static_cast<uint32_t>(u.req.n_kt);
   u.group = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(in_req / n_kt));
   u.kt = __builtin_amdgcn_readfirstlane(static_cast<int32_t>(in_req)) -
