@@ -22,35 +22,40 @@ __device__ __forceinline__ uint32_t ld_ro_byte(const uint8_t* p) {
   return w >> (8 * (a & 3)) & 0xffu;
 }
 
-// Blocks of 16 keys, one to each lane: where the block of the keys from `kb` on
-// (kb a multiple of 16, within the table) begins in K and in V, and its exponents.
-// A wave makes these for 64 blocks at once and takes one with a few lane reads:
-// page numbers, products of strides and scales worked out block by block on the
-// scalar unit are some 100 instructions each.
-struct F8Window {
-  uint32_t k_lo, k_hi, v_lo, v_hi;
-  uint32_t e;  // of K, and of V above bit 8
+// Where a block of 16 keys begins in K and in V, and its exponents (K's, and V's
+// above bit 8). The lanes of a wave make these for 64 blocks at once, kept in LDS or
+// in registers: page numbers, products of strides and scales worked out block by
+// block on the scalar unit are some 100 instructions each.
+struct F8Block {
+  uint64_t k, v;
+  uint32_t e;
 };
-__device__ __forceinline__ F8Window f8_window(const F8Params& p, const int32_t* table,
-                                              int32_t head, int32_t kb) {
+// The block of the keys from `kb` on: a multiple of 16, within the table.
+__device__ __forceinline__ F8Block f8_block(const F8Params& p, const int32_t* table, int32_t head,
+                                            int32_t kb) {
   const uint32_t page = mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
   const int32_t entry = table[page];
   const int64_t id =
       static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks) ? entry : 0;
   const int32_t in = kb - static_cast<int32_t>(page * p.bs_div.d);
-  const uint64_t k = reinterpret_cast<uint64_t>(p.k.base + head * p.k.s_head) + id * p.k.s_block +
-                     static_cast<uint64_t>(in) * static_cast<uint32_t>(p.k.s_slot);
-  const uint64_t v = reinterpret_cast<uint64_t>(p.v.base + head * p.v.s_head) + id * p.v.s_block +
-                     static_cast<uint64_t>(in) * static_cast<uint32_t>(p.v.s_slot);
+  F8Block b;
+  b.k = reinterpret_cast<uint64_t>(p.k.base + head * p.k.s_head) + id * p.k.s_block +
+        static_cast<uint64_t>(in) * static_cast<uint32_t>(p.k.s_slot);
+  b.v = reinterpret_cast<uint64_t>(p.v.base + head * p.v.s_head) + id * p.v.s_block +
+        static_cast<uint64_t>(in) * static_cast<uint32_t>(p.v.s_slot);
   const int64_t e = (id * p.n_sub + in / kF8Span) * p.num_kv_heads + head;
-  return {static_cast<uint32_t>(k), static_cast<uint32_t>(k >> 32), static_cast<uint32_t>(v),
-          static_cast<uint32_t>(v >> 32),
-          static_cast<uint32_t>(p.k_exp[e]) | static_cast<uint32_t>(p.v_exp[e]) << 8};
+  b.e = static_cast<uint32_t>(p.k_exp[e]) | static_cast<uint32_t>(p.v_exp[e]) << 8;
+  return b;
 }
-__device__ __forceinline__ const char* f8_lane_address(uint32_t lo, uint32_t hi, int lane) {
+// A wave's blocks in LDS.
+struct F8Window {
+  u32x4 address[64];  // of K, of V
+  uint32_t e[64];
+};
+__device__ __forceinline__ const char* f8_uniform(uint32_t lo, uint32_t hi) {
   return reinterpret_cast<const char*>(
-      static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, lane))) |
-      static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(hi, lane))) << 32);
+      static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lo))) |
+      static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(hi))) << 32);
 }
 
 // Two codes of a word (its low or high half) as two 16-bit values, scaled.

@@ -35,12 +35,24 @@ struct WideOf {
   static constexpr int kCodes = D / 16;   // 16-code pieces of a row in the cache
   static constexpr int kBuf = kP16WideKeys * kRow;
   static constexpr int kLoads = D / 64;   // loads of a wave per tile and stream
-  // The place of 16-byte piece c of row t in LDS.
+  // Whether the next tile is stored between the PV products, or behind them.
+  static constexpr bool kBetween = D != 256;
+  // The place of 16-byte piece c of row t in LDS. Stores of 8 lanes, every second
+  // piece of a row, take all 32 banks, reads (the same piece of 16 rows of K, four
+  // of 4 rows of V) all 64.
   static __device__ __forceinline__ int k_piece(int t, int c) {
-    return c ^ (D == 64 ? (t >> 1) & 7 : t & 15);
+    if constexpr (D == 64) return c ^ (t & 1) ^ ((t >> 1) & 7);
+    return (((c >> 1) & 7) ^ (t & 7)) | ((c ^ (t >> 3)) & 1) << 3 | (c >> 4) << 4;
   }
   static __device__ __forceinline__ int v_piece(int t, int c) {
-    return c ^ (D == 64 ? ((t >> 1) & 1) << 2 : (t & 3) << 2);
+    if constexpr (D == 64) return ((c >> 1) ^ (t & 2)) | ((c ^ t) & 1) << 2;
+    return (((c >> 1) & 7) ^ 2 * (t & 3)) | ((c ^ t) & 1) << 3 | (c >> 4) << 4;
+  }
+  // A piece and the next, apart.
+  static constexpr uint32_t kOddK = D == 64 ? 16 : 128, kOddV = D == 64 ? 64 : 128;
+  // In K, a row and the i-th after it that a lane stores, apart.
+  static __device__ __forceinline__ uint32_t k_row(int i) {
+    return D == 128 ? 128u * i : 64u * (i & 1) | 128u * (i >> 1);
   }
 };
 
@@ -51,6 +63,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
   constexpr int kBM = kP16WideRows, kKT = kP16WideKeys;
   constexpr float kSlack = 8.0f, kBias = 16.0f;
   __shared__ __attribute__((aligned(16))) char lds[4 * W::kBuf];  // K, K, V, V
+  __shared__ F8Window s_window[kP16Waves];
   __shared__ int32_t s_nan[2][kP16Waves];
   __shared__ float s_scale[2][kP16Waves];
   __shared__ uint16_t s_bad[W::kO][64 * kP16Waves];  // columns that a row's NaN is in
@@ -88,13 +101,13 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     int64_t token, head;
     p16_row<kBM>(p, gr.req.q0, u, min(row, rows - 1), token, head);
 
-    // The keys [row_lo, row_hi) that the lane's row sees. The piece's 64-key tiles
+    // The lane's row sees the keys before row_hi, of them its window. The piece's 64-key tiles
     // [t0, t1) from base on, of those that the unit sees any key of; those of them in
     // [full0, full1) are seen whole by all rows of the unit, those outside of
     // [w0, w1) by none of the wave's, and those in [wf0, wf1) whole by all of these.
     const int len = gr.req.len, base = gr.req.base;
     const bool idle = 32 * wave >= rows;  // a wave without rows only loads
-    int row_lo = gr.req.lo, row_hi = len;
+    int row_hi = len;
     int t0 = 0, t1, full0, full1, w0, w1, wf0, wf1;
     {
       const int n = p.qsl == nullptr
@@ -107,7 +120,6 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             static_cast<uint32_t>(u.rt * kBM + min(r, rows - 1))));
       };
       row_hi = hi_of(static_cast<int>(token) - gr.req.q0);
-      row_lo = lo_of(row_hi);
       // First tile of the keys from `key` on, and one past the last of those before.
       const auto down = [&](int key) { return key > base ? (key - base) >> 6 : 0; };
       const auto up = [&](int key) { return key > base ? (key - base + kKT - 1) >> 6 : 0; };
@@ -127,6 +139,8 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       wf1 = uniform(down(w_first));
     }
 
+    const auto row_lo_of = [&] { return p.window > 0 ? max(row_hi - p.window, 0) : 0; };
+
     float m = kNegInf, l = 0.0f;
     bool bad = false;
     f32x16 o[W::kO];
@@ -137,13 +151,16 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 
     const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
     // The block of 16 keys that the wave brings of tile t: itself, or the last
-    // one. Lane i knows that of tile window + i.
+    // one. Entry i of the wave's window is that of tile window + i.
     const auto block = [&](int t) { return min(base + kKT * t + 16 * wave, (len - 1) & ~15); };
     int window = t0;
-    F8Window w;
     const auto refill = [&](int t) {
       window = t;
-      w = f8_window(p, table, u.head, block(t + lane));
+      const F8Block b = f8_block(p, table, u.head, block(t + lane));
+      s_window[wave].address[lane] =
+          (u32x4){static_cast<uint32_t>(b.k), static_cast<uint32_t>(b.k >> 32),
+                  static_cast<uint32_t>(b.v), static_cast<uint32_t>(b.v >> 32)};
+      s_window[wave].e[lane] = b.e;
     };
     // Lane: 16 codes from column 16 c on of row r and of every kStep-th after it.
     constexpr int kStep = 64 / W::kCodes;
@@ -152,9 +169,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     uint32_t ke = 0, ve = 0;
     const auto load = [&](int t) {
       const int kb = block(t), at_lane = t - window;
-      const char* ks = f8_lane_address(w.k_lo, w.k_hi, at_lane);
-      const char* vs = f8_lane_address(w.v_lo, w.v_hi, at_lane);
-      const uint32_t e = __builtin_amdgcn_readlane(w.e, at_lane);
+      const u32x4 address = s_window[wave].address[at_lane];
+      const char* ks = f8_uniform(address[0], address[1]);
+      const char* vs = f8_uniform(address[2], address[3]);
+      const uint32_t e = __builtin_amdgcn_readfirstlane(s_window[wave].e[at_lane]);
       ke = e & 0xffu;
       ve = e >> 8;
       const uint32_t k_slot = static_cast<uint32_t>(p.k.s_slot);
@@ -175,24 +193,28 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
         }
       }
     };
-    // The loaded tile t into buffer `buf`; the scales of K's blocks, in fp16. The
-    // pieces' places differ in bits that an exclusive or or an addition sets.
-    const auto store = [&](int t, int buf) {
+    // Part `part` of four of the loaded tile into buffer `buf`. The pieces' places
+    // differ in bits that an exclusive or or an addition sets.
+    const auto store = [&](int buf, int part) {
       char* kd = lds + buf * W::kBuf + 16 * wave * W::kRow;
       char* vd = kd + 2 * W::kBuf;
       const uint32_t ka = r0 * W::kRow + 16 * W::k_piece(r0, 2 * c0);
       const uint32_t va = r0 * W::kRow + 16 * W::v_piece(r0, 2 * c0);
-      const float k_scale = f8_scale(ke), v_scale = f8_scale(ve);
 #pragma unroll
-      for (int i = 0; i < W::kLoads; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          static_assert(kStep % 4 == 0 && (D == 64 || kStep * W::kLoads == 16), "bits of a row");
-          *reinterpret_cast<u32x4*>(kd + (ka ^ (16u * e) ^ (16u * (kStep * i))) + kStep * i * W::kRow) =
-              f8_eight<kF16>(kc[i][2 * e], kc[i][2 * e + 1], kF16 ? 1.0f : k_scale);
-          *reinterpret_cast<u32x4*>(vd + va + 16 * e + kStep * i * W::kRow) =
-              f8_eight<false>(vc[i][2 * e], vc[i][2 * e + 1], v_scale);
-        }
+      for (int q = 0; q < W::kLoads; ++q) {
+        const int at = part * W::kLoads + q, i = (at >> 1) % W::kLoads, e = at & 1;
+        if (at < 2 * W::kLoads)
+          *reinterpret_cast<u32x4*>(kd + (ka ^ (W::kOddK * e) ^ W::k_row(i)) +
+                                    kStep * i * W::kRow) =
+              f8_eight<kF16>(kc[i][2 * e], kc[i][2 * e + 1], kF16 ? 1.0f : f8_scale(ke));
+        else
+          *reinterpret_cast<u32x4*>(vd + (va ^ (W::kOddV * e)) + kStep * i * W::kRow) =
+              f8_eight<false>(vc[i][2 * e], vc[i][2 * e + 1], f8_scale(ve));
+      }
+    };
+    // What the others have to know of it: whether there is a NaN in V, where not
+    // all rows see all of tile t; the scale of K's block, in fp16.
+    const auto tell = [&](int t, int buf) {
       if (t < full0 || t >= full1) {
         bool any = false;
 #pragma unroll
@@ -202,7 +224,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
         const bool nan = __ballot(any) != 0;
         if (lane == 0) s_nan[buf][wave] = nan;
       }
-      if (kF16 && lane == 0) s_scale[buf][wave] = k_scale;
+      if (kF16 && lane == 0) s_scale[buf][wave] = f8_scale(ke);
+    };
+    const auto store_all = [&](int t, int buf) {
+#pragma unroll
+      for (int part = 0; part < 4; ++part) store(buf, part);
+      tell(t, buf);
     };
 
     int buf = 0;
@@ -225,7 +252,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, at, takers, !whole);
     }
     at += take;
-    if (t0 < t1) store(t0, 0);
+    if (t0 < t1) store_all(t0, 0);
 
     for (int t = t0; t < t1; ++t, buf ^= 1) {
       lds_barrier();  // tile t is in LDS, and nobody reads tile t - 1 any more
@@ -241,7 +268,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
         for (int j = 0; j < W::kO; ++j) {
           uint32_t bits = 0;
 #pragma unroll 1
-          for (int k = max(row_lo - k0, 0); k < min(row_hi - k0, kKT); ++k)
+          for (int k = max(row_lo_of() - k0, 0); k < min(row_hi - k0, kKT); ++k)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int col = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -266,7 +293,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       }
       const bool mine = t >= w0 && t < w1;
       if (more && t + 1 - window == 64) refill(t + 1);
-      if (more && !mine) load(t + 1);
+      if (more && !mine) {
+        load(t + 1);
+        store_all(t + 1, buf ^ 1);
+      }
       if (mine) {
         // Scores: K operands four products ahead.
         f32x16 s[2];
@@ -321,6 +351,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             for (int i = 0; i < 16; ++i) s[b][i] *= s_scale[buf][2 * b + (i >> 3)];
         }
         if (t < wf0 || t >= wf1) {
+          const int row_lo = row_lo_of();
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -379,6 +410,9 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __builtin_amdgcn_sched_barrier(0);
+          // The first operands, read before the softmax, are waited for before the
+          // next ones are asked for, and not with them.
+          if (i == 0) __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
           if (i < 3) read_v(i + 1);
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -386,10 +420,18 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             o[j] = mfma32<false>(vf[i & 1][j], pf[i], o[j]);
             if constexpr (kF16) o[j] = mfma32<false>(vf[i & 1][j], pl[i], o[j]);
           }
+          // Behind the last tile, the registers' old codes, which nobody reads.
+          if constexpr (W::kBetween) store(buf ^ 1, i);
+        }
+        if (more) {
+          if constexpr (!W::kBetween) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store(buf ^ 1, i);
+          }
+          tell(t + 1, buf ^ 1);
         }
         __builtin_amdgcn_s_setprio(1);
       }
-      if (more) store(t + 1, buf ^ 1);
     }
 
     if (bad) {
@@ -399,6 +441,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[j][i] = bits >> i & 1u ? __builtin_nanf("") : o[j][i];
       }
+    }
+    {
+      // The row's place again, rather than in registers through the loop.
+      int again = min(row, rows - 1);
+      asm volatile("" : "+v"(again));
+      p16_row<kBM>(p, gr.req.q0, u, again, token, head);
     }
     const SwapPair ls = swap_halves(l);
     const float sum = ls.a + ls.b;
