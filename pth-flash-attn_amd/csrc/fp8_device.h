@@ -52,8 +52,11 @@ struct F8Window {
   u32x4 address[64];  // of K, of V
   uint32_t e[64];
 };
-__device__ __forceinline__ const char* f8_uniform(uint32_t lo, uint32_t hi) {
-  return reinterpret_cast<const char*>(
+// An address in memory made of its words, which are the same in all lanes. (Of no
+// named address space, its loads would count and wait with those from LDS.)
+typedef const char __attribute__((address_space(1))) * GlobalBytes;
+__device__ __forceinline__ GlobalBytes f8_uniform(uint32_t lo, uint32_t hi) {
+  return reinterpret_cast<GlobalBytes>(
       static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(lo))) |
       static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(hi))) << 32);
 }
@@ -79,18 +82,22 @@ __device__ __forceinline__ u32x4 f8_eight(uint32_t a, uint32_t b, float scale) {
   return (u32x4){f8_pair_lo<kF16>(a, scale), f8_pair_hi<kF16>(a, scale), f8_pair_lo<kF16>(b, scale),
                  f8_pair_hi<kF16>(b, scale)};
 }
-// Whether a word holds a NaN code (0x7f or 0xff).
-__device__ __forceinline__ bool f8_has_nan(uint32_t w) {
-  return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+// 0x80 in each byte of a word that is a NaN code (0x7f or 0xff).
+__device__ __forceinline__ uint32_t f8_nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
-// Two bf16 values, 0 for a NaN; and 1 for a NaN, 0 otherwise.
-__device__ __forceinline__ uint32_t f8_without_nan(uint32_t w) {
-  return ((w & 0x7fffu) > 0x7f80u ? 0u : w & 0xffffu) |
-         ((w & 0x7fff0000u) > 0x7f800000u ? 0u : w & 0xffff0000u);
+// Whether a word holds one.
+__device__ __forceinline__ bool f8_has_nan(uint32_t w) {
+  return f8_nan_bytes(w) != 0;
 }
 __device__ __forceinline__ uint32_t f8_nan_ones(uint32_t w) {
   return ((w & 0x7fffu) > 0x7f80u ? 0x3f80u : 0u) |
          ((w & 0x7fff0000u) > 0x7f800000u ? 0x3f800000u : 0u);
+}
+// Two bf16 values, 0 for a NaN.
+__device__ __forceinline__ uint32_t f8_without_nan(uint32_t w) {
+  return ((w & 0x7fffu) > 0x7f80u ? 0u : w & 0xffffu) |
+         ((w & 0x7fff0000u) > 0x7f800000u ? 0u : w & 0xffff0000u);
 }
 
 }  // namespace

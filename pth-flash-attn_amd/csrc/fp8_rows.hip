@@ -19,10 +19,10 @@
 //
 // Numerics. Scores, m, l and o are 32 bits. K's codes are exact in the queries'
 // type and V's scaled values in bf16, whose range they need; P is a bf16 pair
-// hi + lo (16 significant bits). A key behind the request's last takes the
-// address of a visible one and the weight 0; one that a row of a draft may not
-// see has the weight 0, and where its V is NaN it is taken out of that product
-// and put back into the rows that see it.
+// hi + lo (16 significant bits). A key that a row does not see (behind its own,
+// behind the request's last one in its block, before the window) has the weight 0
+// there, and where its V is NaN that is taken out of the products and put back into
+// the rows that see it.
 //
 // Bound: the cache's bytes, each read once, by one work-group.
 
@@ -47,6 +47,13 @@ struct RowsDim {
 constexpr float kBias = 16.0f;
 constexpr int kChunk = 64, kBlocks = kChunk / kF8Span;
 
+// A load with the non-temporal hint: of bytes that the launch reads once.
+template <class T>
+__device__ __forceinline__ T ld_once(GlobalBytes p) {
+  typedef T __attribute__((address_space(1))) Global;
+  return __builtin_nontemporal_load(reinterpret_cast<const Global*>(p));
+}
+
 template <int kWords>
 struct Words;
 template <>
@@ -69,6 +76,8 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
   // before it.
   __shared__ f32x4 s_x[kP16Waves][R::kO][64];
   __shared__ float s_m[kP16Waves][kBM], s_l[kP16Waves][kBM];
+  // Of a NaN in V: its keys in a chunk, by column; the outputs of a lane that meet it.
+  __shared__ uint64_t s_nan_keys[kP16Waves][D], s_bad[kP16Waves][64];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -121,51 +130,52 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
     }
 
     float m = kNegInf, l = 0.0f;
+    bool bad = false;
     f32x4 o[R::kO];
 #pragma unroll
     for (int j = 0; j < R::kO; ++j) o[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
+    const uint64_t k_base = reinterpret_cast<uint64_t>(p.k.base + u.head * p.k.s_head);
+    const uint64_t v_base = reinterpret_cast<uint64_t>(p.v.base + u.head * p.v.s_head);
     const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
     const int step = kChunk * parts;
     const int k_end = min(gr.req.base + ((gr.kt + take) << p.key_tile_log2), len);
     int k0 = gr.req.base + (gr.kt << p.key_tile_log2) + kChunk * part;
 
-    // 16-key blocks: the one that stands for the keys from k on (itself, or the
-    // last one), its entry of the block table, its first rows and its scales.
-    const auto start = [&](int k) { return min(k, (len - 1) & ~15); };
-    const auto page_of = [&](int kb) {
-      return mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
+    // The chunk's blocks of 16 keys: block b is the one of the keys from k + 16 b on,
+    // or the last one, and lane l knows block l % 4. Its entry of the block table is
+    // read a chunk before its address is made and its exponents are asked for.
+    const auto start = [&](int k) { return min(k + kF8Span * (lane & 3), (len - 1) & ~15); };
+    const auto entry_of = [&](int k) {
+      return table[mulhi32(static_cast<uint32_t>(start(k)), p.bs_div.mul) >> p.bs_div.shift];
     };
-    const auto entry_of = [&](int k) { return ld_ro(table, page_of(start(k))); };
-    struct Block {
-      int32_t kb;
-      const char *k, *v;
-      uint32_t ke, ve;
+    uint64_t k_at = 0, v_at = 0;
+    uint32_t ke = 0, ve = 0;
+    const auto place = [&](int k, int32_t entry) {
+      const int kb = start(k);
+      const uint32_t page = mulhi32(static_cast<uint32_t>(kb), p.bs_div.mul) >> p.bs_div.shift;
+      const uint32_t id = static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks)
+                              ? static_cast<uint32_t>(entry)
+                              : 0u;
+      const uint32_t in = static_cast<uint32_t>(kb) - page * p.bs_div.d;
+      k_at = k_base + id * p.k.s_block + in * static_cast<uint64_t>(p.k.s_slot);
+      v_at = v_base + id * p.v.s_block + in * static_cast<uint64_t>(p.v.s_slot);
+      const uint32_t e = (id * static_cast<uint32_t>(p.n_sub) + in / kF8Span) *
+                             static_cast<uint32_t>(p.num_kv_heads) +
+                         static_cast<uint32_t>(u.head);
+      ke = p.k_exp[e];
+      ve = p.v_exp[e];
     };
-    const auto block = [&](int k, int32_t entry) {
-      Block b;
-      b.kb = start(k);
-      const int64_t id =
-          static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_blocks) ? entry : 0;
-      const int64_t in = b.kb - static_cast<int32_t>(page_of(b.kb) * p.bs_div.d);
-      b.k = p.k.base + id * p.k.s_block + in * p.k.s_slot + u.head * p.k.s_head;
-      b.v = p.v.base + id * p.v.s_block + in * p.v.s_slot + u.head * p.v.s_head;
-      const int64_t e = (id * p.n_sub + in / kF8Span) * p.num_kv_heads + u.head;
-      b.ke = ld_ro_byte(p.k_exp + e);
-      b.ve = ld_ro_byte(p.v_exp + e);
-      return b;
+    const auto block_at = [](uint64_t at_lane, int b) {
+      return reinterpret_cast<GlobalBytes>(
+          static_cast<uint64_t>(static_cast<uint32_t>(
+              __builtin_amdgcn_readlane(static_cast<uint32_t>(at_lane), b))) |
+          static_cast<uint64_t>(static_cast<uint32_t>(
+              __builtin_amdgcn_readlane(static_cast<uint32_t>(at_lane >> 32), b)))
+              << 32);
     };
-    // Byte `col` of row i of a block, brought into the request's keys.
-    const auto row_of = [&](const char* rows_at, int64_t s_slot, int kb, int i, int col) {
-      const int r = min(max(i, lo - kb), len - 1 - kb);
-      return rows_at + (__umul24(static_cast<uint32_t>(r), static_cast<uint32_t>(s_slot)) + col);
-    };
-
-    int32_t entry[kBlocks] = {};
-    if (k0 < k_end) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) entry[b] = entry_of(k0 + kF8Span * b);
-    }
+    int32_t entry = 0;
+    if (k0 < k_end) entry = entry_of(k0);
     // Q: 16 bytes per product, zeros in rows that the unit lacks.
     if (!first && parts > 1) __syncthreads();  // the last group's sums have been read
     first = false;
@@ -182,26 +192,35 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
 
     u32x4 kf[kBlocks][R::kK];
     V vf[kBlocks][4];
-    Block blk[kBlocks];
-    const auto load_k = [&](int b) {
-      const char* src = row_of(blk[b].k, p.k.s_slot, blk[b].kb, r16, 16 * g);
+    // The lane's places in a block: of K's row, of V's first one.
+    const uint32_t k_off = __umul24(r16, static_cast<uint32_t>(p.k.s_slot)) + 16 * g;
+    const uint32_t v_off = __umul24(4 * g, static_cast<uint32_t>(p.v.s_slot)) + R::kRun * r16;
+    const auto load_k = [&] {
+      uint32_t k_here = k_off;  // here, so that it is added by the load itself
+      asm volatile("" : "+v"(k_here));
 #pragma unroll
-      for (int j = 0; j < R::kK; ++j) kf[b][j] = ld_nt<u32x4>(src + 64 * j);
+      for (int b = 0; b < kBlocks; ++b) {
+        const GlobalBytes src = block_at(k_at, b);
+#pragma unroll
+        for (int j = 0; j < R::kK; ++j) kf[b][j] = ld_once<u32x4>(src + k_here + 64 * j);
+      }
     };
-    const auto load_v = [&](int b) {
+    const auto load_v = [&] {
+      uint32_t v_here = v_off;
+      asm volatile("" : "+v"(v_here));
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        vf[b][e] = ld_nt<V>(row_of(blk[b].v, p.v.s_slot, blk[b].kb, 4 * g + e, R::kRun * r16));
+      for (int b = 0; b < kBlocks; ++b) {
+        const GlobalBytes src = block_at(v_at, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          vf[b][e] = ld_once<V>(src + e * static_cast<uint32_t>(p.v.s_slot) + v_here);
+      }
     };
     if (k0 < k_end) {
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) blk[b] = block(k0 + kF8Span * b, entry[b]);
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) load_k(b);
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) load_v(b);
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) entry[b] = entry_of(k0 + step + kF8Span * b);
+      place(k0, entry);
+      load_k();
+      entry = entry_of(k0 + step);
+      load_v();
       // One chunk. kMore: the next one's loads are issued on the way.
       const auto chunk = [&](auto more) {
         constexpr bool kMore = decltype(more)::value;
@@ -209,8 +228,8 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
         float ks[kBlocks], vs[kBlocks];
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
-          ks[b] = f8_scale(blk[b].ke) * p.scale_log2;
-          vs[b] = f8_scale(blk[b].ve);
+          ks[b] = f8_scale(__builtin_amdgcn_readlane(ke, b)) * p.scale_log2;
+          vs[b] = f8_scale(__builtin_amdgcn_readlane(ve, b));
         }
         f32x4 s[kBlocks];
 #pragma unroll
@@ -224,18 +243,17 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
           }
         }
         if constexpr (kMore) {
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) blk[b] = block(next + kF8Span * b, entry[b]);
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) load_k(b);
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) entry[b] = entry_of(next + step + kF8Span * b);
+          // Not before the last product, in whose registers they arrive.
+          __builtin_amdgcn_sched_barrier(0);
+          place(next, entry);
+          load_k();
+          entry = entry_of(next + step);
         }
         float t[4 * kBlocks];
 #pragma unroll
         for (int e = 0; e < 4 * kBlocks; ++e) t[e] = s[e >> 2][e & 3] * ks[e >> 2];
         const bool edge = k0 < all_lo || k0 + kChunk > all_hi;
-        if (edge) {
+        if (__builtin_expect(edge, 0)) {
 #pragma unroll
           for (int e = 0; e < 4 * kBlocks; ++e) {
             const int key = k0 + 16 * (e >> 2) + 4 * g + (e & 3);
@@ -264,9 +282,11 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
         }
 #pragma unroll
         for (int j = 0; j < R::kO; ++j) o[j] *= alpha;
-        // Whether rows that do not see all of these keys may meet a NaN.
+        // Whether a row may meet a NaN of a key that it does not see.
         bool nan = false;
-        if (edge && p.causal && p.qsl != nullptr) {
+        if (__builtin_expect(edge, 0)) {
+          // Kept in the branch: V is still on its way, and nothing else asks for it here.
+          asm volatile("" ::: "memory");
           bool any = false;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
@@ -276,61 +296,81 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
               for (int i = 0; i < R::kWords; ++i) any |= f8_has_nan(word(vf[b][e], i));
           nan = __ballot(any) != 0;
         }
-        // Products of 32 keys, two columns of a word at a time.
+        // Products of 32 keys, two columns of a word (its low or its high half) at a
+        // time; kClean: without NaNs. (V is not changed: the registers' copies would
+        // wait for it before the softmax, in chunks that have none, too.)
         const auto pv = [&](auto clean) {
           constexpr bool kClean = decltype(clean)::value;
-          u32x4 sees[kBlocks / 2];
-          if constexpr (kClean) {
-#pragma unroll
-            for (int e = 0; e < 4 * kBlocks; e += 2) {
-              const int key = k0 + 16 * (e >> 2) + 4 * g + (e & 3);
-              sees[e >> 3][(e & 7) >> 1] = (key >= row_lo && key < row_hi ? 0x3f80u : 0u) |
-                                           (key + 1 >= row_lo && key + 1 < row_hi ? 0x3f800000u : 0u);
-            }
-          }
+          const auto codes = [&](int b, int e, int i) {
+            const uint32_t w = word(vf[b][e], i);
+            return kClean ? w & ~((f8_nan_bytes(w) >> 7) * 0xffu) : w;
+          };
 #pragma unroll
           for (int h = 0; h < kBlocks / 2; ++h)
 #pragma unroll
             for (int i = 0; i < R::kWords; ++i)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                u32x4 a0, a1;
+                u32x4 a[2];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int b = 2 * h + (e >> 1);
-                  const uint32_t w = __builtin_amdgcn_perm(
-                      word(vf[b][2 * (e & 1) + 1], i), word(vf[b][2 * (e & 1)], i),
-                      c ? 0x07030602u : 0x05010400u);
-                  a0[e] = f8_pair_lo<false>(w, vs[b]);
-                  a1[e] = f8_pair_hi<false>(w, vs[b]);
+                  const uint32_t w =
+                      __builtin_amdgcn_perm(codes(b, 2 * (e & 1) + 1, i), codes(b, 2 * (e & 1), i),
+                                            c ? 0x07030602u : 0x05010400u);
+                  a[0][e] = f8_pair_lo<false>(w, vs[b]);
+                  a[1][e] = f8_pair_hi<false>(w, vs[b]);
                 }
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                   f32x4& acc = o[4 * i + 2 * c + d];
-                  u32x4 a = d ? a1 : a0;
-                  if constexpr (kClean) {
-                    u32x4 ones;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      ones[e] = f8_nan_ones(a[e]);
-                      a[e] = f8_without_nan(a[e]);
-                    }
-                    const f32x4 met =
-                        mfma16<false>(ones, sees[h], (f32x4){0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                      acc[e] = met[e] > 0.0f ? __builtin_nanf("") : acc[e];
-                  }
-                  acc = mfma16<false>(a, hi[h], acc);
-                  acc = mfma16<false>(a, lo_[h], acc);
+                  acc = mfma16<false>(a[d], hi[h], acc);
+                  acc = mfma16<false>(a[d], lo_[h], acc);
                 }
               }
         };
-        if (nan) pv(std::true_type{});
-        else pv(std::false_type{});
-        if constexpr (kMore) {
+        if (__builtin_expect(nan, 0)) {
+          // The keys of which a column holds a NaN, as bits; then the columns of the
+          // lane's row that see one of them, for the unit's end.
+          uint64_t* keys = s_nan_keys[wave];
+          for (int i = lane; i < D; i += 64) keys[i] = 0;
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) load_v(b);
+          for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < R::kWords; ++i) {
+                const uint32_t w = word(vf[b][e], i), n = f8_nan_bytes(w);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  atomicOr(reinterpret_cast<unsigned long long*>(&keys[R::kRun * r16 + 4 * i + c]),
+                           static_cast<unsigned long long>(n >> (8 * c + 7) & 1u)
+                               << (16 * b + 4 * g + e));
+              }
+          // No branch here differs between lanes: it would change the loop's form.
+          const auto before = [](int key) {  // bits of the keys before it
+            return key <= 0 ? 0ull : ~0ull >> (64 - min(key, 64));
+          };
+          const uint64_t sees = before(row_hi - k0) & ~before(row_lo - k0);
+          uint64_t hit = bad ? s_bad[wave][lane] : 0;
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+            for (int j = 0; j < R::kO; ++j)
+              hit |= static_cast<uint64_t>((keys[R::kRun * (4 * g + i) + j] & sees) != 0)
+                     << (R::kO * i + j);
+          s_bad[wave][lane] = hit;
+          bad = true;
+          pv(std::true_type{});
+        } else {
+          pv(std::false_type{});
+        }
+        if constexpr (kMore) {
+          __builtin_amdgcn_sched_barrier(0);
+          load_v();
+          // Unlike the loads before the loop: the compiler would merge both at its
+          // head, and copy K and O in every chunk.
+          asm volatile("; the next chunk");
           k0 = next;
         }
       };
@@ -341,6 +381,14 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
     if (gr.kt == 0 && (!whole || p.notes > 0)) {
       noted |= !whole;
       if (threadIdx.x == 0) p16_note<D>(p, gr, wg, tiles, begin, takers, !whole);
+    }
+    if (__builtin_expect(bad, 0)) {
+      const uint64_t hit = s_bad[wave][lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < R::kO; ++j)
+          o[j][i] = hit >> (R::kO * i + j) & 1 ? __builtin_nanf("") : o[j][i];
     }
     // The unit's first wave joins the others' sums to its own.
     l = xor_sum(l);

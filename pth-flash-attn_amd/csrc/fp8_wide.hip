@@ -17,9 +17,9 @@
 // bits. bf16: K's and V's values are exact, P is rounded once, and l sums the
 // rounded P. fp16: K's codes are exact in fp16, their scale is a factor of the
 // scores; V is in bf16, whose range its values need, and P a bf16 pair hi + lo.
-// A row does not see the keys behind its own: where one of these has a NaN in V,
-// it is taken out of the products of the tile and put back into the rows that
-// do see it.
+// A row does not see the keys behind its own, nor the slots behind the request's
+// last key in their block: where one of these has a NaN in V, it is taken out of the
+// products of the tile and put back into the rows that do see it.
 
 #include "fp8_device.h"
 
@@ -165,32 +165,24 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     // Lane: 16 codes from column 16 c on of row r and of every kStep-th after it.
     constexpr int kStep = 64 / W::kCodes;
     const int r0 = lane / W::kCodes, c0 = lane % W::kCodes;
+    typedef u32x4 __attribute__((address_space(1))) GlobalPiece;
     u32x4 kc[W::kLoads], vc[W::kLoads];
     uint32_t ke = 0, ve = 0;
     const auto load = [&](int t) {
-      const int kb = block(t), at_lane = t - window;
+      const int at_lane = t - window;
       const u32x4 address = s_window[wave].address[at_lane];
-      const char* ks = f8_uniform(address[0], address[1]);
-      const char* vs = f8_uniform(address[2], address[3]);
+      const GlobalBytes ks = f8_uniform(address[0], address[1]);
+      const GlobalBytes vs = f8_uniform(address[2], address[3]);
       const uint32_t e = __builtin_amdgcn_readfirstlane(s_window[wave].e[at_lane]);
       ke = e & 0xffu;
       ve = e >> 8;
       const uint32_t k_slot = static_cast<uint32_t>(p.k.s_slot);
       const uint32_t v_slot = static_cast<uint32_t>(p.v.s_slot);
-      if (kb + kF8Span <= len) {
-        const uint32_t ko = __umul24(r0, k_slot) + 16 * c0, vo = __umul24(r0, v_slot) + 16 * c0;
+      const uint32_t ko = __umul24(r0, k_slot) + 16 * c0, vo = __umul24(r0, v_slot) + 16 * c0;
 #pragma unroll
-        for (int i = 0; i < W::kLoads; ++i) {
-          kc[i] = *reinterpret_cast<const u32x4*>(ks + static_cast<int64_t>(i * kStep) * k_slot + ko);
-          vc[i] = *reinterpret_cast<const u32x4*>(vs + static_cast<int64_t>(i * kStep) * v_slot + vo);
-        }
-      } else {  // keys past the last one repeat it
-#pragma unroll
-        for (int i = 0; i < W::kLoads; ++i) {
-          const uint32_t from = min(r0 + i * kStep, len - 1 - kb);
-          kc[i] = *reinterpret_cast<const u32x4*>(ks + (__umul24(from, k_slot) + 16 * c0));
-          vc[i] = *reinterpret_cast<const u32x4*>(vs + (__umul24(from, v_slot) + 16 * c0));
-        }
+      for (int i = 0; i < W::kLoads; ++i) {
+        kc[i] = *reinterpret_cast<const GlobalPiece*>(ks + static_cast<int64_t>(i * kStep) * k_slot + ko);
+        vc[i] = *reinterpret_cast<const GlobalPiece*>(vs + static_cast<int64_t>(i * kStep) * v_slot + vo);
       }
     };
     // Part `part` of four of the loaded tile into buffer `buf`. The pieces' places
@@ -215,7 +207,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     // What the others have to know of it: whether there is a NaN in V, where not
     // all rows see all of tile t; the scale of K's block, in fp16.
     const auto tell = [&](int t, int buf) {
-      if (t < full0 || t >= full1) {
+      if (__builtin_expect(t < full0 || t >= full1, 0)) {
         bool any = false;
 #pragma unroll
         for (int i = 0; i < W::kLoads; ++i)
@@ -260,22 +252,25 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       const int k0 = base + kKT * t;
       const char* kt = lds + buf * W::kBuf;
       const char* vt = kt + 2 * W::kBuf;
-      if ((t < full0 || t >= full1) &&
-          (s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] | s_nan[buf][3]) != 0) {
+      const bool masked = t < full0 || t >= full1;
+      if (__builtin_expect(masked && (s_nan[buf][0] | s_nan[buf][1] | s_nan[buf][2] |
+                                      s_nan[buf][3]) != 0, 0)) {
         // A NaN in V that not all rows see: the lane's columns of which its row sees
         // one are noted, and the tile is rid of them.
 #pragma unroll 1
         for (int j = 0; j < W::kO; ++j) {
           uint32_t bits = 0;
 #pragma unroll 1
-          for (int k = max(row_lo_of() - k0, 0); k < min(row_hi - k0, kKT); ++k)
+          for (int k = 0; k < kKT; ++k) {
+            const bool sees = k0 + k >= row_lo_of() && k0 + k < row_hi;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int col = 32 * j + 8 * (i >> 2) + 4 * h + (i & 3);
               const uint16_t w = *reinterpret_cast<const uint16_t*>(
                   vt + k * W::kRow + 16 * W::v_piece(k & 15, col >> 3) + 2 * (col & 7));
-              bits |= (w & 0x7fffu) > 0x7f80u ? 1u << i : 0u;
+              bits |= sees && (w & 0x7fffu) > 0x7f80u ? 1u << i : 0u;
             }
+          }
           s_bad[j][threadIdx.x] = static_cast<uint16_t>(bits | (bad ? s_bad[j][threadIdx.x] : 0u));
         }
         bad = true;
@@ -292,7 +287,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
         lds_barrier();
       }
       const bool mine = t >= w0 && t < w1;
-      if (more && t + 1 - window == 64) refill(t + 1);
+      if (__builtin_expect(more && t + 1 - window == 64, 0)) refill(t + 1);
       if (more && !mine) {
         load(t + 1);
         store_all(t + 1, buf ^ 1);
@@ -350,7 +345,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] *= s_scale[buf][2 * b + (i >> 3)];
         }
-        if (t < wf0 || t >= wf1) {
+        if (__builtin_expect(t < wf0 || t >= wf1, 0)) {
           const int row_lo = row_lo_of();
 #pragma unroll
           for (int b = 0; b < 2; ++b)

@@ -335,8 +335,8 @@ std::string f8_cache_sizes(const PthAttnCacheF8& c) {
     return "num_blocks >= 1, num_kv_heads 1 .. 65535";
   if (c.block_size < kF8Span || c.block_size % kF8Span != 0)
     return "block_size must be a positive multiple of 16";
-  if (static_cast<int64_t>(c.num_blocks) * (c.block_size / kF8Span) > INT32_MAX)
-    return "num_blocks x block_size must be less than 2^35";
+  if (static_cast<int64_t>(c.num_blocks) * (c.block_size / kF8Span) > INT32_MAX / c.num_kv_heads)
+    return "num_blocks x block_size x num_kv_heads must be less than 2^35";
   return "";
 }
 
