@@ -90,10 +90,6 @@ __device__ __forceinline__ uint32_t f8_nan_bytes(uint32_t w) {
 __device__ __forceinline__ bool f8_has_nan(uint32_t w) {
   return f8_nan_bytes(w) != 0;
 }
-__device__ __forceinline__ uint32_t f8_nan_ones(uint32_t w) {
-  return ((w & 0x7fffu) > 0x7f80u ? 0x3f80u : 0u) |
-         ((w & 0x7fff0000u) > 0x7f800000u ? 0x3f800000u : 0u);
-}
 // Two bf16 values, 0 for a NaN.
 __device__ __forceinline__ uint32_t f8_without_nan(uint32_t w) {
   return ((w & 0x7fffu) > 0x7f80u ? 0u : w & 0xffffu) |

@@ -62,6 +62,78 @@ bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   return span <= most;
 }
 
+// The keys that a request of so many tokens may see: their last window + tokens - 1,
+// from a block's beginning on.
+int64_t span_of(const F8Params& p, int64_t tokens) {
+  return p.window > 0 ? std::min<int64_t>(p.max_keys, int64_t{p.window} + tokens - 1 + 15)
+                      : p.max_keys;
+}
+
+// Whether a batch whose longest request has `longest` tokens is one of prompts and
+// decodes, so that requests of few rows get their own launch: eight of them, if the
+// others are as long as the longest, and work enough for what that launch costs. Whole
+// calls of decodes with prompts, 32 / 8 heads of 128, one launch and two: 60 of 2,000
+// keys with 2 x 512 tokens 119.8 and 91.2 us, 120 with 1 x 512 176 and 134, 200 of 1,000
+// with 2 x 32 142 and 120; 8 of 2,000 with 1 x 512 53 and 66, 20 of 1,000 with 4 x 8 28
+// and 48, 14 of 500 with 2 x 17 20 and 32.
+constexpr int64_t kMixedBytes = int64_t{5} << 24;  // of K, at the longest length
+bool mixed(const F8Params& p, int32_t head_size, int64_t longest) {
+  const int64_t few = p.num_reqs - (p.num_tokens + longest - 1) / longest;
+  return p.group <= kP16RowsRows && few >= 8 &&
+         few * span_of(p, 1) * p.num_kv_heads * head_size >= kMixedBytes;
+}
+
+// The kernel of few or many rows over the requests that p names, and the join.
+// `longest`: of their query tokens (a choice only).
+int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t longest,
+                    int32_t cus, hipStream_t stream) {
+  const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
+  // Bounds of the partition: row tiles and groups of all requests, key tiles of one.
+  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.group;
+  const int64_t reqs = p.num_reqs;
+  int64_t row_tiles = rows / bm + reqs;
+  if (p.qsl == nullptr) row_tiles = reqs * ((p.group + bm - 1) / bm);
+  else if (p.most_rows <= bm) row_tiles = reqs;
+  else if (p.least_rows > 0) row_tiles = rows / bm + std::min(reqs, rows / p.least_rows);
+  int64_t tokens = p.qsl ? p.num_tokens : 1;
+  if (p.qsl && p.most_rows <= bm) tokens = std::max<int64_t>(p.most_rows / p.group, 1);
+  const int64_t span = span_of(p, tokens);
+  const int64_t units = row_tiles * p.num_kv_heads;
+  if (units == 0) return PTH_ATTN_OK;
+  const bool whole = wide ? whole_wide(head_size, span, units, cus) : whole_rows(head_size, span);
+  p.team = wide ? 1 : team_of(p, span, std::min(bm, longest * p.group), whole, cus);
+  if (whole)
+    while (p.team > 1 && units / p.team < p16_resident(head_size) * cus) p.team /= 2;
+  p.key_tile_log2 = wide ? 6 : 8 - (p.team >> 1);
+  if (whole)
+    while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
+  p.slot_rows = static_cast<int32_t>(p.qsl ? bm : std::min<int64_t>(bm, p.group));
+  const int64_t key_tiles =
+      std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
+  const int64_t groups =
+      p.qsl == nullptr ? reqs * ((row_tiles / reqs * p.num_kv_heads + p.team - 1) / p.team)
+                       : units / p.team + (p.team > 1 ? reqs : 0);
+  // A causal unit's share is up to five tiles more than its keys (f8_tiles).
+  PA_REQUIRE(units < INT32_MAX / (key_tiles + 6), "the launch exceeds 2^31 tiles");
+  const int64_t fill =
+      cus * (wide ? p16_resident(head_size) : rows_per_cu(head_size, groups, cus));
+  p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
+  if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
+  p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
+  hipError_t err = wide ? launch_f8_wide_kernel(p, f16, head_size, stream)
+                        : launch_f8_rows_kernel(p, f16, head_size, stream);
+  // Work-groups of the join per note (p16_launch.hip has the measurements).
+  const int32_t items = p.team * p.slot_rows, least = wide ? 16 : 1;
+  const int32_t y =
+      p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
+  if (err == hipSuccess && key_tiles > 1)
+    err = launch_f8_combine_kernel(p, f16, wide, head_size, y, stream);
+  if (err != hipSuccess)
+    return fail(PTH_ATTN_ECUDA,
+                std::string("paged 8-bit attention launch: ") + hipGetErrorString(err));
+  return PTH_ATTN_OK;
+}
+
 }  // namespace
 
 int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
@@ -138,56 +210,23 @@ int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
   p.n_sub = c.block_size / kF8Span;
   p.causal = a.causal ? 1 : 0;
 
-  const bool wide = a.query_start_loc != nullptr &&
-                    static_cast<int64_t>(a.max_query_len) * p.group > kP16RowsRows;
-  const int64_t bm = wide ? kP16WideRows : kP16RowsRows;
   const int64_t rows = static_cast<int64_t>(a.num_tokens) * p.group;
   PA_REQUIRE(rows < INT32_MAX - 1024, "num_tokens x heads per KV head exceeds 2^31");
-  // Bounds of the partition: groups of all requests, key tiles of one. A
-  // request's tokens see its last window + tokens - 1 keys.
-  const int64_t row_tiles = a.query_start_loc == nullptr
-                                ? a.num_reqs * ((p.group + bm - 1) / bm)
-                                : rows / bm + a.num_reqs;
-  const int64_t tokens = a.query_start_loc ? a.num_tokens : 1;
-  const int64_t span = p.window > 0
-                           ? std::min<int64_t>(p.max_keys, int64_t{p.window} + tokens - 1 + 15)
-                           : p.max_keys;
-  const int64_t units = row_tiles * c.num_kv_heads;
-  const bool whole =
-      wide ? whole_wide(c.head_size, span, units, cus) : whole_rows(c.head_size, span);
-  const int64_t each = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
-  p.team = wide ? 1 : team_of(p, span, std::min(bm, each * p.group), whole, cus);
-  if (whole)
-    while (p.team > 1 && units / p.team < p16_resident(c.head_size) * cus) p.team /= 2;
-  p.key_tile_log2 = wide ? 6 : 8 - (p.team >> 1);
-  if (whole)
-    while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
-  p.slot_rows = static_cast<int32_t>(a.query_start_loc ? bm : std::min<int64_t>(bm, p.group));
-  const int64_t key_tiles =
-      std::max<int64_t>((span + (1 << p.key_tile_log2) - 1) >> p.key_tile_log2, 1);
-  const int64_t groups =
-      a.query_start_loc == nullptr
-          ? a.num_reqs * ((row_tiles / a.num_reqs * c.num_kv_heads + p.team - 1) / p.team)
-          : units / p.team + (p.team > 1 ? a.num_reqs : 0);
-  // A causal unit's share is up to five tiles more than its keys (f8_tiles).
-  PA_REQUIRE(units < INT32_MAX / (key_tiles + 6), "the launch exceeds 2^31 tiles");
-  const int64_t fill =
-      cus * (wide ? p16_resident(c.head_size) : rows_per_cu(c.head_size, groups, cus));
-  p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
-  if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
-  p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
-  const bool f16 = a.dtype == PTH_ATTN_F16;
-  hipError_t err = wide ? launch_f8_wide_kernel(p, f16, c.head_size, stream)
-                        : launch_f8_rows_kernel(p, f16, c.head_size, stream);
-  // Work-groups of the join per note (p16_launch.hip has the measurements).
-  const int32_t items = p.team * p.slot_rows, least = wide ? 16 : 1;
-  const int32_t y =
-      p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
-  if (err == hipSuccess && key_tiles > 1)
-    err = launch_f8_combine_kernel(p, f16, wide, c.head_size, y, stream);
-  if (err != hipSuccess)
-    return fail(PTH_ATTN_ECUDA, std::string("paged 8-bit attention launch: ") + hipGetErrorString(err));
-  return PTH_ATTN_OK;
+  p.least_rows = 0;
+  p.most_rows = INT32_MAX;
+  const int64_t longest = a.query_start_loc ? std::max(a.max_query_len, 1) : 1;
+  const bool wide = longest * p.group > kP16RowsRows && a.query_start_loc != nullptr;
+  if (!wide || !mixed(p, c.head_size, longest))
+    return launch_part(p, c.head_size, a.dtype == PTH_ATTN_F16, wide,
+                       std::max<int64_t>(longest, 1), cus, stream);
+  // Requests of up to 16 rows by one kernel, the others by the other.
+  F8Params few = p;
+  p.least_rows = kP16RowsRows + 1;
+  few.most_rows = kP16RowsRows;
+  const int32_t rc = launch_part(p, c.head_size, a.dtype == PTH_ATTN_F16, true, longest, cus, stream);
+  if (rc != PTH_ATTN_OK) return rc;
+  return launch_part(few, c.head_size, a.dtype == PTH_ATTN_F16, false,
+                     std::max<int64_t>(kP16RowsRows / p.group, 1), cus, stream);
 }
 
 }  // namespace pa

@@ -47,11 +47,12 @@ struct RowsDim {
 constexpr float kBias = 16.0f;
 constexpr int kChunk = 64, kBlocks = kChunk / kF8Span;
 
-// A load with the non-temporal hint: of bytes that the launch reads once.
-template <class T>
-__device__ __forceinline__ T ld_once(GlobalBytes p) {
+// A load; kOnce: with the non-temporal hint, of cache lines that no other wave reads.
+template <class T, bool kOnce>
+__device__ __forceinline__ T load_of(GlobalBytes p) {
   typedef T __attribute__((address_space(1))) Global;
-  return __builtin_nontemporal_load(reinterpret_cast<const Global*>(p));
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const Global*>(p));
+  else return *reinterpret_cast<const Global*>(p);
 }
 
 template <int kWords>
@@ -66,7 +67,7 @@ __device__ __forceinline__ uint32_t word(uint32_t w, int) { return w; }
 template <class V>
 __device__ __forceinline__ uint32_t word(const V& w, int i) { return w[i]; }
 
-template <int D, bool kF16>
+template <int D, bool kF16, bool kOnce>
 __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
     const F8Params p) {
   using R = RowsDim<D>;
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
       for (int b = 0; b < kBlocks; ++b) {
         const GlobalBytes src = block_at(k_at, b);
 #pragma unroll
-        for (int j = 0; j < R::kK; ++j) kf[b][j] = ld_once<u32x4>(src + k_here + 64 * j);
+        for (int j = 0; j < R::kK; ++j) kf[b][j] = load_of<u32x4, kOnce>(src + k_here + 64 * j);
       }
     };
     const auto load_v = [&] {
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
         const GlobalBytes src = block_at(v_at, b);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          vf[b][e] = ld_once<V>(src + e * static_cast<uint32_t>(p.v.s_slot) + v_here);
+          vf[b][e] = load_of<V, kOnce>(src + e * static_cast<uint32_t>(p.v.s_slot) + v_here);
       }
     };
     if (k0 < k_end) {
@@ -333,7 +334,8 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
           // The keys of which a column holds a NaN, as bits; then the columns of the
           // lane's row that see one of them, for the unit's end.
           uint64_t* keys = s_nan_keys[wave];
-          for (int i = lane; i < D; i += 64) keys[i] = 0;
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) keys[64 * i + lane] = 0;
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -347,7 +349,10 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
                            static_cast<unsigned long long>(n >> (8 * c + 7) & 1u)
                                << (16 * b + 4 * g + e));
               }
-          // No branch here differs between lanes: it would change the loop's form.
+          // No branch or loop here differs between lanes. It would change the outer
+          // loop's form; and where a loop of a lane's own columns ended, the compiler put
+          // the copies that save the walk's registers before the lanes were switched on
+          // again (D = 256), so that the next unit was looked up with what lay there.
           const auto before = [](int key) {  // bits of the keys before it
             return key <= 0 ? 0ull : ~0ull >> (64 - min(key, 64));
           };
@@ -452,18 +457,27 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
 hipError_t launch_f8_rows_kernel(const F8Params& p, bool f16, int head_size, hipStream_t stream) {
   note_kernel("f8_rows");
   const dim3 grid(static_cast<unsigned>(p.num_wg)), block(64 * kP16Waves);
+  // Two heads of 64 share a cache line where they lie side by side (64 requests of
+  // 1,024 to 32,768 keys, 8 heads: NHD pages 246 us with the hint, 210 without; HND
+  // pages 180, 198. D = 128 346, 371).
+  const auto shared = [&](const CacheStream& s) {
+    return p.num_kv_heads > 1 && s.s_head < 128 && s.s_slot > s.s_head;
+  };
+  const bool once = !(shared(p.k) || shared(p.v));
   switch (head_size) {
     case 64:
-      if (f16) f8_rows<64, true><<<grid, block, 0, stream>>>(p);
-      else f8_rows<64, false><<<grid, block, 0, stream>>>(p);
+      if (f16 && once) f8_rows<64, true, true><<<grid, block, 0, stream>>>(p);
+      else if (f16) f8_rows<64, true, false><<<grid, block, 0, stream>>>(p);
+      else if (once) f8_rows<64, false, true><<<grid, block, 0, stream>>>(p);
+      else f8_rows<64, false, false><<<grid, block, 0, stream>>>(p);
       break;
     case 256:
-      if (f16) f8_rows<256, true><<<grid, block, 0, stream>>>(p);
-      else f8_rows<256, false><<<grid, block, 0, stream>>>(p);
+      if (f16) f8_rows<256, true, true><<<grid, block, 0, stream>>>(p);
+      else f8_rows<256, false, true><<<grid, block, 0, stream>>>(p);
       break;
     default:
-      if (f16) f8_rows<128, true><<<grid, block, 0, stream>>>(p);
-      else f8_rows<128, false><<<grid, block, 0, stream>>>(p);
+      if (f16) f8_rows<128, true, true><<<grid, block, 0, stream>>>(p);
+      else f8_rows<128, false, true><<<grid, block, 0, stream>>>(p);
   }
   return hipGetLastError();
 }

@@ -68,6 +68,8 @@ struct F8Params : P16Params {
   const uint8_t *k_exp, *v_exp;
   int32_t n_sub;
   int32_t causal;
+  // The launch is for requests of so many rows; others are as without tokens.
+  int32_t least_rows, most_rows;
 };
 
 // A cut group: the slots that hold it (0: none is cut) and, above kP16CutShift,
@@ -106,6 +108,8 @@ __device__ __forceinline__ P16Req p16_request_of(const P& p, int r, int q0, int 
   const P16Tokens t = p16_tokens(q0, q1, p.num_tokens);
   x.q0 = t.first;
   x.rows = t.count * p.group;
+  if constexpr (P::kF8)
+    if (x.rows < p.least_rows || x.rows > p.most_rows) x.rows = 0;
   x.len = min(max(len, 0), p.max_keys);
   x.lo = p.window > 0 ? max(x.len - p.window, 0) : 0;
   if constexpr (P::kF8)

@@ -13,7 +13,10 @@ from pth_flash_attn import capi, ops
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
-FEW, MANY = 1, 1 << 20  # max_query_len: the kernel of 16-row units, of 128-row units
+# max_query_len: the kernel of 16-row units, of 128-row units; of both, each for its
+# requests, where more than eight of them could have FAR keys.
+FEW, MANY, BOTH = 1, 17, 1 << 20
+FAR = 1 << 17
 
 
 def check(c, q, q_lens, scale, kernel=None, **kw):
@@ -23,13 +26,13 @@ def check(c, q, q_lens, scale, kernel=None, **kw):
     ref = {k: kw[k] for k in ("window", "causal") if k in kw}
     G = q.shape[1] // c.k.shape[2]
     many = (max(q_lens) if kernel is None else kernel) * G > 16 and not kw.get("decode")
-    assert capi.AttnLib().last_kernel() == ("f8_wide" if many else "f8_rows")
+    assert capi.AttnLib().last_kernel() == ("f8_wide" if many and kernel != BOTH else "f8_rows")
     want, tol = reference(q, c.keys, q_lens, scale, single=many and q.dtype == BF, **ref)
     assert_close(out, want, tol)
     return out
 
 
-@pytest.mark.parametrize("kernel", [FEW, MANY])
+@pytest.mark.parametrize("kernel", [FEW, MANY, BOTH])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize(("layout", "block"), [("NHD", 16), ("HND", 32), ("NHD", 48), ("HND", 816)])
@@ -37,9 +40,11 @@ def test_mixed_lengths(kernel, dtype, D, layout, block):
     """Decodes, drafts, prompts, an empty request, tokens without a place among the keys."""
     q_lens = [1, 3, 0, 17, 1, 40, 2, 70, 5]
     lens = [1, 3, 5, 100, 900, 40, 0, 333, 3]
-    c = make_cache(lens, Hkv=2, D=D, block=block, seed=D + block, layout=layout, width=60)
+    far = kernel == BOTH
+    c = make_cache(lens, Hkv=2, D=D, block=block, seed=D + block, layout=layout,
+                   width=FAR // block + 1 if far else 60)
     q = queries(sum(q_lens), 8, D, dtype, 1)
-    check(c, q, q_lens, 0.3 / math.sqrt(D), kernel)
+    check(c, q, q_lens, 0.3 / math.sqrt(D), kernel, max_len=FAR if far else None)
 
 
 @pytest.mark.parametrize("kernel", [FEW, MANY])
@@ -51,6 +56,34 @@ def test_windows(kernel, window, D, dtype):
     c = make_cache(lens, Hkv=1, D=D, block=32, seed=window)
     q = queries(sum(q_lens), 4, D, dtype, 2)
     check(c, q, q_lens, 1 / math.sqrt(D), kernel, window=window)
+
+
+@pytest.mark.parametrize("window", [0, 3000])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompts_and_decodes_in_a_batch(window, dtype):
+    """Each kernel leaves the other's rows alone, and rows of no request stay; a
+    captured call follows requests that change from one to the other."""
+    q_lens = [1, 60, 1, 4, 5, 1, 0, 1, 130, 1, 2, 1]
+    lens = [700, 60, 33, 4, 500, 1, 9, 0, 3400, 64, 1, 5000]
+    c = make_cache(lens, Hkv=32, D=128, block=16, seed=77)
+    q = queries(sum(q_lens) + 3, 64, 128, dtype, 77)
+    out = check(c, q, q_lens, 0.1, BOTH, window=window)
+    assert out[-3:].isnan().all() and not out[:-3].isnan().any()
+    starts, ws, out = starts_of(q_lens), workspace(128), torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            attend(c, q, q_lens, 0.1, max_q=BOTH, window=window, starts=starts, ws=ws, out=out)
+        for new in (q_lens, q_lens[::-1], [17] * 12, [0] * 12, [1] * 12):
+            starts.copy_(starts_of(new))
+            out.fill_(7.0)
+            graph.replay()
+            eager = torch.full_like(q, 7.0)
+            attend(c, q, new, 0.1, max_q=BOTH, window=window, out=eager)
+            side.synchronize()
+            assert torch.equal(out, eager)
 
 
 @pytest.mark.parametrize("kernel", [FEW, MANY])
