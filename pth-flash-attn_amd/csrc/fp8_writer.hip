@@ -2,19 +2,25 @@
 // and back (fp8.h has the format).
 //
 // The writer. A block's scale depends on all its tokens of the call, which may
-// stand anywhere in slot_mapping. A work-group takes a run of tokens and one
-// KV head, puts the blocks of its tokens into a table in LDS, and reads the
-// whole of slot_mapping against it: then it knows of each of its blocks the
-// first token of the call and the last token of every slot. It takes the
-// blocks whose first token is its own, one for each wave at a time and for K
-// and V apart: the rows of up to 16 tokens in registers, their largest value
-// over the wave, the scale, the codes. So a value is read once and a code
-// written once, whatever the order of the tokens, in one launch and without
-// an atomic in memory. Rows that the block holds already are touched only if
-// its scale grows.
+// stand anywhere in slot_mapping. A work-group takes a run of tokens, of one KV
+// head or of all, puts the blocks of its tokens into a table in LDS, and reads
+// the whole of slot_mapping against it: then it knows of each of its blocks the
+// first token of the call and the last token of every slot. It takes the blocks
+// whose first token is its own, one for each wave at a time, for each head and
+// for K and V apart: the rows of up to 16 tokens in registers, their largest
+// value over the wave, the scale, the codes. So a value is read once and a code
+// written once, whatever the order of the tokens, in one launch and without an
+// atomic in memory. Rows that the block holds already are touched only if its
+// scale grows.
 //
-// The reader: a work-group finds the pages of 16 rows in LDS, then each thread
-// takes 16 codes at a time.
+// Bound: its bytes, behind the reading of slot_mapping (8 heads of 128, bf16:
+// 16,384 tokens, 101 MB, 27.3 us, of which that takes 5; 30,000 tokens 42 us,
+// 4.4 TB/s); latency for a decode step (64 tokens 4.9 us).
+//
+// The reader. A work-group finds the pages of up to 16 rows in LDS, then each
+// thread takes 8 codes, 16 bytes of a 16-bit row, at a time, eight such at once.
+// Bound: its bytes (20,480 tokens, 8 heads of 128, bf16: 126 MB, 26.4 us, 4.8
+// TB/s); latency for short prefixes (256 tokens 4.0 us).
 
 #include <hip/hip_runtime.h>
 
@@ -28,10 +34,18 @@ namespace pa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kWriteTokens = 128;       // of a work-group, at most
-constexpr int kTable = 2 * kWriteTokens;  // entries, a power of two, one per thread
-static_assert(kTable == kThreads, "a thread looks at each entry");
+constexpr int kManyThreads = 1024;
+constexpr int kWriteTokens = 128;         // of a work-group, at most
+constexpr int kTable = 2 * kWriteTokens;  // entries, a power of two
+static_assert(kTable <= kThreads, "a thread looks at an entry");
+// Tokens from which a work-group has kManyThreads threads and all heads, so that fewer
+// of them read slot_mapping, and a work-group's tokens otherwise (8 heads of 128: 16,384
+// tokens 27.3 us, 37.6 with 256 threads and a head; 4,096 11.0 and 13.7; 2,048 9.0 and
+// 8.1; 64 6.9 and 5.0).
+constexpr int kManyTokens = 4096, kFewTokens = 16;
+// Of slot_mapping that a thread asks for at once (4, 8, 16: 16,384 tokens 27.3, 27.3,
+// 28.1 us, 64 tokens 4.9, 5.0, 5.4).
+constexpr int kSlotsAhead = 4;
 
 struct WriteF8Params {
   const char* src[2];  // keys, values
@@ -44,7 +58,7 @@ struct WriteF8Params {
   int32_t n_sub;
   int32_t num_kv_heads;
   int32_t num_tokens;
-  int32_t tokens;  // of a work-group
+  int32_t tokens, heads;  // of a work-group
 };
 
 // Eight values of a source row as 32-bit ones. kWide: on a 16-byte address.
@@ -81,65 +95,79 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
 #pragma unroll
-  for (int i = 32; i > 0; i >>= 1) x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), i)));
+  for (int i = 32; i > 0; i >>= 1)
+    x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), i)));
   return x;
 }
 
-template <int D, class T, bool kWide>
+template <int D, class T, bool kWide, int kThreads>
 __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kPasses = kF8Span / kRows;
-  __shared__ int32_t s_block[kTable], s_first[kTable], s_row[kTable][kF8Span];
+  constexpr int kWaves = kThreads / 64;
+  __shared__ int32_t s_block[kTable], s_first[kTable], s_row[kTable * kF8Span];
   __shared__ int32_t s_list[kTable];
   __shared__ int32_t s_count;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t0 = static_cast<int>(blockIdx.x) * p.tokens;
   const int t1 = min(t0 + p.tokens, p.num_tokens);
-  const int head = blockIdx.y;
+  const int head0 = static_cast<int>(blockIdx.y) * p.heads;
+  const int heads = min(p.heads, p.num_kv_heads - head0);
 
-  s_block[threadIdx.x] = -1;
-  s_first[threadIdx.x] = INT32_MAX;
+  if (threadIdx.x < kTable) {
+    s_block[threadIdx.x] = -1;
+    s_first[threadIdx.x] = INT32_MAX;
+  }
 #pragma unroll
-  for (int i = 0; i < kF8Span; ++i) s_row[threadIdx.x][i] = -1;
+  for (int i = 0; i < kTable * kF8Span / kThreads; ++i) s_row[kThreads * i + threadIdx.x] = -1;
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  const auto place = [](int32_t block) {
-    return static_cast<int>(static_cast<uint32_t>(block) * 0x9e3779b1u >> 24) & (kTable - 1);
-  };
+  const auto place = [](int32_t block) { return (block ^ block >> 8) & (kTable - 1); };
   // At most half of the entries are taken: every search ends at an empty one.
-  for (int t = t0 + static_cast<int>(threadIdx.x); t < t1; t += kThreads) {
-    const int64_t slot = p.slot_mapping[t];
-    if (slot < 0 || slot >= p.num_slots) continue;
-    const int32_t block = static_cast<int32_t>(slot / kF8Span);
-    for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
-      const int32_t was = atomicCAS(&s_block[i], -1, block);
-      if (was == -1 || was == block) break;
-    }
-  }
-  __syncthreads();
-  for (int t = threadIdx.x; t < p.num_tokens; t += kThreads) {
-    const int64_t slot = p.slot_mapping[t];
-    if (slot < 0 || slot >= p.num_slots) continue;
-    const int32_t block = static_cast<int32_t>(slot / kF8Span);
-    for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
-      const int32_t is = s_block[i];
-      if (is == block) {
-        atomicMin(&s_first[i], t);
-        atomicMax(&s_row[i][slot % kF8Span], t);
+  if (static_cast<int>(threadIdx.x) < t1 - t0) {
+    const int64_t slot = p.slot_mapping[t0 + threadIdx.x];
+    if (static_cast<uint64_t>(slot) < static_cast<uint64_t>(p.num_slots)) {
+      const int32_t block = static_cast<int32_t>(slot / kF8Span);
+      for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
+        const int32_t was = atomicCAS(&s_block[i], -1, block);
+        if (was == -1 || was == block) break;
       }
-      if (is == block || is == -1) break;
     }
   }
   __syncthreads();
-  if (s_first[threadIdx.x] >= t0 && s_first[threadIdx.x] < t1)
+  for (int base = 0; base < p.num_tokens; base += kSlotsAhead * kThreads) {
+    int64_t slot[kSlotsAhead];
+#pragma unroll
+    for (int a = 0; a < kSlotsAhead; ++a)
+      slot[a] = p.slot_mapping[min(base + kThreads * a + static_cast<int>(threadIdx.x),
+                                   p.num_tokens - 1)];
+#pragma unroll
+    for (int a = 0; a < kSlotsAhead; ++a) {
+      const int t = base + kThreads * a + static_cast<int>(threadIdx.x);
+      if (t >= p.num_tokens || static_cast<uint64_t>(slot[a]) >= static_cast<uint64_t>(p.num_slots))
+        continue;
+      const int32_t block = static_cast<int32_t>(slot[a] / kF8Span);
+      for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
+        const int32_t is = s_block[i];
+        if (is == block) {
+          atomicMin(&s_first[i], t);
+          atomicMax(&s_row[kF8Span * i + static_cast<int>(slot[a] % kF8Span)], t);
+        }
+        if (is == block || is == -1) break;
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kTable && s_first[threadIdx.x] >= t0 && s_first[threadIdx.x] < t1)
     s_list[atomicAdd(&s_count, 1)] = threadIdx.x;
   __syncthreads();
 
   const int c = lane % kLanes, r = lane / kLanes;
-  const int units = 2 * s_count;
+  const int units = 2 * heads * s_count;
   for (int u = wave; u < units; u += kWaves) {
     const int kv = u & 1;
-    const int entry = __builtin_amdgcn_readfirstlane(s_list[u >> 1]);
+    const int of = (u >> 1) / heads, head = head0 + (u >> 1) - of * heads;
+    const int entry = __builtin_amdgcn_readfirstlane(s_list[of]);
     const int32_t block = __builtin_amdgcn_readfirstlane(s_block[entry]);
     const int32_t page = static_cast<int32_t>(p.sub_div.div(static_cast<uint32_t>(block)));
     const int32_t sub = block - page * p.n_sub;
@@ -150,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      token[i] = s_row[entry][kRows * i + r];
+      token[i] = s_row[kF8Span * entry + kRows * i + r];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
       if (token[i] >= 0)
@@ -166,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
         top = max(top, b < 0x7f800000u ? b : 0u);
       }
     top = wave_max(top);
-    const bool begun = s_row[entry][0] >= 0;
+    const bool begun = s_row[kF8Span * entry] >= 0;
     const uint32_t old = begun ? 0u : min(had, static_cast<uint32_t>(kF8MostExp));
     const uint32_t e = max(old, exponent_for(top));
     const float unit = e ? __builtin_bit_cast(float, (254u - e) << 23) : 0.0f;
@@ -175,7 +203,8 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
                  static_cast<int64_t>(kF8Span * sub + r) * s.s_slot +
                  static_cast<int64_t>(head) * s.s_head + 8 * c;
     const bool grown = !begun && e > old;
-    const float move = old && old + 127 > e ? __builtin_bit_cast(float, (old + 127u - e) << 23) : 0.0f;
+    const float move =
+        old && old + 127 > e ? __builtin_bit_cast(float, (old + 127u - e) << 23) : 0.0f;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       u32x2* dst = reinterpret_cast<u32x2*>(cell + static_cast<int64_t>(kRows * i) * s.s_slot);
@@ -216,17 +245,19 @@ struct GatherF8Params {
   int64_t reach;  // tokens that a row of the block table holds
   Div32 bs_div, item_div;
   int32_t n_sub, num_blocks, num_reqs, num_tokens, num_kv_heads;
-  int32_t row_items;  // 16-code pieces of a row's heads
+  int32_t row_items;  // 8-code pieces of a row's heads
+  int32_t tokens;     // of a work-group
 };
 
-constexpr int kGatherTokens = 16;
+constexpr int kGatherTokens = 16;  // of a work-group, at most
+constexpr int kPiecesAhead = 8;    // that a thread asks for at once
 
 template <int D, int kType>  // kType: PTH_ATTN_F32, F16 or BF16
 __global__ __launch_bounds__(kThreads) void gather_kv_f8(const GatherF8Params p) {
-  constexpr int kPieces = D / 16;
+  constexpr int kPieces = D / 8, kBytes = kType == PTH_ATTN_F32 ? 4 : 2;
   __shared__ int64_t s_k[kGatherTokens], s_v[kGatherTokens], s_e[kGatherTokens];
-  const int t0 = static_cast<int>(blockIdx.x) * kGatherTokens;
-  if (threadIdx.x < kGatherTokens) {
+  const int t0 = static_cast<int>(blockIdx.x) * p.tokens;
+  if (static_cast<int>(threadIdx.x) < p.tokens) {
     const int t = t0 + static_cast<int>(threadIdx.x);
     // The last request that begins at or before the row, if it ends behind it.
     int lo = 0, hi = p.num_reqs;
@@ -257,44 +288,55 @@ __global__ __launch_bounds__(kThreads) void gather_kv_f8(const GatherF8Params p)
     s_e[threadIdx.x] = e;
   }
   __syncthreads();
-  const int items = 2 * kGatherTokens * p.row_items;
-  for (int i = threadIdx.x; i < items; i += kThreads) {
-    const int row = static_cast<int>(p.item_div.div(static_cast<uint32_t>(i)));
-    const int item = i - row * p.row_items;
-    const int kv = row & 1, t = row >> 1;
-    const int64_t e = s_e[t];
-    if (e == -2) continue;
-    const int head = item / kPieces, c = item % kPieces;
-    u32x4 w = {0u, 0u, 0u, 0u};
-    float scale = 0.0f;
-    if (e >= 0) {
-      w = *reinterpret_cast<const u32x4*>(p.cache[kv].base + (kv ? s_v[t] : s_k[t]) +
-                                          head * p.cache[kv].s_head + 16 * c);
-      scale = f8_scale(p.scale[kv][e + head]);
+  const int items = 2 * p.tokens * p.row_items;
+  for (int base = threadIdx.x; base < items; base += kPiecesAhead * kThreads) {
+    u32x2 w[kPiecesAhead];
+    uint32_t exponent[kPiecesAhead];
+    char* dst[kPiecesAhead];
+#pragma unroll
+    for (int a = 0; a < kPiecesAhead; ++a) {
+      const int i = min(base + kThreads * a, items - 1);
+      const int row = static_cast<int>(p.item_div.div(static_cast<uint32_t>(i)));
+      const int item = i - row * p.row_items;
+      const int kv = row & 1, t = row >> 1;
+      const int head = item / kPieces, c = item % kPieces;
+      // Where there is no page, the null page's codes are read, and not used.
+      const int64_t e = s_e[t];
+      w[a] = *reinterpret_cast<const u32x2*>(p.cache[kv].base + (kv ? s_v[t] : s_k[t]) +
+                                             head * p.cache[kv].s_head + 8 * c);
+      exponent[a] = p.scale[kv][max(e, int64_t{0}) + head];
+      if (e < 0) {
+        w[a] = (u32x2){0u, 0u};
+        exponent[a] = 0;
+      }
+      dst[a] = base + kThreads * a < items && e != -2
+                   ? p.dst[kv] + static_cast<int64_t>(t0 + t) * p.s_tok[kv] + head * p.s_head[kv] +
+                         8 * kBytes * c
+                   : nullptr;
     }
-    char* dst = p.dst[kv] + static_cast<int64_t>(t0 + t) * p.s_tok[kv] +
-                head * p.s_head[kv] + 16 * (kType == PTH_ATTN_F32 ? 4 : 2) * c;
-    float x[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false);
-      const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
-      x[4 * j] = a[0] * scale;
-      x[4 * j + 1] = a[1] * scale;
-      x[4 * j + 2] = b[0] * scale;
-      x[4 * j + 3] = b[1] * scale;
-    }
-    if constexpr (kType == PTH_ATTN_F32) {
+    for (int a = 0; a < kPiecesAhead; ++a) {
+      const float scale = f8_scale(exponent[a]);
+      float x[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        reinterpret_cast<f32x4*>(dst)[j] = (f32x4){x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]};
-    } else {
-      constexpr bool kF16 = kType == PTH_ATTN_F16;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        reinterpret_cast<u32x4*>(dst)[j] = (u32x4){
-            pack16<kF16>(x[8 * j], x[8 * j + 1]), pack16<kF16>(x[8 * j + 2], x[8 * j + 3]),
-            pack16<kF16>(x[8 * j + 4], x[8 * j + 5]), pack16<kF16>(x[8 * j + 6], x[8 * j + 7])};
+      for (int j = 0; j < 2; ++j) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[a][j], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[a][j], true);
+        x[4 * j] = lo[0] * scale;
+        x[4 * j + 1] = lo[1] * scale;
+        x[4 * j + 2] = hi[0] * scale;
+        x[4 * j + 3] = hi[1] * scale;
+      }
+      if (dst[a] == nullptr) continue;
+      if constexpr (kType == PTH_ATTN_F32) {
+        reinterpret_cast<f32x4*>(dst[a])[0] = (f32x4){x[0], x[1], x[2], x[3]};
+        reinterpret_cast<f32x4*>(dst[a])[1] = (f32x4){x[4], x[5], x[6], x[7]};
+      } else {
+        constexpr bool kF16 = kType == PTH_ATTN_F16;
+        *reinterpret_cast<u32x4*>(dst[a]) =
+            (u32x4){pack16<kF16>(x[0], x[1]), pack16<kF16>(x[2], x[3]), pack16<kF16>(x[4], x[5]),
+                    pack16<kF16>(x[6], x[7])};
+      }
     }
   }
 }
@@ -308,16 +350,22 @@ bool on16(const void* p, int64_t tok, int64_t n_tok, int64_t head, int64_t n_hea
          used_stride(head, n_head) % 16 == 0;
 }
 
-template <int D, class T>
+template <int D, class T, int kThreads>
 void write_as(const WriteF8Params& w, bool wide, dim3 grid, hipStream_t stream) {
-  if (wide) write_kv_f8<D, T, true><<<grid, kThreads, 0, stream>>>(w);
-  else write_kv_f8<D, T, false><<<grid, kThreads, 0, stream>>>(w);
+  if (wide) write_kv_f8<D, T, true, kThreads><<<grid, kThreads, 0, stream>>>(w);
+  else write_kv_f8<D, T, false, kThreads><<<grid, kThreads, 0, stream>>>(w);
+}
+template <int D, class T>
+void write_t(const WriteF8Params& w, bool wide, bool many, dim3 grid, hipStream_t stream) {
+  if (many) write_as<D, T, kManyThreads>(w, wide, grid, stream);
+  else write_as<D, T, kThreads>(w, wide, grid, stream);
 }
 template <int D>
-void write_d(const WriteF8Params& w, int dtype, bool wide, dim3 grid, hipStream_t stream) {
-  if (dtype == PTH_ATTN_F32) write_as<D, float>(w, wide, grid, stream);
-  else if (dtype == PTH_ATTN_F16) write_as<D, _Float16>(w, wide, grid, stream);
-  else write_as<D, __bf16>(w, wide, grid, stream);
+void write_d(const WriteF8Params& w, int dtype, bool wide, bool many, dim3 grid,
+             hipStream_t stream) {
+  if (dtype == PTH_ATTN_F32) write_t<D, float>(w, wide, many, grid, stream);
+  else if (dtype == PTH_ATTN_F16) write_t<D, _Float16>(w, wide, many, grid, stream);
+  else write_t<D, __bf16>(w, wide, many, grid, stream);
 }
 template <int D>
 void gather_d(const GatherF8Params& g, int dtype, dim3 grid, hipStream_t stream) {
@@ -398,18 +446,18 @@ int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
   w.num_tokens = a.num_tokens;
   const int32_t cus = resident_workgroups();
   PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
-  // Fewer tokens of a work-group while that leaves compute units idle.
-  w.tokens = kWriteTokens;
-  while (w.tokens > 2 && static_cast<int64_t>(a.num_tokens) * c.num_kv_heads < int64_t{4} * cus * w.tokens)
-    w.tokens /= 2;
+  const bool many = a.num_tokens >= kManyTokens;
+  w.heads = many ? c.num_kv_heads : 1;
+  w.tokens = many ? kWriteTokens : kFewTokens;
+  while (many && w.tokens > kFewTokens && a.num_tokens < cus * w.tokens) w.tokens /= 2;
   const bool wide = on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
                     on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head, c.num_kv_heads);
   const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + w.tokens - 1) / w.tokens),
-                  static_cast<unsigned>(c.num_kv_heads));
+                  static_cast<unsigned>((c.num_kv_heads + w.heads - 1) / w.heads));
   switch (c.head_size) {
-    case 64: write_d<64>(w, a.kv_dtype, wide, grid, stream); break;
-    case 256: write_d<256>(w, a.kv_dtype, wide, grid, stream); break;
-    default: write_d<128>(w, a.kv_dtype, wide, grid, stream);
+    case 64: write_d<64>(w, a.kv_dtype, wide, many, grid, stream); break;
+    case 256: write_d<256>(w, a.kv_dtype, wide, many, grid, stream); break;
+    default: write_d<128>(w, a.kv_dtype, wide, many, grid, stream);
   }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess)
@@ -464,9 +512,16 @@ int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream) {
   g.num_reqs = a.num_reqs;
   g.num_tokens = a.num_tokens;
   g.num_kv_heads = c.num_kv_heads;
-  g.row_items = c.num_kv_heads * (c.head_size / 16);
+  g.row_items = c.num_kv_heads * (c.head_size / 8);
   g.item_div = Div32::make(static_cast<uint32_t>(g.row_items));
-  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + kGatherTokens - 1) / kGatherTokens));
+  // Fewer rows of a work-group while that leaves compute units without a second one
+  // (8 heads of 128, 16, 8 and 4 rows: 20,480 tokens 26.6, 28.1, 36.6 us, 4,096 11.4,
+  // 8.8, 10.5, 1,024 8.5, 5.8, 5.0, 64 8.0, 5.3, 4.5).
+  const int32_t cus = resident_workgroups();
+  PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
+  g.tokens = kGatherTokens;
+  while (g.tokens > 4 && a.num_tokens < 2 * cus * g.tokens) g.tokens /= 2;
+  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + g.tokens - 1) / g.tokens));
   switch (c.head_size) {
     case 64: gather_d<64>(g, a.kv_dtype, grid, stream); break;
     case 256: gather_d<256>(g, a.kv_dtype, grid, stream); break;

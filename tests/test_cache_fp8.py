@@ -84,6 +84,34 @@ def test_orders(T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("odd", [False, True])
+def test_write_many(D, dtype, odd):
+    """As many tokens as give a work-group all heads: runs of blocks, their tokens in
+    order but for some that stand elsewhere in the call, padding between."""
+    block, Hkv, T = (48, 3, 4997) if odd else (16, 1, 4200)
+    key, value = source(T, Hkv, D, dtype, D + 1, odd)
+    pages = T // block + 9
+    gen = torch.Generator(device="cuda").manual_seed(D + odd)
+    slots = torch.arange(T, device="cuda") + 21
+    moved = torch.randperm(T, generator=gen, device="cuda")[:200]
+    slots[moved] = slots[moved.roll(1)]
+    slots[77::501] = -1
+    slots[78::503] = slots[5]
+    check_write(key, value, filled(pages, block, Hkv, D, "HND" if odd else "NHD", 8, 16 * odd), slots)
+
+
+@pytest.mark.gpu
+def test_write_longest_runs():
+    """The most tokens of a work-group, each in a block of its own."""
+    T = 34000
+    key, value = source(T, 1, 64, BF, 12)
+    slots = 16 * torch.randperm(T, generator=torch.Generator().manual_seed(1)).cuda() + 3
+    check_write(key, value, filled(T, 16, 1, 64, "NHD", 9), slots)
+
+
+@pytest.mark.gpu
 def test_growth_and_begin():
     """A block's scale grows with its tokens and not back; its first slot begins
     it anew."""
@@ -160,6 +188,20 @@ def test_gather(D, dtype, layout):
         want = torch.cat([c.keys[r][j][first[r] : first[r] + n[r]] for r in range(5)])
         assert torch.equal(out[2 : 2 + len(want)], want.to(dtype))
         assert (out[:2] == 7).all() and (out[2 + len(want) :] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [(2100, 1, 2095), (4000, 0, 4999, 3)])
+def test_gather_many(n):
+    """Work-groups of more rows, which requests end inside of."""
+    first = [3 + 16 * r for r in range(len(n))]
+    c = make_cache([a + b for a, b in zip(first, n)], Hkv=3, D=64, block=16, seed=5, spread=40)
+    outs = [torch.full((sum(n) + 1, 3, 64), 7.0, dtype=BF, device="cuda") for _ in range(2)]
+    ops.gather_cache_fp8(*outs, *c.views, c.table, starts_of(n),
+                         torch.tensor(first, dtype=torch.int32, device="cuda"))
+    for out, j in ((outs[0], 0), (outs[1], 1)):
+        want = torch.cat([c.keys[r][j][first[r] :] for r in range(len(n))])
+        assert torch.equal(out[:-1], want.to(BF)) and (out[-1] == 7).all()
 
 
 @pytest.mark.gpu
