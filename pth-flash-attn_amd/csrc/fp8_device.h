@@ -9,17 +9,22 @@
 namespace pa {
 namespace {
 
+// A run of codes, and its words.
+template <int kWords>
+struct Words;
+template <>
+struct Words<1> { typedef uint32_t type; };
+template <>
+struct Words<2> { typedef u32x2 type; };
+template <>
+struct Words<4> { typedef u32x4 type; };
+__device__ __forceinline__ uint32_t word(uint32_t w, int) { return w; }
+template <class V>
+__device__ __forceinline__ uint32_t word(const V& w, int i) { return w[i]; }
+
 // 2^(e - 127), 0 for e = 0.
 __device__ __forceinline__ float f8_scale(uint32_t e) {
   return __builtin_bit_cast(float, min(e, static_cast<uint32_t>(kF8MostExp)) << 23);
-}
-
-// A byte of a wave-uniform address on the scalar unit, which reads the aligned
-// word that holds it (allocations are whole words).
-__device__ __forceinline__ uint32_t ld_ro_byte(const uint8_t* p) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-  const uint32_t w = static_cast<uint32_t>(ld_ro(reinterpret_cast<const int32_t*>(a & ~uintptr_t{3}), 0));
-  return w >> (8 * (a & 3)) & 0xffu;
 }
 
 // Where a block of 16 keys begins in K and in V, and its exponents (K's, and V's

@@ -55,18 +55,6 @@ __device__ __forceinline__ T load_of(GlobalBytes p) {
   else return *reinterpret_cast<const Global*>(p);
 }
 
-template <int kWords>
-struct Words;
-template <>
-struct Words<1> { typedef uint32_t type; };
-template <>
-struct Words<2> { typedef u32x2 type; };
-template <>
-struct Words<4> { typedef u32x4 type; };
-__device__ __forceinline__ uint32_t word(uint32_t w, int) { return w; }
-template <class V>
-__device__ __forceinline__ uint32_t word(const V& w, int i) { return w[i]; }
-
 template <int D, bool kF16, bool kOnce>
 __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
     const F8Params p) {

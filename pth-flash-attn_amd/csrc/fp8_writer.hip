@@ -13,14 +13,17 @@
 // atomic in memory. Rows that the block holds already are touched only if its
 // scale grows.
 //
-// Bound: its bytes, behind the reading of slot_mapping (8 heads of 128, bf16:
-// 16,384 tokens, 101 MB, 27.3 us, of which that takes 5; 30,000 tokens 42 us,
-// 4.4 TB/s); latency for a decode step (64 tokens 4.9 us).
+// Bound: its bytes, behind the reading of slot_mapping (8 heads of 128, bf16, cold:
+// 16,384 tokens, 101 MB, 26.8 us, of which that takes some 4); latency for a decode
+// step, whose tokens lie in blocks of their own (64 tokens 5.3 us).
 //
-// The reader. A work-group finds the pages of up to 16 rows in LDS, then each
-// thread takes 8 codes, 16 bytes of a 16-bit row, at a time, eight such at once.
-// Bound: its bytes (20,480 tokens, 8 heads of 128, bf16: 126 MB, 26.4 us, 4.8
-// TB/s); latency for short prefixes (256 tokens 4.0 us).
+// The reader. A work-group finds the pages of up to 16 rows in LDS, then each thread
+// reads four pieces of codes at once and writes each as 16 bytes, a wave of them a
+// kilobyte, past the caches (20,480 tokens, 8 heads of 128, bf16: 23.0 us, 30.0 with
+// plain stores). Waves take K or V, not lanes: lanes that differ would read the
+// launch's parameters from memory (48 us).
+// Bound: its bytes (126 MB, 5.5 TB/s); latency for short prefixes (200 tokens of 4
+// heads of 64 2.9 us).
 
 #include <hip/hip_runtime.h>
 
@@ -38,11 +41,16 @@ constexpr int kManyThreads = 1024;
 constexpr int kWriteTokens = 128;         // of a work-group, at most
 constexpr int kTable = 2 * kWriteTokens;  // entries, a power of two
 static_assert(kTable <= kThreads, "a thread looks at an entry");
-// Tokens from which a work-group has kManyThreads threads and all heads, so that fewer
-// of them read slot_mapping, and a work-group's tokens otherwise (8 heads of 128: 16,384
-// tokens 27.3 us, 37.6 with 256 threads and a head; 4,096 11.0 and 13.7; 2,048 9.0 and
-// 8.1; 64 6.9 and 5.0).
-constexpr int kManyTokens = 4096, kFewTokens = 16;
+// A work-group has 256 threads, one head and 2 or 4 tokens where that makes no more than
+// four work-groups for a compute unit; otherwise kManyThreads threads, and 16 tokens of a
+// head or, from so many tokens on, 8 to kWriteTokens of all heads, so that few read
+// slot_mapping (8 heads of 128, from cold memory: 16,384 tokens in runs 26.8 us, 100 with
+// 256 threads and 16 tokens; 1,024 tokens in blocks of their own 14.0, and 28.0 with 8
+// tokens of all heads, in runs 6.7 and 7.3; 64 in blocks of their own 5.3, 20 with 16
+// tokens and 256 threads).
+constexpr int kManyTokens = 2048;
+// A filter of blocks, bits: without it 16,384 tokens take 28.7 us.
+constexpr int kFilter = 16384;
 // Of slot_mapping that a thread asks for at once (4, 8, 16: 16,384 tokens 27.3, 27.3,
 // 28.1 us, 64 tokens 4.9, 5.0, 5.4).
 constexpr int kSlotsAhead = 4;
@@ -106,6 +114,7 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
   constexpr int kWaves = kThreads / 64;
   __shared__ int32_t s_block[kTable], s_first[kTable], s_row[kTable * kF8Span];
   __shared__ int32_t s_list[kTable];
+  __shared__ uint32_t s_maybe[kFilter / 32];
   __shared__ int32_t s_count;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,44 +123,66 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
   const int head0 = static_cast<int>(blockIdx.y) * p.heads;
   const int heads = min(p.heads, p.num_kv_heads - head0);
 
+  // The run's slots and the first ones of all are asked for before the table is clear.
+  int64_t own = -1, slot[kSlotsAhead];
+  if (static_cast<int>(threadIdx.x) < t1 - t0) own = p.slot_mapping[t0 + threadIdx.x];
+  const auto ask = [&](int base) {
+#pragma unroll
+    for (int a = 0; a < kSlotsAhead; ++a)
+      slot[a] = p.slot_mapping[min(base + kThreads * a + static_cast<int>(threadIdx.x),
+                                   p.num_tokens - 1)];
+  };
+  ask(0);
   if (threadIdx.x < kTable) {
     s_block[threadIdx.x] = -1;
     s_first[threadIdx.x] = INT32_MAX;
   }
 #pragma unroll
   for (int i = 0; i < kTable * kF8Span / kThreads; ++i) s_row[kThreads * i + threadIdx.x] = -1;
+#pragma unroll
+  for (int i = threadIdx.x; i < kFilter / 32; i += kThreads) s_maybe[i] = 0;
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
   const auto place = [](int32_t block) { return (block ^ block >> 8) & (kTable - 1); };
+  // A bit for each block, shared by few: most tokens of other runs end there.
+  const auto filter = [](int64_t of) {
+    const uint32_t block = static_cast<uint32_t>(of / kF8Span);
+    return (block ^ block >> 14) & (kFilter - 1);
+  };
+  const auto known = [&](int64_t of) {
+    return static_cast<uint64_t>(of) < static_cast<uint64_t>(p.num_slots);
+  };
   // At most half of the entries are taken: every search ends at an empty one.
-  if (static_cast<int>(threadIdx.x) < t1 - t0) {
-    const int64_t slot = p.slot_mapping[t0 + threadIdx.x];
-    if (static_cast<uint64_t>(slot) < static_cast<uint64_t>(p.num_slots)) {
-      const int32_t block = static_cast<int32_t>(slot / kF8Span);
-      for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
-        const int32_t was = atomicCAS(&s_block[i], -1, block);
-        if (was == -1 || was == block) break;
-      }
+  if (known(own)) {
+    const int32_t block = static_cast<int32_t>(own / kF8Span);
+    for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
+      const int32_t was = atomicCAS(&s_block[i], -1, block);
+      if (was == -1 || was == block) break;
     }
+    const uint32_t bit = filter(own);
+    atomicOr(&s_maybe[bit >> 5], 1u << (bit & 31));
   }
   __syncthreads();
   for (int base = 0; base < p.num_tokens; base += kSlotsAhead * kThreads) {
-    int64_t slot[kSlotsAhead];
+    int64_t now[kSlotsAhead];
+    bool maybe[kSlotsAhead];
 #pragma unroll
-    for (int a = 0; a < kSlotsAhead; ++a)
-      slot[a] = p.slot_mapping[min(base + kThreads * a + static_cast<int>(threadIdx.x),
-                                   p.num_tokens - 1)];
+    for (int a = 0; a < kSlotsAhead; ++a) {
+      now[a] = slot[a];
+      const uint32_t bit = filter(now[a]);
+      maybe[a] = s_maybe[bit >> 5] >> (bit & 31) & 1;
+    }
+    if (base + kSlotsAhead * kThreads < p.num_tokens) ask(base + kSlotsAhead * kThreads);
 #pragma unroll
     for (int a = 0; a < kSlotsAhead; ++a) {
       const int t = base + kThreads * a + static_cast<int>(threadIdx.x);
-      if (t >= p.num_tokens || static_cast<uint64_t>(slot[a]) >= static_cast<uint64_t>(p.num_slots))
-        continue;
-      const int32_t block = static_cast<int32_t>(slot[a] / kF8Span);
+      if (!maybe[a] || t >= p.num_tokens || !known(now[a])) continue;
+      const int32_t block = static_cast<int32_t>(now[a] / kF8Span);
       for (int i = place(block);; i = (i + 1) & (kTable - 1)) {
         const int32_t is = s_block[i];
         if (is == block) {
           atomicMin(&s_first[i], t);
-          atomicMax(&s_row[kF8Span * i + static_cast<int>(slot[a] % kF8Span)], t);
+          atomicMax(&s_row[kF8Span * i + static_cast<int>(now[a] % kF8Span)], t);
         }
         if (is == block || is == -1) break;
       }
@@ -173,18 +204,27 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
     const int32_t sub = block - page * p.n_sub;
     uint8_t* exponent = p.scale[kv] + static_cast<int64_t>(block) * p.num_kv_heads + head;
     const uint32_t had = *exponent;
+    const CacheStream& s = p.cache[kv];
+    char* cell = const_cast<char*>(s.base) + static_cast<int64_t>(page) * s.s_block +
+                 static_cast<int64_t>(kF8Span * sub + r) * s.s_slot +
+                 static_cast<int64_t>(head) * s.s_head + 8 * c;
+    const bool begun = s_row[kF8Span * entry] >= 0;
     int32_t token[kPasses];
     float x[kPasses][8];
+    u32x2 held[kPasses];  // what the block's other rows hold, in case its scale grows
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       token[i] = s_row[kF8Span * entry + kRows * i + r];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+      held[i] = (u32x2){0u, 0u};
       if (token[i] >= 0)
         load_eight<T, kWide>(p.src[kv] + static_cast<int64_t>(token[i]) * p.s_tok[kv] +
                                  static_cast<int64_t>(head) * p.s_head[kv] + 8 * sizeof(T) * c,
                              x[i]);
+      else if (!begun)
+        held[i] = *reinterpret_cast<const u32x2*>(cell + static_cast<int64_t>(kRows * i) * s.s_slot);
     }
 #pragma unroll
     for (int i = 0; i < kPasses; ++i)
@@ -194,14 +234,9 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
         top = max(top, b < 0x7f800000u ? b : 0u);
       }
     top = wave_max(top);
-    const bool begun = s_row[kF8Span * entry] >= 0;
     const uint32_t old = begun ? 0u : min(had, static_cast<uint32_t>(kF8MostExp));
     const uint32_t e = max(old, exponent_for(top));
     const float unit = e ? __builtin_bit_cast(float, (254u - e) << 23) : 0.0f;
-    const CacheStream& s = p.cache[kv];
-    char* cell = const_cast<char*>(s.base) + static_cast<int64_t>(page) * s.s_block +
-                 static_cast<int64_t>(kF8Span * sub + r) * s.s_slot +
-                 static_cast<int64_t>(head) * s.s_head + 8 * c;
     const bool grown = !begun && e > old;
     const float move =
         old && old + 127 > e ? __builtin_bit_cast(float, (old + 127u - e) << 23) : 0.0f;
@@ -218,12 +253,11 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
         *dst = (u32x2){codes4(x[i][0], x[i][1], x[i][2], x[i][3]),
                        codes4(x[i][4], x[i][5], x[i][6], x[i][7])};
       } else if (grown) {
-        const u32x2 w = *dst;
         u32x2 y;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false);
-          const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], false);
+          const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], true);
           y[j] = codes4(a[0] * move, a[1] * move, b[0] * move, b[1] * move);
         }
         *dst = y;
@@ -245,98 +279,110 @@ struct GatherF8Params {
   int64_t reach;  // tokens that a row of the block table holds
   Div32 bs_div, item_div;
   int32_t n_sub, num_blocks, num_reqs, num_tokens, num_kv_heads;
-  int32_t row_items;  // 8-code pieces of a row's heads
+  int32_t row_items;  // pieces of a row's heads
   int32_t tokens;     // of a work-group
 };
 
 constexpr int kGatherTokens = 16;  // of a work-group, at most
-constexpr int kPiecesAhead = 8;    // that a thread asks for at once
+constexpr int kPiecesAhead = 4;    // that a thread asks for at once
 
 template <int D, int kType>  // kType: PTH_ATTN_F32, F16 or BF16
 __global__ __launch_bounds__(kThreads) void gather_kv_f8(const GatherF8Params p) {
-  constexpr int kPieces = D / 8, kBytes = kType == PTH_ATTN_F32 ? 4 : 2;
-  __shared__ int64_t s_k[kGatherTokens], s_v[kGatherTokens], s_e[kGatherTokens];
+  constexpr int kBytes = kType == PTH_ATTN_F32 ? 4 : 2;
+  constexpr int kCodes = 16 / kBytes, kPieces = D / kCodes;  // of a piece; of a head's row
+  __shared__ int64_t s_at[2][kGatherTokens], s_e[kGatherTokens];
   const int t0 = static_cast<int>(blockIdx.x) * p.tokens;
-  if (static_cast<int>(threadIdx.x) < p.tokens) {
-    const int t = t0 + static_cast<int>(threadIdx.x);
-    // The last request that begins at or before the row, if it ends behind it.
-    int lo = 0, hi = p.num_reqs;
+  {
+    // The last request that begins at or before the row, if it ends behind it: 16 lanes
+    // look for a row's, a 16th of the requests that are left at each step.
+    const int of = threadIdx.x / 16, j = threadIdx.x % 16, group = threadIdx.x & 48;
+    const int t = t0 + of;
+    int lo = 0, hi = of < p.tokens ? p.num_reqs : 0;
     while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (p.starts[mid + 1] <= t) lo = mid + 1;
-      else hi = mid;
+      const int step = (hi - lo + 15) >> 4, at = lo + (j + 1) * step;
+      const bool begun = at <= hi && p.starts[at] <= t;
+      const int n = __popcll(__ballot(begun) >> group & 0xffff);
+      hi = min(hi, lo + (n + 1) * step - 1);
+      lo = min(lo + n * step, hi);
     }
-    int64_t e = -2;  // -2: no request's; -1: no page
-    int64_t k = 0, v = 0;
-    if (t < p.num_tokens && lo < p.num_reqs && p.starts[lo] <= t) {
-      e = -1;
-      const int64_t pos = static_cast<int64_t>(p.first ? p.first[lo] : 0) + t -
-                          static_cast<int64_t>(p.starts[lo]);
-      if (pos >= 0 && pos < p.reach) {
-        const uint32_t entry = p.bs_div.div(static_cast<uint32_t>(pos));
-        const int32_t page = p.block_table[lo * p.bt_stride + entry];
-        if (page >= 0 && page < p.num_blocks) {
-          const int64_t in = pos - static_cast<int64_t>(entry) * p.bs_div.d;
-          k = page * p.cache[0].s_block + in * p.cache[0].s_slot;
-          v = page * p.cache[1].s_block + in * p.cache[1].s_slot;
-          e = (static_cast<int64_t>(page) * p.n_sub + in / kF8Span) * p.num_kv_heads;
+    if (j == 0 && of < p.tokens) {
+      int64_t e = -2;  // -2: no request's; -1: no page
+      int64_t k = 0, v = 0;
+      if (t < p.num_tokens && lo < p.num_reqs && p.starts[lo] <= t) {
+        e = -1;
+        const int64_t pos = static_cast<int64_t>(p.first ? p.first[lo] : 0) + t -
+                            static_cast<int64_t>(p.starts[lo]);
+        if (pos >= 0 && pos < p.reach) {
+          const uint32_t entry = p.bs_div.div(static_cast<uint32_t>(pos));
+          const int32_t page = p.block_table[lo * p.bt_stride + entry];
+          if (page >= 0 && page < p.num_blocks) {
+            const int64_t in = pos - static_cast<int64_t>(entry) * p.bs_div.d;
+            k = page * p.cache[0].s_block + in * p.cache[0].s_slot;
+            v = page * p.cache[1].s_block + in * p.cache[1].s_slot;
+            e = (static_cast<int64_t>(page) * p.n_sub + in / kF8Span) * p.num_kv_heads;
+          }
         }
       }
+      s_at[0][of] = k;
+      s_at[1][of] = v;
+      s_e[of] = e;
     }
-    s_k[threadIdx.x] = k;
-    s_v[threadIdx.x] = v;
-    s_e[threadIdx.x] = e;
   }
   __syncthreads();
-  const int items = 2 * p.tokens * p.row_items;
-  for (int base = threadIdx.x; base < items; base += kPiecesAhead * kThreads) {
-    u32x2 w[kPiecesAhead];
+  // K by the even waves, V by the odd ones.
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kv = wave & 1;
+  const CacheStream s = p.cache[kv];
+  const uint8_t* exponents = p.scale[kv];
+  char* out = p.dst[kv] + static_cast<int64_t>(t0) * p.s_tok[kv];
+  constexpr int kStep = kThreads / 2;
+  const int items = p.tokens * p.row_items;
+  for (int base = (wave >> 1) * 64 + static_cast<int>(threadIdx.x & 63); base < items;
+       base += kPiecesAhead * kStep) {
+    typedef typename Words<kCodes / 4>::type Piece;
+    Piece w[kPiecesAhead];
     uint32_t exponent[kPiecesAhead];
     char* dst[kPiecesAhead];
 #pragma unroll
     for (int a = 0; a < kPiecesAhead; ++a) {
-      const int i = min(base + kThreads * a, items - 1);
-      const int row = static_cast<int>(p.item_div.div(static_cast<uint32_t>(i)));
-      const int item = i - row * p.row_items;
-      const int kv = row & 1, t = row >> 1;
+      const int i = min(base + kStep * a, items - 1);
+      const int t = static_cast<int>(p.item_div.div(static_cast<uint32_t>(i)));
+      const int item = i - t * p.row_items;
       const int head = item / kPieces, c = item % kPieces;
       // Where there is no page, the null page's codes are read, and not used.
       const int64_t e = s_e[t];
-      w[a] = *reinterpret_cast<const u32x2*>(p.cache[kv].base + (kv ? s_v[t] : s_k[t]) +
-                                             head * p.cache[kv].s_head + 8 * c);
-      exponent[a] = p.scale[kv][max(e, int64_t{0}) + head];
+      w[a] = *reinterpret_cast<const Piece*>(s.base + s_at[kv][t] + head * s.s_head + kCodes * c);
+      exponent[a] = exponents[max(e, int64_t{0}) + head];
       if (e < 0) {
-        w[a] = (u32x2){0u, 0u};
+        w[a] = Piece{};
         exponent[a] = 0;
       }
-      dst[a] = base + kThreads * a < items && e != -2
-                   ? p.dst[kv] + static_cast<int64_t>(t0 + t) * p.s_tok[kv] + head * p.s_head[kv] +
-                         8 * kBytes * c
+      dst[a] = base + kStep * a < items && e != -2
+                   ? out + t * p.s_tok[kv] + head * p.s_head[kv] + kCodes * kBytes * c
                    : nullptr;
     }
 #pragma unroll
     for (int a = 0; a < kPiecesAhead; ++a) {
       const float scale = f8_scale(exponent[a]);
-      float x[8];
+      float x[kCodes];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[a][j], false);
-        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[a][j], true);
+      for (int j = 0; j < kCodes / 4; ++j) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(word(w[a], j), false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(word(w[a], j), true);
         x[4 * j] = lo[0] * scale;
         x[4 * j + 1] = lo[1] * scale;
         x[4 * j + 2] = hi[0] * scale;
         x[4 * j + 3] = hi[1] * scale;
       }
       if (dst[a] == nullptr) continue;
+      u32x4 y;
       if constexpr (kType == PTH_ATTN_F32) {
-        reinterpret_cast<f32x4*>(dst[a])[0] = (f32x4){x[0], x[1], x[2], x[3]};
-        reinterpret_cast<f32x4*>(dst[a])[1] = (f32x4){x[4], x[5], x[6], x[7]};
+        y = __builtin_bit_cast(u32x4, (f32x4){x[0], x[1], x[2], x[3]});
       } else {
         constexpr bool kF16 = kType == PTH_ATTN_F16;
-        *reinterpret_cast<u32x4*>(dst[a]) =
-            (u32x4){pack16<kF16>(x[0], x[1]), pack16<kF16>(x[2], x[3]), pack16<kF16>(x[4], x[5]),
-                    pack16<kF16>(x[6], x[7])};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = pack16<kF16>(x[2 * j], x[2 * j + 1]);
       }
+      __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(dst[a]));
     }
   }
 }
@@ -446,10 +492,18 @@ int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
   w.num_tokens = a.num_tokens;
   const int32_t cus = resident_workgroups();
   PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
-  const bool many = a.num_tokens >= kManyTokens;
-  w.heads = many ? c.num_kv_heads : 1;
-  w.tokens = many ? kWriteTokens : kFewTokens;
-  while (many && w.tokens > kFewTokens && a.num_tokens < cus * w.tokens) w.tokens /= 2;
+  w.tokens = 2;
+  w.heads = 1;
+  while (static_cast<int64_t>(a.num_tokens) * c.num_kv_heads > int64_t{4} * cus * w.tokens)
+    w.tokens *= 2;
+  const bool many = w.tokens > 4;
+  if (many && a.num_tokens < kManyTokens) {
+    w.tokens = 16;
+  } else if (many) {
+    w.heads = c.num_kv_heads;
+    w.tokens = 8;
+    while (w.tokens < kWriteTokens && a.num_tokens >= 2 * cus * w.tokens) w.tokens *= 2;
+  }
   const bool wide = on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
                     on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head, c.num_kv_heads);
   const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + w.tokens - 1) / w.tokens),
@@ -477,8 +531,9 @@ int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream) {
   PA_REQUIRE(sizes.empty(), sizes);
   PA_REQUIRE(a.kv_dtype == PTH_ATTN_F32 || a.kv_dtype == PTH_ATTN_F16 || a.kv_dtype == PTH_ATTN_BF16,
              "kv_dtype must be PTH_ATTN_F32, PTH_ATTN_F16 or PTH_ATTN_BF16");
-  PA_REQUIRE(a.num_tokens >= 0 && a.num_reqs >= 0 && a.block_table_width >= 0,
-             "num_tokens, num_reqs and block_table_width must be >= 0");
+  PA_REQUIRE(a.num_tokens >= 0 && a.num_reqs >= 0 && a.num_reqs < 1 << 30 &&
+                 a.block_table_width >= 0,
+             "num_tokens and block_table_width must be >= 0, num_reqs 0 .. 2^30 - 1");
   if (a.num_tokens == 0 || a.num_reqs == 0) return PTH_ATTN_OK;
   PA_REQUIRE(a.key && a.value && a.row_start_loc, "key, value and row_start_loc must be non-NULL");
   PA_REQUIRE(a.block_table || a.block_table_width == 0, "block_table must be non-NULL");
@@ -512,15 +567,17 @@ int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream) {
   g.num_reqs = a.num_reqs;
   g.num_tokens = a.num_tokens;
   g.num_kv_heads = c.num_kv_heads;
-  g.row_items = c.num_kv_heads * (c.head_size / 8);
+  g.row_items = c.num_kv_heads * (c.head_size / (a.kv_dtype == PTH_ATTN_F32 ? 4 : 8));
   g.item_div = Div32::make(static_cast<uint32_t>(g.row_items));
-  // Fewer rows of a work-group while that leaves compute units without a second one
-  // (8 heads of 128, 16, 8 and 4 rows: 20,480 tokens 26.6, 28.1, 36.6 us, 4,096 11.4,
-  // 8.8, 10.5, 1,024 8.5, 5.8, 5.0, 64 8.0, 5.3, 4.5).
   const int32_t cus = resident_workgroups();
   PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
+  // A work-group's rows: few enough for one turn of its threads; fewer where that leaves
+  // compute units without a second work-group (8 heads of 128, 16, 8, 4 rows: 20,480
+  // tokens 25.9, 24.0, 23.0 us, 1,024 7.8, 5.6, 4.4; one head, 20,480 5.6, 7.5, 8.8).
   g.tokens = kGatherTokens;
-  while (g.tokens > 4 && a.num_tokens < 2 * cus * g.tokens) g.tokens /= 2;
+  while (g.tokens > 2 && (g.tokens * g.row_items > kPiecesAhead * kThreads / 2 ||
+                          (g.tokens > 4 && a.num_tokens < 2 * cus * g.tokens)))
+    g.tokens /= 2;
   const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + g.tokens - 1) / g.tokens));
   switch (c.head_size) {
     case 64: gather_d<64>(g, a.kv_dtype, grid, stream); break;
