@@ -50,9 +50,14 @@ int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
 }
 
 // Whether every group is left whole, so that there is nothing to join: where
-// all are short.
-bool whole_rows(int32_t head_size, int64_t span) {
-  return span <= (head_size == 256 ? 128 : 512);
+// all are short. Decodes, whole and cut, 512 keys: 1 request and 1 KV head of 128
+// 8.1 and 9.5 us, 64 and 8 heads 19.3 and 19.9; 768 keys 9.5 and 9.5, 26.4 and 25.2;
+// 1,024 keys 12.3 and 10.0, 33.5 and 30.4. Heads of 64, 1,024 keys: 16 requests, 8 heads
+// 10.3 and 11.2, 64 requests 25.5 and 22.8. Heads of 256, 64 requests, 4 heads, 256 keys
+// 14.5 and 17.0, 512 keys 20.0 and 21.0, of one request 16.9 and 15.9.
+bool whole_rows(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
+  if (head_size == 256) return span <= 256;
+  return span <= (head_size == 64 && units <= cus / 2 ? 1024 : 512);
 }
 bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   const int64_t round = int64_t{p16_resident(head_size)} * cus;
@@ -100,10 +105,16 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   const int64_t span = span_of(p, tokens);
   const int64_t units = row_tiles * p.num_kv_heads;
   if (units == 0) return PTH_ATTN_OK;
-  const bool whole = wide ? whole_wide(head_size, span, units, cus) : whole_rows(head_size, span);
+  const bool whole = wide ? whole_wide(head_size, span, units, cus) : whole_rows(head_size, span, units, cus);
   p.team = wide ? 1 : team_of(p, span, std::min(bm, longest * p.group), whole, cus);
+  // Fewer units side by side while compute units lack work-groups, and further only
+  // where all of a unit's waves have keys (8 heads of 128, 128 keys, one unit and two: 16
+  // requests 6.9 and 7.5 us, 64 requests 8.8 and 8.0).
   if (whole)
-    while (p.team > 1 && units / p.team < p16_resident(head_size) * cus) p.team /= 2;
+    while (p.team > 1 && (units / p.team < cus ||
+                          (units / p.team < p16_resident(head_size) * cus &&
+                           64 * 2 * kP16Waves / p.team <= span + 63)))
+      p.team /= 2;
   p.key_tile_log2 = wide ? 6 : 8 - (p.team >> 1);
   if (whole)
     while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
