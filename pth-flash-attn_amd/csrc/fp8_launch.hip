@@ -59,12 +59,16 @@ bool whole_rows(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   if (head_size == 256) return span <= 256;
   return span <= (head_size == 64 && units <= cus / 2 ? 1024 : 512);
 }
+// Prompts, where the units are as many as the longest has a share in the whole: whole
+// ones end unevenly, cut ones write and read their sums. 8 heads of 128, whole and cut: 1
+// prompt of 2,048 tokens 63 and 74 us, of 8,192 550 and 610; 4 of 2,048 173 and 216; 4 of
+// 1,800 behind 4,000 keys 600 and 625; one head, 1 of 2,048 53 and 40, 5 of 2,000 behind
+// 2,000 189 and 153. Heads of 256, 4 of them: 1 of 1,024 58 and 52, of 4,096 211 and 277.
+// Many short units are better walked by work-groups that stay: 64 of 256 140 and 123.
 bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
-  const int64_t round = int64_t{p16_resident(head_size)} * cus;
-  int64_t most = head_size == 256 ? 512 : 1024;
-  if (units < cus / 8 || units > 8 * cus) most = head_size == 256 ? 128 : 512;
-  else if (10 * units >= 7 * round && units <= round) most = 1536;
-  return span <= most;
+  if (units > 5 * p16_resident(head_size) * cus && span < 1024) return false;
+  if (head_size == 256) return span <= 512 || (units >= cus && span * cus <= 2048 * units);
+  return span <= 1024 || span * cus <= 1024 * units;
 }
 
 // The keys that a request of so many tokens may see: their last window + tokens - 1,
@@ -115,7 +119,9 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
                           (units / p.team < p16_resident(head_size) * cus &&
                            64 * 2 * kP16Waves / p.team <= span + 63)))
       p.team /= 2;
-  p.key_tile_log2 = wide ? 6 : 8 - (p.team >> 1);
+  // 64-key tiles of many rows are shared out by what a unit sees (f8_steps), so that a
+  // group left whole has larger ones.
+  p.key_tile_log2 = wide ? (whole ? 7 : 6) : 8 - (p.team >> 1);
   if (whole)
     while ((int64_t{1} << p.key_tile_log2) < span) ++p.key_tile_log2;
   p.slot_rows = static_cast<int32_t>(p.qsl ? bm : std::min<int64_t>(bm, p.group));
@@ -129,15 +135,17 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   const int64_t fill =
       cus * (wide ? p16_resident(head_size) : rows_per_cu(head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
-  if (key_tiles == 1) p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, 8 * cus));
-  p.notes = key_tiles == 1 ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
+  const bool cuts = wide ? !whole : key_tiles > 1;
+  if (!cuts)
+    p.num_wg = static_cast<int32_t>(std::min<int64_t>(groups, (wide ? 64 : 8) * cus));
+  p.notes = !cuts ? -1 : groups <= p.num_wg ? static_cast<int32_t>(groups) : 0;
   hipError_t err = wide ? launch_f8_wide_kernel(p, f16, head_size, stream)
                         : launch_f8_rows_kernel(p, f16, head_size, stream);
   // Work-groups of the join per note (p16_launch.hip has the measurements).
   const int32_t items = p.team * p.slot_rows, least = wide ? 16 : 1;
   const int32_t y =
       p.notes > 0 ? std::min(items, std::max(least, (wide ? 8 : 4) * cus / p.notes)) : least;
-  if (err == hipSuccess && key_tiles > 1)
+  if (err == hipSuccess && cuts)
     err = launch_f8_combine_kernel(p, f16, wide, head_size, y, stream);
   if (err != hipSuccess)
     return fail(PTH_ATTN_ECUDA,

@@ -71,16 +71,27 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  // The work-groups of an XCD (every eighth) take neighbouring shares, so
-  // that the row tiles of one KV head read its keys from one L2.
-  const int per = p.num_wg >> 3;
-  const int wg = per * 8 == p.num_wg
-                     ? static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3)
-                     : static_cast<int>(blockIdx.x);
   P16Cursor cur;
   const int64_t tiles = p16_begin<kBM>(p, cur, lane);
-  if (wg == 0) p16_note_groups<kBM, D>(p, cur, lane);
   const int takers = p16_takers(p, tiles);
+  // The work-groups of an XCD (every eighth) take neighbouring shares, so that the row
+  // tiles of one KV head read its keys from one L2; those without a share are last, in
+  // each XCD alike. Where groups are left whole and the keys' streams (a KV head of a
+  // request) do not divide by the XCDs, these take shares in turn instead.
+  const bool cuts = p.notes >= 0;
+  bool apart = (p.num_wg & 7) == 0;
+  if (!cuts && p.num_reqs <= 64) {
+    const int streams =
+        p.num_kv_heads *
+        __popcll(__ballot(p16_count<kBM>(p, cur.of, lane).groups > 0));
+    apart = apart && ((streams & 7) == 0 || streams >= 32);
+  }
+  int wg = blockIdx.x;
+  if (apart) {
+    const int per = (takers + 7) >> 3, xcd = wg & 7, nth = wg >> 3;
+    wg = nth < per ? xcd * per + nth : wg;
+  }
+  if (wg == 0) p16_note_groups<kBM, D>(p, cur, lane);
   if (wg >= takers) {
     if (threadIdx.x == 0) p16_note_none<D>(p, wg);
     return;
@@ -94,7 +105,17 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
     const bool whole = take == gr.req.n_kt;
     const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
-    const P16Unit u = p16_unit(gr.req, gr.group);
+    P16Unit u = p16_unit(gr.req, gr.group);
+    if (!cuts) {
+      // Left whole, a request's last row tiles go first, so that the long ones of causal
+      // prompts do not end last; in turn, the KV heads of each.
+      if (!apart) {
+        const uint32_t heads = static_cast<uint32_t>(p.num_kv_heads);
+        u.rt = static_cast<int32_t>(static_cast<uint32_t>(gr.group) / heads);
+        u.head = gr.group - u.rt * static_cast<int32_t>(heads);
+      }
+      u.rt = gr.req.n_rt - 1 - u.rt;
+    }
     const int rows = min(kBM, gr.req.rows - u.rt * kBM);
     const int row = 32 * wave + r32;
     const bool live = row < rows;

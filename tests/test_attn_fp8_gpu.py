@@ -132,6 +132,29 @@ def test_long_chunks(D, dtype, q_lens, lens):
     assert torch.equal(out, attend(c, q, q_lens, 1 / math.sqrt(D), max_q=MANY))
 
 
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize(("reqs", "Hkv"), [(3, 3), (2, 4), (33, 1), (70, 2)])
+def test_many_prompts(reqs, Hkv, window):
+    """Units left whole, in the orders of their row tiles and KV heads, requests without
+    tokens among them; more than a wave's lanes of requests."""
+    q_lens = [[0, 40, 300, 17, 129][(3 * i) % 5] if i else 260 for i in range(reqs)]
+    lens = [n + (50 * i) % 350 for i, n in enumerate(q_lens)]
+    c = make_cache(lens, Hkv=Hkv, D=64, block=16, seed=reqs)
+    q = queries(sum(q_lens), 4 * Hkv, 64, BF, reqs)
+    check(c, q, q_lens, 0.125, MANY, window=window)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize(("reqs", "Hkv", "D"), [(1, 1, 128), (12, 2, 64), (180, 8, 256)])
+def test_short_prompts(reqs, Hkv, D, causal):
+    """No request longer than a tile: few that are left whole, many that are not."""
+    q_lens = [17 + i % 9 for i in range(reqs)]
+    lens = [n + (5 * i) % 36 for i, n in enumerate(q_lens)]
+    c = make_cache(lens, Hkv=Hkv, D=D, block=16, seed=reqs)
+    q = queries(sum(q_lens), Hkv, D, BF, reqs)
+    check(c, q, q_lens, 1 / math.sqrt(D), MANY, causal=causal)
+
+
 @pytest.mark.parametrize("kernel", [FEW, MANY])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_peaked_and_wide_scores(kernel, dtype):
