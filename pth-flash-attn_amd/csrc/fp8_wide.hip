@@ -20,6 +20,15 @@
 // A row does not see the keys behind its own, nor the slots behind the request's
 // last key in their block: where one of these has a NaN in V, it is taken out of the
 // products of the tile and put back into the rows that do see it.
+//
+// Bound: the SIMDs' issue. 4 requests of 2,048 rows against 4,096 keys, 32 heads over 8
+// of 128, 533 us, 1,031 TFLOP/s: matrix instructions 47 % of the cycles, vector ones
+// (softmax, conversions) 44 %, and little of the two goes on at once, be it of one wave
+// (a product of 32 cycles with four additions behind it takes 46) or of two. So codes are
+// converted once for four waves, and nothing else is asked of a tile than its softmax
+// needs. Heads of 64 339 us. Heads of 256, 16 over 8, 709 us: registers for one wave of a
+// SIMD alone, and 64 KB written to LDS and 256 KB read for a tile, at some 80 bytes a
+// cycle.
 
 #include "fp8_device.h"
 
@@ -35,8 +44,9 @@ struct WideOf {
   static constexpr int kCodes = D / 16;   // 16-code pieces of a row in the cache
   static constexpr int kBuf = kP16WideKeys * kRow;
   static constexpr int kLoads = D / 64;   // loads of a wave per tile and stream
-  // Whether the next tile is stored between the PV products, or behind them.
-  static constexpr bool kBetween = D != 256;
+  // Whether the next tile's addresses are asked for before the scores (heads of 256, one
+  // wave on a SIMD: 716 and 709 us; heads of 128 533 and 540), or where they are needed.
+  static constexpr bool kEarly = D == 256;
   // The place of 16-byte piece c of row t in LDS. Stores of 8 lanes, every second
   // piece of a row, take all 32 banks, reads (the same piece of 16 rows of K, four
   // of 4 rows of V) all 64.
@@ -189,12 +199,19 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     typedef u32x4 __attribute__((address_space(1))) GlobalPiece;
     u32x4 kc[W::kLoads], vc[W::kLoads];
     uint32_t ke = 0, ve = 0;
+    u32x4 found = {0u, 0u, 0u, 0u};
+    uint32_t found_e = 0;
+    const auto find = [&](int t) {
+      found = s_window[wave].address[t - window];
+      found_e = s_window[wave].e[t - window];
+    };
     const auto load = [&](int t) {
       const int at_lane = t - window;
-      const u32x4 address = s_window[wave].address[at_lane];
+      const u32x4 address = W::kEarly ? found : s_window[wave].address[at_lane];
       const GlobalBytes ks = f8_uniform(address[0], address[1]);
       const GlobalBytes vs = f8_uniform(address[2], address[3]);
-      const uint32_t e = __builtin_amdgcn_readfirstlane(s_window[wave].e[at_lane]);
+      const uint32_t e = __builtin_amdgcn_readfirstlane(W::kEarly ? found_e
+                                                                  : s_window[wave].e[at_lane]);
       ke = e & 0xffu;
       ve = e >> 8;
       const uint32_t k_slot = static_cast<uint32_t>(p.k.s_slot);
@@ -202,8 +219,10 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       const uint32_t ko = __umul24(r0, k_slot) + 16 * c0, vo = __umul24(r0, v_slot) + 16 * c0;
 #pragma unroll
       for (int i = 0; i < W::kLoads; ++i) {
-        kc[i] = *reinterpret_cast<const GlobalPiece*>(ks + static_cast<int64_t>(i * kStep) * k_slot + ko);
-        vc[i] = *reinterpret_cast<const GlobalPiece*>(vs + static_cast<int64_t>(i * kStep) * v_slot + vo);
+        kc[i] = *reinterpret_cast<const GlobalPiece*>(
+            ks + static_cast<int64_t>(i * kStep) * k_slot + ko);
+        vc[i] = *reinterpret_cast<const GlobalPiece*>(
+            vs + static_cast<int64_t>(i * kStep) * v_slot + vo);
       }
     };
     // Part `part` of four of the loaded tile into buffer `buf`. The pieces' places
@@ -249,6 +268,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     lds_barrier();  // the last unit's reads of both buffers are done
     if (t0 < t1) {
       refill(t0);
+      if constexpr (W::kEarly) find(t0);
       load(t0);
     }
     u32x4 q[W::kQ];
@@ -309,6 +329,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       }
       const bool mine = t >= w0 && t < w1;
       if (__builtin_expect(more && t + 1 - window == 64, 0)) refill(t + 1);
+      if (W::kEarly && more) find(t + 1);
       if (more && !mine) {
         load(t + 1);
         store_all(t + 1, buf ^ 1);
@@ -437,15 +458,9 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
             if constexpr (kF16) o[j] = mfma32<false>(vf[i & 1][j], pl[i], o[j]);
           }
           // Behind the last tile, the registers' old codes, which nobody reads.
-          if constexpr (W::kBetween) store(buf ^ 1, i);
+          store(buf ^ 1, i);
         }
-        if (more) {
-          if constexpr (!W::kBetween) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) store(buf ^ 1, i);
-          }
-          tell(t + 1, buf ^ 1);
-        }
+        if (more) tell(t + 1, buf ^ 1);
         __builtin_amdgcn_s_setprio(1);
       }
     }
