@@ -14,12 +14,13 @@
 namespace pa {
 namespace {
 
-// Slots per group up to which a larger team pays, and key rows that a
-// work-group reads for each row of sums in its slots, below which the slots'
-// bytes cost more than a larger team's reads save: as p16_launch.hip has them,
-// where a key row is twice the bytes.
+// Slots per group up to which a larger team pays (p16_launch.hip has the measurements),
+// and key rows that a work-group reads for each row of sums in its slots, below which the
+// slots' bytes cost more than a larger team's reads save. One request, 8 heads of 128,
+// teams of 1, 2, 4: 1,024 keys 10.3, 10.0, 11.0 us; 4,096 12.8, 12.1, 11.9; 131,072 66, 56,
+// 52. 64 requests of 1,024 to 32,768 530, 447, 406.
 constexpr int64_t kMostSlots = 128;
-constexpr int64_t kLeastReads = 16;
+constexpr int64_t kLeastReads = 4;
 
 bool rows_aligned(const void* p, int64_t a, int64_t b) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a % 16 == 0 && b % 16 == 0;
@@ -44,8 +45,11 @@ int32_t team_of(const F8Params& p, int64_t span, int64_t rows, bool whole, int32
   return team;
 }
 
-// The 16-row kernel's work-groups per compute unit where groups are cut.
-int64_t rows_per_cu(int32_t head_size, int64_t groups, int32_t cus) {
+// The 16-row kernel's work-groups per compute unit where groups are cut: one of four
+// units side by side (256 requests to 4,096 keys, 8 heads of 128, one and two 193 and 202
+// us), more of fewer (1,024 requests to 1,000 keys, one head, one, two, three 59, 51, 63).
+int64_t rows_per_cu(const F8Params& p, int32_t head_size, int64_t groups, int32_t cus) {
+  if (p.team == 4) return 1;
   return std::min<int64_t>(p16_resident(head_size), std::max<int64_t>(1, groups / cus));
 }
 
@@ -109,7 +113,8 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   const int64_t span = span_of(p, tokens);
   const int64_t units = row_tiles * p.num_kv_heads;
   if (units == 0) return PTH_ATTN_OK;
-  const bool whole = wide ? whole_wide(head_size, span, units, cus) : whole_rows(head_size, span, units, cus);
+  const bool whole = wide ? whole_wide(head_size, span, units, cus)
+                          : whole_rows(head_size, span, units, cus);
   p.team = wide ? 1 : team_of(p, span, std::min(bm, longest * p.group), whole, cus);
   // Fewer units side by side while compute units lack work-groups, and further only
   // where all of a unit's waves have keys (8 heads of 128, 128 keys, one unit and two: 16
@@ -133,7 +138,7 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   // A causal unit's share is up to five tiles more than its keys (f8_tiles).
   PA_REQUIRE(units < INT32_MAX / (key_tiles + 6), "the launch exceeds 2^31 tiles");
   const int64_t fill =
-      cus * (wide ? p16_resident(head_size) : rows_per_cu(head_size, groups, cus));
+      cus * (wide ? p16_resident(head_size) : rows_per_cu(p, head_size, groups, cus));
   p.num_wg = static_cast<int32_t>(std::min(groups * key_tiles, fill));
   const bool cuts = wide ? !whole : key_tiles > 1;
   if (!cuts)
@@ -242,7 +247,8 @@ int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
   F8Params few = p;
   p.least_rows = kP16RowsRows + 1;
   few.most_rows = kP16RowsRows;
-  const int32_t rc = launch_part(p, c.head_size, a.dtype == PTH_ATTN_F16, true, longest, cus, stream);
+  const int32_t rc =
+      launch_part(p, c.head_size, a.dtype == PTH_ATTN_F16, true, longest, cus, stream);
   if (rc != PTH_ATTN_OK) return rc;
   return launch_part(few, c.head_size, a.dtype == PTH_ATTN_F16, false,
                      std::max<int64_t>(kP16RowsRows / p.group, 1), cus, stream);

@@ -494,7 +494,8 @@ int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
   PA_REQUIRE(cus > 0, "cannot query the compute-unit count of the current device");
   w.tokens = 2;
   w.heads = 1;
-  while (static_cast<int64_t>(a.num_tokens) * c.num_kv_heads > int64_t{4} * cus * w.tokens)
+  while (w.tokens <= 4 &&
+         static_cast<int64_t>(a.num_tokens) * c.num_kv_heads > int64_t{4} * cus * w.tokens)
     w.tokens *= 2;
   const bool many = w.tokens > 4;
   if (many && a.num_tokens < kManyTokens) {

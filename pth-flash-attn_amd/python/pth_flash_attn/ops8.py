@@ -272,8 +272,9 @@ def paged_attn_fp8_fwd(
     calls, and calls that can run at the same time need one each. ``out`` may be
     ``q`` itself; other than that they share no memory.
 
-    At most two launches, whose sizes depend on host integers only, so a captured
-    graph replays as the lengths change. Allocates nothing, reads nothing back,
+    At most four launches (two where the batch is not one of prompts and decodes),
+    whose sizes depend on host integers only, so a captured graph replays as the
+    lengths change. Allocates nothing, reads nothing back,
     is deterministic. Rows of q, out and the cache are 16-byte aligned.
     """
     _op("paged_attn_fp8_fwd")(out, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
