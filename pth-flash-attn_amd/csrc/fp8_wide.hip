@@ -44,6 +44,11 @@ struct WideOf {
   static constexpr int kCodes = D / 16;   // 16-code pieces of a row in the cache
   static constexpr int kBuf = kP16WideKeys * kRow;
   static constexpr int kLoads = D / 64;   // loads of a wave per tile and stream
+  // Units left whole of more keys than 2^(kSort - 1) go by length, others request by
+  // request. Ragged batches gain, even ones of short units lose: 5 prompts of 500 to 2,500
+  // tokens behind 100 to 6,200 keys, 8 heads of 128, 323 and 388 us, 16 of 1,024 232 and 221,
+  // 16 of 256 49 and 39; 4 heads of 256, 4 of 1,024 81 and 104, 16 of 512 113 and 132.
+  static constexpr int kSort = D == 256 ? 9 : 10;
   // Whether the next tile's addresses are asked for before the scores (heads of 256, one
   // wave on a SIMD: 716 and 709 us; heads of 128 533 and 540), or where they are needed.
   static constexpr bool kEarly = D == 256;
@@ -66,6 +71,62 @@ struct WideOf {
   }
 };
 
+// Units that are left whole by the keys that they see, most first, so that all
+// compute units end together: unit `at` of that order, of up to 64 requests (a lane knows
+// its own). A causal request's row tile rt sees prefix + 128 (rt + 1) / G keys or its
+// window, so that it has a count of units with more than x keys in closed form, and a
+// search over x (in steps of 64 keys, at most 128) finds the step that holds the unit.
+// Within a step requests follow each other, and KV heads in turn: eight of them an XCD
+// each, whose L2 has their keys.
+__device__ __forceinline__ P16Group f8_longest(const F8Params& p, const P16Cursor& c, int32_t at,
+                                               int lane, P16Unit& u) {
+  const P16Req x = p16_request_of<kP16WideRows>(p, lane, c.of.q0, c.of.q1, c.of.len);
+  const int n_rt = lane < p.num_reqs ? x.n_rt : 0;
+  const bool grows = p.causal && p.qsl != nullptr;
+  const int per = 128 / p.group + 1;  // tokens of a unit
+  const int cap = p.window > 0 ? p.window + per : INT32_MAX;
+  const int prefix =
+      grows ? x.len - static_cast<int>(p.g_div.div(static_cast<uint32_t>(x.rows))) : x.len;
+  const int most = __builtin_amdgcn_readfirstlane(
+      wave_max32(n_rt > 0 ? min(x.len + per, cap) : 0));
+  int step = 6;
+  while (most >> step >= 128) ++step;
+  const auto more = [&](int i) {  // the lane's row tiles that see more than i << step keys
+    const int64_t keys = static_cast<int64_t>(i) << step;
+    const int64_t rest = keys - prefix;
+    const int seen = static_cast<int>(
+        min(max(grows ? rest * p.group >> 7 : (rest < 0 ? 0 : int64_t{n_rt}), int64_t{0}),
+            static_cast<int64_t>(n_rt)));
+    return i < 0 ? n_rt : keys >= cap ? 0 : n_rt - seen;
+  };
+  const auto all = [&](int n) {
+    return __builtin_amdgcn_readlane(wave_scan32(n), 63) * p.num_kv_heads;
+  };
+  int lo = -1, hi = (most >> step) + 1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (all(more(mid)) > at) lo = mid;
+    else hi = mid;
+  }
+  const int above = more(hi), here = more(lo) - above;
+  const int32_t nth = at - all(above);
+  const int incl = wave_scan32(here) * p.num_kv_heads;
+  const int j = __builtin_amdgcn_readfirstlane(
+      min(static_cast<int>(__popcll(__ballot(incl <= nth))), 63));
+  const int in = nth - (j > 0 ? __builtin_amdgcn_readlane(incl, j - 1) : 0);
+  P16Group gr;
+  gr.r = __builtin_amdgcn_readfirstlane(min(j, p.num_reqs - 1));
+  gr.req = p16_request_of<kP16WideRows>(p, gr.r, __builtin_amdgcn_readlane(c.of.q0, j),
+                                        __builtin_amdgcn_readlane(c.of.q1, j),
+                                        __builtin_amdgcn_readlane(c.of.len, j));
+  gr.group = gr.kt = gr.number = 0;
+  const int before = __builtin_amdgcn_readlane(above, j);
+  const int k = static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(p.num_kv_heads));
+  u.head = __builtin_amdgcn_readfirstlane(in - k * p.num_kv_heads);
+  u.rt = __builtin_amdgcn_readfirstlane(max(gr.req.n_rt - 1 - before - k, 0));
+  return gr;
+}
+
 template <int D, bool kF16>
 __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     const F8Params p) {
@@ -84,20 +145,12 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
   P16Cursor cur;
   const int64_t tiles = p16_begin<kBM>(p, cur, lane);
   const int takers = p16_takers(p, tiles);
-  // The work-groups of an XCD (every eighth) take neighbouring shares, so that the row
-  // tiles of one KV head read its keys from one L2; those without a share are last, in
-  // each XCD alike. Where groups are left whole and the keys' streams (a KV head of a
-  // request) do not divide by the XCDs, these take shares in turn instead.
+  // Where groups are cut, the work-groups of an XCD (every eighth) take neighbouring
+  // shares, so that the row tiles of one KV head read its keys from one L2; those without
+  // a share are last, in each XCD alike.
   const bool cuts = p.notes >= 0;
-  bool apart = (p.num_wg & 7) == 0;
-  if (!cuts && p.num_reqs <= 64) {
-    const int streams =
-        p.num_kv_heads *
-        __popcll(__ballot(p16_count<kBM>(p, cur.of, lane).groups > 0));
-    apart = apart && ((streams & 7) == 0 || streams >= 32);
-  }
   int wg = blockIdx.x;
-  if (apart) {
+  if (cuts && (p.num_wg & 7) == 0) {
     const int per = (takers + 7) >> 3, xcd = wg & 7, nth = wg >> 3;
     wg = nth < per ? xcd * per + nth : wg;
   }
@@ -111,21 +164,23 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
   bool noted = false;
 
   while (at < end) {
-    const P16Group gr = p16_locate<kBM>(p, cur, at, lane);
-    const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
-    const bool whole = take == gr.req.n_kt;
-    const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
-    P16Unit u = p16_unit(gr.req, gr.group);
-    if (!cuts) {
-      // Left whole, a request's last row tiles go first, so that the long ones of causal
-      // prompts do not end last; in turn, the KV heads of each.
-      if (!apart) {
+    P16Unit u;
+    P16Group gr;
+    if (cuts || p.num_reqs > 64 || p.key_tile_log2 < W::kSort) {
+      gr = p16_locate<kBM>(p, cur, at, lane);
+      u = p16_unit(gr.req, gr.group);
+      if (!cuts) {  // a request's last row tiles first, in turn the KV heads of each
         const uint32_t heads = static_cast<uint32_t>(p.num_kv_heads);
         u.rt = static_cast<int32_t>(static_cast<uint32_t>(gr.group) / heads);
         u.head = gr.group - u.rt * static_cast<int32_t>(heads);
+        u.rt = gr.req.n_rt - 1 - u.rt;
       }
-      u.rt = gr.req.n_rt - 1 - u.rt;
+    } else {
+      gr = f8_longest(p, cur, static_cast<int32_t>(at), lane, u);
     }
+    const int take = static_cast<int>(min(static_cast<int64_t>(gr.req.n_kt - gr.kt), end - at));
+    const bool whole = take == gr.req.n_kt;
+    const int slot = 2 * wg + (gr.kt == 0 ? 1 : 0);
     const int rows = min(kBM, gr.req.rows - u.rt * kBM);
     const int row = 32 * wave + r32;
     const bool live = row < rows;
