@@ -87,10 +87,10 @@ int64_t span_of(const F8Params& p, int64_t tokens) {
 // decodes, so that requests of few rows get their own launch: eight of them, if the
 // others are as long as the longest, and work enough for what that launch costs. Whole
 // calls of decodes with prompts, 32 / 8 heads of 128, one launch and two: 60 of 2,000
-// keys with 2 x 512 tokens 119.8 and 91.2 us, 120 with 1 x 512 176 and 134, 200 of 1,000
-// with 2 x 32 142 and 120; 8 of 2,000 with 1 x 512 53 and 66, 20 of 1,000 with 4 x 8 28
-// and 48, 14 of 500 with 2 x 17 20 and 32.
-constexpr int64_t kMixedBytes = int64_t{5} << 24;  // of K, at the longest length
+// keys (123 MB) with 2 x 512 tokens 68 and 72 us, 90 122 and 94, 120 with 1 x 512 132 and
+// 114, 200 of 1,000 with 2 x 32 140 and 116; 8 of 2,000 (21 MB) with 1 x 512 53 and 65, 20 of
+// 1,000 with 4 x 8 29 and 46.
+constexpr int64_t kMixedBytes = int64_t{1} << 27;  // of K, at the longest length
 bool mixed(const F8Params& p, int32_t head_size, int64_t longest) {
   const int64_t few = p.num_reqs - (p.num_tokens + longest - 1) / longest;
   return p.group <= kP16RowsRows && few >= 8 &&
