@@ -101,13 +101,6 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   return static_cast<uint32_t>(w);
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-#pragma unroll
-  for (int i = 32; i > 0; i >>= 1)
-    x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), i)));
-  return x;
-}
-
 template <int D, class T, bool kWide, int kThreads>
 __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kPasses = kF8Span / kRows;
@@ -233,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
         const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
         top = max(top, b < 0x7f800000u ? b : 0u);
       }
-    top = wave_max(top);
+    top = static_cast<uint32_t>(wave_max32(static_cast<int32_t>(top)));
     const uint32_t old = begun ? 0u : min(had, static_cast<uint32_t>(kF8MostExp));
     const uint32_t e = max(old, exponent_for(top));
     const float unit = e ? __builtin_bit_cast(float, (254u - e) << 23) : 0.0f;
