@@ -144,6 +144,18 @@ def test_many_prompts(reqs, Hkv, window):
     check(c, q, q_lens, 0.125, MANY, window=window)
 
 
+@pytest.mark.parametrize(("causal", "window"), [(True, 0), (True, 600), (False, 0)])
+@pytest.mark.parametrize(("D", "Hq", "Hkv"), [(64, 15, 3), (128, 8, 8), (256, 8, 2)])
+def test_ragged_prompts(D, Hq, Hkv, causal, window):
+    """Units that go by the keys that they see: prompts alone and behind long prefixes,
+    tokens before the first key, lengths that tie."""
+    q_lens = [200, 33, 900, 17, 450, 0, 60]
+    lens = [3000, 33, 900, 2500, 2733, 5000, 20]
+    c = make_cache(lens, Hkv=Hkv, D=D, block=16, seed=D)
+    q = queries(sum(q_lens), Hq, D, BF, D)
+    check(c, q, q_lens, 1 / math.sqrt(D), MANY, causal=causal, window=window)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize(("reqs", "Hkv", "D"), [(1, 1, 128), (12, 2, 64), (180, 8, 256)])
 def test_short_prompts(reqs, Hkv, D, causal):
