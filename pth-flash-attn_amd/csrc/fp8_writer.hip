@@ -14,8 +14,8 @@
 // scale grows.
 //
 // Bound: its bytes, behind the reading of slot_mapping (8 heads of 128, bf16, cold:
-// 16,384 tokens, 101 MB, 26.8 us, of which that takes some 4); latency for a decode
-// step, whose tokens lie in blocks of their own (64 tokens 5.3 us).
+// 16,384 tokens, 101 MB, 23.0 us); latency for a decode step, whose tokens lie in blocks
+// of their own (64 tokens 4.8 us).
 //
 // The reader. A work-group finds the pages of up to 16 rows in LDS, then each thread
 // reads four pieces of codes at once and writes each as 16 bytes, a wave of them a
@@ -30,6 +30,7 @@
 #include <algorithm>
 #include <climits>
 #include <string>
+#include <type_traits>
 
 #include "fp8_device.h"
 
@@ -42,18 +43,17 @@ constexpr int kWriteTokens = 128;         // of a work-group, at most
 constexpr int kTable = 2 * kWriteTokens;  // entries, a power of two
 static_assert(kTable <= kThreads, "a thread looks at an entry");
 // A work-group has 256 threads, one head and 2 or 4 tokens where that makes no more than
-// four work-groups for a compute unit; otherwise kManyThreads threads, and 16 tokens of a
-// head or, from so many tokens on, 8 to kWriteTokens of all heads, so that few read
-// slot_mapping (8 heads of 128, from cold memory: 16,384 tokens in runs 26.8 us, 100 with
-// 256 threads and 16 tokens; 1,024 tokens in blocks of their own 14.0, and 28.0 with 8
-// tokens of all heads, in runs 6.7 and 7.3; 64 in blocks of their own 5.3, 20 with 16
-// tokens and 256 threads).
-constexpr int kManyTokens = 2048;
-// A filter of blocks, bits: without it 16,384 tokens take 28.7 us.
+// four work-groups for a compute unit; otherwise kManyThreads threads, one work-group for
+// each compute unit at a time (its registers are half of the unit's or more), of 16 tokens
+// and some heads or, from kManyTokens tokens on, of up to kWriteTokens tokens and all heads,
+// so that few read slot_mapping. 8 heads of 128, bf16, cold: 2,048 tokens 6.2 us against 7.1
+// with all heads, 4,096 tokens 9.2 against 9.0.
+constexpr int kManyTokens = 4096;
+// A filter of blocks, bits: without it 16,384 tokens take 25.7 us, with it 23.1.
 constexpr int kFilter = 16384;
-// Of slot_mapping that a thread asks for at once (4, 8, 16: 16,384 tokens 27.3, 27.3,
-// 28.1 us, 64 tokens 4.9, 5.0, 5.4).
-constexpr int kSlotsAhead = 4;
+// Of slot_mapping that a thread asks for at once (1, 2, 4, 8: 16,384 tokens 24.4, 23.0,
+// 23.1, 23.4 us, 64 tokens 4.7, 4.8, 5.0, 5.3).
+constexpr int kSlotsAhead = 2;
 
 struct WriteF8Params {
   const char* src[2];  // keys, values
@@ -69,21 +69,33 @@ struct WriteF8Params {
   int32_t tokens, heads;  // of a work-group
 };
 
-// Eight values of a source row as 32-bit ones. kWide: on a 16-byte address.
-template <class T, bool kWide>
-__device__ __forceinline__ void load_eight(const char* src, float (&x)[8]) {
-  T y[8];
-  if constexpr (kWide) {
-    u32x4 w[sizeof(T) / 2];
-#pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const u32x4*>(src)[i];
-    __builtin_memcpy(y, w, sizeof(y));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = reinterpret_cast<const T*>(src)[i];
+// Eight values of a source row. kWide: on a 16-byte address.
+template <class T>
+struct Eight {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ float operator[](int i) const {
+    T x[8];
+    __builtin_memcpy(x, w, sizeof(x));
+    return static_cast<float>(x[i]);
   }
+};
+template <class T, bool kWide>
+__device__ __forceinline__ Eight<T> load_eight(const char* src) {
+  Eight<T> y;
+  if constexpr (kWide) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(y[i]);
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i) {
+      const u32x4 v = reinterpret_cast<const u32x4*>(src)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y.w[4 * i + j] = v[j];
+    }
+  } else {
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = reinterpret_cast<const T*>(src)[i];
+    __builtin_memcpy(y.w, x, sizeof(x));
+  }
+  return y;
 }
 
 // The smallest exponent whose scale brings the value with these bits (not
@@ -93,6 +105,9 @@ __device__ __forceinline__ uint32_t exponent_for(uint32_t bits) {
   const int e = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
   return static_cast<uint32_t>(min(max(e, 1), kF8MostExp));
 }
+
+// 448 x 2^119, the largest value that the largest scale's codes reach.
+constexpr uint32_t kMostBits = 0x7f600000u;
 
 // Four 32-bit values, within the codes' range or NaN, as codes.
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
@@ -105,6 +120,10 @@ template <int D, class T, bool kWide, int kThreads>
 __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
   constexpr int kLanes = D / 8, kRows = 64 / kLanes, kPasses = kF8Span / kRows;
   constexpr int kWaves = kThreads / 64;
+  // Whether values that are all finite and small enough have a way of their own (16,384
+  // tokens, 8 heads of 128, bf16: 23.1 us, 26.5 without it and with loads in branches): not
+  // where a row's registers would go to scratch (4 heads of 256, fp32: 70.8 us, 35.6).
+  constexpr bool kTwo = D * sizeof(T) < 1024;
   __shared__ int32_t s_block[kTable], s_first[kTable], s_row[kTable * kF8Span];
   __shared__ int32_t s_list[kTable];
   __shared__ uint32_t s_maybe[kFilter / 32];
@@ -198,64 +217,95 @@ __global__ __launch_bounds__(kThreads) void write_kv_f8(const WriteF8Params p) {
     uint8_t* exponent = p.scale[kv] + static_cast<int64_t>(block) * p.num_kv_heads + head;
     const uint32_t had = *exponent;
     const CacheStream& s = p.cache[kv];
+    // The block, and the lane's place in it.
     char* cell = const_cast<char*>(s.base) + static_cast<int64_t>(page) * s.s_block +
-                 static_cast<int64_t>(kF8Span * sub + r) * s.s_slot +
-                 static_cast<int64_t>(head) * s.s_head + 8 * c;
-    const bool begun = s_row[kF8Span * entry] >= 0;
-    int32_t token[kPasses];
-    float x[kPasses][8];
+                 static_cast<int64_t>(kF8Span * sub) * s.s_slot +
+                 static_cast<int64_t>(head) * s.s_head;
+    const uint32_t in_cell = __umul24(r, static_cast<uint32_t>(s.s_slot)) + 8 * c;
+    const int32_t* rows = s_row + kF8Span * entry;
+    const bool begun = rows[0] >= 0;
+    Eight<T> x[kPasses];
     u32x2 held[kPasses];  // what the block's other rows hold, in case its scale grows
-    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      token[i] = s_row[kF8Span * entry + kRows * i + r];
+      const int32_t token = rows[kRows * i + r];
+      const auto load = [&](int32_t t) {
+        return load_eight<T, kWide>(p.src[kv] + static_cast<int64_t>(t) * p.s_tok[kv] +
+                                    static_cast<int64_t>(head) * p.s_head[kv] + 8 * sizeof(T) * c);
+      };
+      if constexpr (kTwo) {
+        // Where there is none, the first token's row is read, and not used: without a
+        // branch the values stay as they are, in half of the registers.
+        x[i] = load(max(token, 0));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-      held[i] = (u32x2){0u, 0u};
-      if (token[i] >= 0)
-        load_eight<T, kWide>(p.src[kv] + static_cast<int64_t>(token[i]) * p.s_tok[kv] +
-                                 static_cast<int64_t>(head) * p.s_head[kv] + 8 * sizeof(T) * c,
-                             x[i]);
-      else if (!begun)
-        held[i] = *reinterpret_cast<const u32x2*>(cell + static_cast<int64_t>(kRows * i) * s.s_slot);
-    }
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
-        top = max(top, b < 0x7f800000u ? b : 0u);
+        for (unsigned j = 0; j < 2 * sizeof(T); ++j)
+          x[i].w[j] &= static_cast<uint32_t>(~(token >> 31));
+      } else {
+        x[i] = Eight<T>{};
+        if (token >= 0) x[i] = load(token);
       }
-    top = static_cast<uint32_t>(wave_max32(static_cast<int32_t>(top)));
+      held[i] = (u32x2){0u, 0u};
+      if (token < 0 && !begun)
+        held[i] = *reinterpret_cast<const u32x2*>(
+            cell + static_cast<int64_t>(kRows * i) * s.s_slot + in_cell);
+    }
+    // Of all values, and where one is not finite or beyond the largest scale's codes, of
+    // the finite ones again.
+    const auto largest = [&](auto any) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
+          most = max(most, decltype(any)::value || b < 0x7f800000u ? b : 0u);
+        }
+      return static_cast<uint32_t>(
+          __builtin_amdgcn_readfirstlane(wave_max32(static_cast<int32_t>(most))));
+    };
+    uint32_t top = largest(std::bool_constant<kTwo>{});
+    const bool plain = kTwo && top <= kMostBits;
+    if (kTwo && !plain) top = largest(std::false_type{});
     const uint32_t old = begun ? 0u : min(had, static_cast<uint32_t>(kF8MostExp));
     const uint32_t e = max(old, exponent_for(top));
     const float unit = e ? __builtin_bit_cast(float, (254u - e) << 23) : 0.0f;
     const bool grown = !begun && e > old;
     const float move =
         old && old + 127 > e ? __builtin_bit_cast(float, (old + 127u - e) << 23) : 0.0f;
+    // (Choosing between two values, as below, takes 96 registers in fp32 of 256, an if 158.)
+    const auto put = [&](auto fine) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      u32x2* dst = reinterpret_cast<u32x2*>(cell + static_cast<int64_t>(kRows * i) * s.s_slot);
-      if (token[i] >= 0) {
+      for (int i = 0; i < kPasses; ++i) {
+        u32x2* dst = reinterpret_cast<u32x2*>(
+            cell + static_cast<int64_t>(kRows * i) * s.s_slot + in_cell);
+        if (rows[kRows * i + r] >= 0) {
+          float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t b = __builtin_bit_cast(uint32_t, x[i][j]) & 0x7fffffffu;
-          const float y = fminf(fmaxf(x[i][j] * unit, -448.0f), 448.0f);
-          x[i][j] = b < 0x7f800000u ? y : __builtin_nanf("");
+          for (int j = 0; j < 8; ++j) {
+            const float v = x[i][j];
+            if constexpr (decltype(fine)::value) {
+              y[j] = v * unit;
+            } else {
+              const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+              const float z = fminf(fmaxf(v * unit, -448.0f), 448.0f);
+              y[j] = b < 0x7f800000u ? z : __builtin_nanf("");
+            }
+          }
+          *dst = (u32x2){codes4(y[0], y[1], y[2], y[3]), codes4(y[4], y[5], y[6], y[7])};
+        } else if (grown) {
+          u32x2 y;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], false);
+            const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], true);
+            y[j] = codes4(a[0] * move, a[1] * move, b[0] * move, b[1] * move);
+          }
+          *dst = y;
         }
-        *dst = (u32x2){codes4(x[i][0], x[i][1], x[i][2], x[i][3]),
-                       codes4(x[i][4], x[i][5], x[i][6], x[i][7])};
-      } else if (grown) {
-        u32x2 y;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], false);
-          const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(held[i][j], true);
-          y[j] = codes4(a[0] * move, a[1] * move, b[0] * move, b[1] * move);
-        }
-        *dst = y;
       }
-    }
+    };
+    if (plain) put(std::bool_constant<kTwo>{});
+    else put(std::false_type{});
     if (lane == 0 && e != had) *exponent = static_cast<uint8_t>(e);
   }
 }
@@ -493,10 +543,12 @@ int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
   const bool many = w.tokens > 4;
   if (many && a.num_tokens < kManyTokens) {
     w.tokens = 16;
+    const int64_t units = static_cast<int64_t>((a.num_tokens + 15) / 16) * c.num_kv_heads;
+    w.heads = static_cast<int32_t>((units + cus - 1) / cus);
   } else if (many) {
+    const int64_t rounds = (int64_t{a.num_tokens} + kWriteTokens * cus - 1) / (kWriteTokens * cus);
     w.heads = c.num_kv_heads;
-    w.tokens = 8;
-    while (w.tokens < kWriteTokens && a.num_tokens >= 2 * cus * w.tokens) w.tokens *= 2;
+    w.tokens = static_cast<int32_t>((a.num_tokens + rounds * cus - 1) / (rounds * cus));
   }
   const bool wide = on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
                     on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head, c.num_kv_heads);
