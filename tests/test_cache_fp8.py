@@ -103,6 +103,21 @@ def test_write_many(D, dtype, odd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("T", [40, 1500, 4095, 4096])
+def test_first_row_not_finite(D, dtype, T):
+    """The first token's row is infinite and NaN: blocks with fewer tokens than slots keep
+    it out, and their other values are of the largest finite size here and there."""
+    key, value = source(T, 3, D, dtype, D + T)
+    key[0], value[0] = math.nan, -math.inf
+    big = torch.finfo(dtype).max
+    key[5::97, 1, 3], value[7::101, 2, 1] = big, -big
+    slots = torch.arange(T, device="cuda") * 5 // 2 + 3  # six or seven of a block's slots
+    check_write(key, value, filled(T * 5 // 32 + 2, 16, 3, D, "NHD", T), slots)
+
+
+@pytest.mark.gpu
 def test_write_longest_runs():
     """The most tokens of a work-group, each in a block of its own."""
     T = 34000
