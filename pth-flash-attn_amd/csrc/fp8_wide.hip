@@ -236,13 +236,13 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
       for (int i = 0; i < 16; ++i) o[j][i] = 0.0f;
 
     const int32_t* table = p.block_table + static_cast<int64_t>(gr.r) * p.bt_stride;
-    // The block of 16 keys that the wave brings of tile t: itself, or the last
-    // one. Entry i of the wave's window is that of tile window + i.
-    const auto block = [&](int t) { return min(base + kKT * t + 16 * wave, (len - 1) & ~15); };
+    // Entry i of the wave's window: the block of 16 keys that it brings of tile
+    // window + i.
     int window = t0;
     const auto refill = [&](int t) {
       window = t;
-      const F8Block b = f8_block(p, table, u.head, block(t + lane));
+      const F8Block b =
+          f8_block(p, table, u.head, f8_tile_block(base, t + lane, t1 - 1, wave, len));
       s_window[wave].address[lane] =
           (u32x4){static_cast<uint32_t>(b.k), static_cast<uint32_t>(b.k >> 32),
                   static_cast<uint32_t>(b.v), static_cast<uint32_t>(b.v >> 32)};

@@ -25,6 +25,7 @@
 #pragma once
 
 #include "attn_stream.h"
+#include "fp8_geometry.h"
 #include "p16_geometry.h"
 
 namespace pa {
