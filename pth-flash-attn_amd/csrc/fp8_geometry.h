@@ -20,4 +20,49 @@ PA_HD int32_t f8_tile_block(int32_t base, int32_t t, int32_t last, int32_t wave,
   return at < end ? at : end;
 }
 
+// Causal 128-row units see a different number of key tiles each: in tokens, unit
+// u's last row sees c + (128 u + 127) / G + 1 keys at most, c being the request's
+// keys before its tokens. Its share of the stream is an upper bound of that
+// whose sums over the units before m have a closed form,
+//   F(m) = floor((m G (c + 128) + 64 m (m + 1)) / 64 G),
+// within two tiles of the unit's need: F's steps are at least what the sum under
+// the floor grows by, less 1, and that leaves the need and the 63 / 64 that it is
+// rounded up by. Where a bound C of what any unit sees is less for the units from
+// some one on, these have C each: of a window, what it and a unit's tokens cover; of
+// tokens without a place among the keys (more tokens than keys), all tiles, beyond
+// which F would grow with the square of the tokens. So a request's units have at most
+// six tiles each more than its keys.
+struct F8Steps {
+  int32_t units;   // row tiles
+  int32_t linear;  // of these, the first ones that F holds for
+  int32_t cap;     // of each behind them
+  int32_t before;  // c; -1: `cap` tiles each
+};
+PA_HD F8Steps f8_causal_steps(int32_t tokens, int32_t len, int32_t n_rt, int32_t n_kt,
+                              int32_t group, int32_t window) {
+  const int32_t c = len > tokens ? len - tokens : 0;
+  F8Steps s = {n_rt, n_rt, n_kt, c};
+  if (window > 0) {
+    const int32_t per = 128 / group + 2;  // tokens of a unit
+    s.cap = ((window + per + 63) >> 6) + 2;
+    if (len < tokens && n_kt < s.cap) s.cap = n_kt;
+  }
+  if (window > 0 || len < tokens) {
+    const int64_t from = (64 * static_cast<int64_t>(s.cap) - c - 128) * group >> 7;
+    s.linear = from < 0 ? 0 : from < n_rt ? static_cast<int32_t>(from) : n_rt;
+  }
+  return s;
+}
+// Tiles of a head's units before m.
+PA_HD int32_t f8_tiles_before(const F8Steps& s, int32_t m, int32_t group, const Div32& g_div) {
+  if (s.before < 0) return m * s.cap;
+  const int64_t l = m < s.linear ? m : s.linear;
+  const uint64_t sum =
+      static_cast<uint64_t>(l * (static_cast<int64_t>(group) * (s.before + int64_t{128})) +
+                            64 * l * (l + 1)) >> 6;
+  const uint32_t f = sum >> 31 == 0 ? g_div.div(static_cast<uint32_t>(sum))
+                                    : static_cast<uint32_t>(sum / static_cast<uint32_t>(group));
+  return static_cast<int32_t>(f) + (m > s.linear ? m - s.linear : 0) * s.cap;
+}
+
 }  // namespace pa

@@ -136,7 +136,7 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   const int64_t groups =
       p.qsl == nullptr ? reqs * ((row_tiles / reqs * p.num_kv_heads + p.team - 1) / p.team)
                        : units / p.team + (p.team > 1 ? reqs : 0);
-  // A causal unit's share is up to five tiles more than its keys (f8_tiles).
+  // The shares of causal units are up to six tiles each more than their keys (F8Steps).
   PA_REQUIRE(units < INT32_MAX / (key_tiles + 6), "the launch exceeds 2^31 tiles");
   const int64_t fill =
       cus * (wide ? p16_resident(head_size) : rows_per_cu(p, head_size, groups, cus));

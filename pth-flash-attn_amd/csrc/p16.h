@@ -122,45 +122,14 @@ __device__ __forceinline__ P16Req p16_request_of(const P& p, int r, int q0, int 
   return x;
 }
 
-// Causal 128-row units see a different number of key tiles each: in tokens, unit
-// u's last row sees c + (128 u + 127) / G + 1 keys at most, c being the request's
-// keys before its tokens. Its share of the stream is an upper bound of that
-// whose sums over the units before m have a closed form,
-//   F(m) = floor((m G (c + 128) + 64 m (m + 1)) / 64 G),
-// within two tiles of the unit's need: F's steps are at least what the sum under
-// the floor grows by, less 1, and that leaves the need and the 63 / 64 that it is
-// rounded up by. With a window, units from the first that a bound C of what a
-// window and a unit's tokens cover is no more for have C each.
-struct F8Steps {
-  int32_t units;   // row tiles
-  int32_t linear;  // of these, the first ones that F holds for
-  int32_t cap;     // of each behind them
-  int32_t before;  // c; -1: `cap` tiles each
-};
+// The shares of a request's 128-row units in the stream (fp8_geometry.h).
 __device__ __forceinline__ F8Steps f8_steps(const F8Params& p, const P16Req& x) {
-  F8Steps s = {x.n_rt, 0, x.n_kt, -1};
-  if (!p.causal || p.qsl == nullptr || p.key_tile_log2 != 6) return s;
+  if (!p.causal || p.qsl == nullptr || p.key_tile_log2 != 6) return {x.n_rt, 0, x.n_kt, -1};
   const int n = static_cast<int>(p.g_div.div(static_cast<uint32_t>(x.rows)));
-  s.before = max(x.len - n, 0);
-  s.linear = x.n_rt;
-  if (p.window > 0) {
-    const int per = 128 / p.group + 2;  // tokens of a unit
-    s.cap = ((p.window + per + 63) >> 6) + 2;
-    const int64_t from =
-        (static_cast<int64_t>(64 * static_cast<int64_t>(s.cap) - s.before - 128) * p.group) >> 7;
-    s.linear = static_cast<int32_t>(min(max(from, int64_t{0}), static_cast<int64_t>(x.n_rt)));
-  }
-  return s;
+  return f8_causal_steps(n, x.len, x.n_rt, x.n_kt, p.group, p.window);
 }
-// Tiles of a head's units before m.
 __device__ __forceinline__ int32_t f8_tiles(const F8Params& p, const F8Steps& s, int32_t m) {
-  if (s.before < 0) return m * s.cap;
-  const int64_t l = min(m, s.linear);
-  const uint64_t sum = static_cast<uint64_t>(l * (static_cast<int64_t>(p.group) * (s.before + 128)) +
-                                             64 * l * (l + 1)) >> 6;
-  const uint32_t f = sum >> 31 == 0 ? p.g_div.div(static_cast<uint32_t>(sum))
-                                    : static_cast<uint32_t>(sum / static_cast<uint32_t>(p.group));
-  return static_cast<int32_t>(f) + max(m - s.linear, 0) * s.cap;
+  return f8_tiles_before(s, m, p.group, p.g_div);
 }
 
 // Length and first and last query token of request `r` (r differs from lane to
