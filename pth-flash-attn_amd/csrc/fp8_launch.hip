@@ -63,18 +63,6 @@ bool whole_rows(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   if (head_size == 256) return span <= 256;
   return span <= (head_size == 64 && units <= cus / 2 ? 1024 : 512);
 }
-// Prompts, where the units are as many as the longest has a share in the whole: whole
-// ones end unevenly, cut ones write and read their sums. 8 heads of 128, whole and cut: 1
-// prompt of 2,048 tokens 63 and 74 us, of 8,192 549 and 611; 4 of 2,048 175 and 216; 4 of
-// 1,900 behind 5,900 keys 855 and 905; 12 of 100 to 2,000 behind up to 7,000 642 and 723; one
-// head, 1 of 2,048 54 and 40, 1 of 8,192 208 and 191. Heads of 256, 4 of them: 1 of 1,024 58
-// and 52, of 4,096 208 and 280; 5 of 500 to 2,500 behind 100 to 6,200 440 and 542.
-// Many short units are better walked by work-groups that stay: 64 of 256 140 and 122.
-bool whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
-  if (units > 5 * p16_resident(head_size) * cus && span < 1024) return false;
-  if (head_size == 256) return span <= 512 || (units >= cus && span * cus <= 2560 * units);
-  return span <= 1024 || span * cus <= 1280 * units;
-}
 
 // The keys that a request of so many tokens may see: their last window + tokens - 1,
 // from a block's beginning on.
@@ -114,7 +102,7 @@ int32_t launch_part(F8Params p, int32_t head_size, bool f16, bool wide, int64_t 
   const int64_t span = span_of(p, tokens);
   const int64_t units = row_tiles * p.num_kv_heads;
   if (units == 0) return PTH_ATTN_OK;
-  const bool whole = wide ? whole_wide(head_size, span, units, cus)
+  const bool whole = wide ? f8_whole_wide(head_size, span, units, cus)
                           : whole_rows(head_size, span, units, cus);
   p.team = wide ? 1 : team_of(p, span, std::min(bm, longest * p.group), whole, cus);
   // Fewer units side by side while compute units lack work-groups, and further only

@@ -120,9 +120,28 @@ static void unit_shares() {
   std::printf("unit shares ok\n");
 }
 
+// A request's keys and a tile of a whole unit, the next power of two, stay below 2^31
+// together, whatever the units.
+static void whole_units() {
+  for (int32_t d : {64, 128, 256})
+    for (int32_t cus : {1, 256})
+      for (int64_t span : {int64_t{1}, int64_t{1024}, int64_t{5000}, (int64_t{1} << 30) - 1,
+                           int64_t{1} << 30, (int64_t{1} << 30) + 1, kMostKeys})
+        for (int64_t units : {int64_t{1}, int64_t{256}, int64_t{1} << 20, int64_t{1} << 28}) {
+          if (!f8_whole_wide(d, span, units, cus)) continue;
+          int64_t tile = 1;
+          while (tile < span) tile *= 2;
+          CHECK(span + tile - 1 <= INT32_MAX, "units of %lld keys whole", (long long)span);
+        }
+  CHECK(f8_whole_wide(128, 8192, 2048, 256) && !f8_whole_wide(128, 8192, 64, 256),
+        "one prompt of 8,192 tokens, eight heads and one");
+  std::printf("whole units ok\n");
+}
+
 int main() {
   tile_blocks();
   unit_shares();
+  whole_units();
   std::printf("ALL OK\n");
   return 0;
 }
