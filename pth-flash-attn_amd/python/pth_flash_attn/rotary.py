@@ -105,5 +105,8 @@ def rotary_turns(rot_dim: int, *, scaling: str = "none", factor: float = 1.0,
         if scaling == "ramp" and factor > 1:
             attention_scale = 0.1 * math.log(factor) + 1.0
         elif scaling == "factors" and factor > 1:
+            if original_max_position == 1:
+                raise ValueError("scaling 'factors' needs original_max_position above 1 or an "
+                                 "attention_scale")
             attention_scale = math.sqrt(1.0 + math.log(factor) / math.log(original_max_position))
     return torch.tensor(signed, dtype=torch.int64).to(device), float(attention_scale)
