@@ -95,10 +95,13 @@ def rotary_turns(rot_dim: int, *, scaling: str = "none", factor: float = 1.0,
     for ``factors`` (where ``factor``, the context's extension, is above 1), 1
     otherwise. The keywords are those of ``rotary_frequencies``.
     """
-    f = rotary_frequencies(rot_dim, scaling=scaling, factor=factor,
-                           original_max_position=original_max_position, **kw)
-    # A float times 2^64 is a whole number or rounds to one of 64 bits.
-    turns = [round(math.ldexp(x / (2 * math.pi), 64)) % (1 << 64) for x in f]
+    try:
+        f = rotary_frequencies(rot_dim, scaling=scaling, factor=factor,
+                               original_max_position=original_max_position, **kw)
+        # A float times 2^64 is a whole number or rounds to one of 64 bits.
+        turns = [round(math.ldexp(x / (2 * math.pi), 64)) % (1 << 64) for x in f]
+    except OverflowError:
+        raise ValueError("the frequencies must be finite, and 2^64 times them") from None
     signed = [t - (1 << 64) if t >= 1 << 63 else t for t in turns]
     if attention_scale is None:
         attention_scale = 1.0

@@ -15,3 +15,12 @@ def test_factors_within_one_position():
         rotary.rotary_turns(8, **kw)
     assert rotary.rotary_turns(8, **kw, attention_scale=1.5)[1] == 1.5
     assert rotary.rotary_turns(8, **{**kw, "factor": 1.0})[1] == 1.0
+
+
+@pytest.mark.parametrize("kw", [
+    {"scaling": "linear", "factor": 1e-300}, {"base": 1e-300, "scaling": "none"},
+    {"scaling": "base", "factor": 1e300, "base": 1e300},
+    {"scaling": "factors", "factors": [1e-300] * 32}])
+def test_frequencies_beyond_a_double(kw):
+    with pytest.raises(ValueError, match="finite"):
+        rotary.rotary_turns(64, device="cpu", **kw)
