@@ -22,6 +22,7 @@ constexpr int kF8Span = 16;     // slots of a scale
 constexpr int kF8MostExp = 246; // of a scale: 448 x 2^119 is the largest value
 
 // Host side.
+constexpr int64_t kMostThreads = 0xffffffff;  // of a launch
 int32_t launch_rotary(const PthAttnRotaryArgs& a, hipStream_t stream);
 int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream);
 int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream);

@@ -552,7 +552,10 @@ int32_t launch_write_f8(const PthAttnWriteF8Args& a, hipStream_t stream) {
   }
   const bool wide = on16(a.key, a.key_stride_token, a.num_tokens, a.key_stride_head, c.num_kv_heads) &&
                     on16(a.value, a.value_stride_token, a.num_tokens, a.value_stride_head, c.num_kv_heads);
-  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + w.tokens - 1) / w.tokens),
+  const int64_t runs = (int64_t{a.num_tokens} + w.tokens - 1) / w.tokens;
+  PA_REQUIRE(runs <= kMostThreads / (many ? kManyThreads : kThreads),
+             "num_tokens needs more than 2^32 threads");
+  const dim3 grid(static_cast<unsigned>(runs),
                   static_cast<unsigned>((c.num_kv_heads + w.heads - 1) / w.heads));
   switch (c.head_size) {
     case 64: write_d<64>(w, a.kv_dtype, wide, many, grid, stream); break;
@@ -624,7 +627,9 @@ int32_t launch_gather_f8(const PthAttnGatherF8Args& a, hipStream_t stream) {
   while (g.tokens > 2 && (g.tokens * g.row_items > kPiecesAhead * kThreads / 2 ||
                           (g.tokens > 4 && a.num_tokens < 2 * cus * g.tokens)))
     g.tokens /= 2;
-  const dim3 grid(static_cast<unsigned>((int64_t{a.num_tokens} + g.tokens - 1) / g.tokens));
+  const int64_t runs = (int64_t{a.num_tokens} + g.tokens - 1) / g.tokens;
+  PA_REQUIRE(runs <= kMostThreads / kThreads, "num_tokens needs more than 2^32 threads");
+  const dim3 grid(static_cast<unsigned>(runs));
   switch (c.head_size) {
     case 64: gather_d<64>(g, a.kv_dtype, grid, stream); break;
     case 256: gather_d<256>(g, a.kv_dtype, grid, stream); break;

@@ -273,7 +273,9 @@ int32_t launch_rotary(const PthAttnRotaryArgs& a, hipStream_t stream) {
   p.tokens = std::max(1, std::min(kRotPairs / half, a.num_tokens >= 4096 ? 4 : 1));
   const int64_t items = heads * p.row_items * p.tokens;
   PA_REQUIRE(items < INT32_MAX, "heads x head_size is too large");
-  const dim3 grid(static_cast<unsigned>((a.num_tokens + p.tokens - 1) / p.tokens),
+  const int64_t groups = (int64_t{a.num_tokens} + p.tokens - 1) / p.tokens;
+  PA_REQUIRE(groups <= kMostThreads / kRotThreads, "num_tokens needs more than 2^32 threads");
+  const dim3 grid(static_cast<unsigned>(groups),
                   static_cast<unsigned>(a.num_tokens >= 1024
                                             ? 1
                                             : std::min<int64_t>((items + kRotThreads - 1) / kRotThreads, 8)));
