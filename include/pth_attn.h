@@ -306,7 +306,7 @@ typedef struct PthAttnRotaryArgs {
   int32_t num_tokens;
   int32_t num_q_heads;
   int32_t num_kv_heads;
-  int32_t head_size; /* 1 .. 1024 */
+  int32_t head_size; /* 2 .. 1024 */
   int32_t rot_dim;   /* even, 2 .. head_size */
   int32_t interleaved;
   int32_t inverse;
@@ -552,8 +552,8 @@ int32_t pth_attn_write_f8_args_bytes(void);
 int32_t pth_attn_gather_f8(const PthAttnGatherF8Args* args, void* stream);
 int32_t pth_attn_gather_f8_args_bytes(void);
 
-/* Attention over a paged 8-bit cache: see PthAttnPagedF8Args. At most two kernels on
- * `stream`, no allocation, no sync. The workspace holds nothing between calls;
+/* Attention over a paged 8-bit cache: see PthAttnPagedF8Args. At most four kernels on
+ * `stream` (two where the batch is not one of prompts and decodes), no allocation, no sync. The workspace holds nothing between calls;
  * calls that overlap in time need one each. */
 int32_t pth_attn_paged_f8(const PthAttnPagedF8Args* args, void* stream);
 int32_t pth_attn_paged_f8_args_bytes(void);

@@ -65,8 +65,7 @@ __global__ __launch_bounds__(64 * kP16Waves, RowsDim<D>::kPerSimd) void f8_rows(
   using R = RowsDim<D>;
   using V = typename Words<R::kWords>::type;
   constexpr int kBM = kP16RowsRows;
-  // The sums of the waves that are not their unit's first, at the end; Q
-  // before it.
+  // The sums of the waves that are not their unit's first, at the end.
   __shared__ f32x4 s_x[kP16Waves][R::kO][64];
   __shared__ float s_m[kP16Waves][kBM], s_l[kP16Waves][kBM];
   // Of a NaN in V: its keys in a chunk, by column; the outputs of a lane that meet it.

@@ -14,8 +14,11 @@
 // Numerics. Scores, m, l and o are 32 bits; the running maximum moves only when
 // a score passes it by 2^kSlack, so most tiles rescale nothing; P is scaled by
 // 2^-kBias, so that sums of values near the type's largest do not leave 32
-// bits. bf16: K's and V's values are exact, P is rounded once, and l sums the
-// rounded P. fp16: K's codes are exact in fp16, their scale is a factor of the
+// bits. bf16: K's and V's values are exact, P is rounded once, to 8 bits, and l sums
+// the rounded P: as in the 16-bit cache's kernel that is an error of the output's own
+// size and independent of it (against 64 bits 0.0022 of an output's size, with an exact P
+// 0.0017), and the rest of P would be a second PV product (fp16, below: 760 us for 533).
+// fp16: K's codes are exact in fp16, their scale is a factor of the
 // scores; V is in bf16, whose range its values need, and P a bf16 pair hi + lo.
 // A row does not see the keys behind its own, nor the slots behind the request's
 // last key in their block: where one of these has a NaN in V, it is taken out of the
@@ -23,10 +26,13 @@
 //
 // Bound: the SIMDs' issue. 4 requests of 2,048 rows against 4,096 keys, 32 heads over 8
 // of 128, 533 us, 1,031 TFLOP/s: matrix instructions 47 % of the cycles, vector ones
-// (softmax, conversions) 44 %, and little of the two goes on at once, be it of one wave
-// (a product of 32 cycles with four additions behind it takes 46) or of two. So codes are
-// converted once for four waves, and nothing else is asked of a tile than its softmax
-// needs. Heads of 64 339 us. Heads of 256, 16 over 8, 709 us: registers for one wave of a
+// (softmax, conversions) 50 %. The two can go on at once: a product of 32 cycles with four
+// additions behind it takes 34, of one wave, and of two waves of a SIMD one's products
+// keep their rate beside the other's additions, these 83 % of theirs. In batches they do
+// so less (sixteen products, then 64 additions: 51 cycles a product, 40 with two waves),
+// and a tile is batches, of scores, softmax and PV, that a barrier starts together in
+// all waves. So codes are converted once for four waves, and nothing else is asked of a
+// tile than its softmax needs. Heads of 64 339 us. Heads of 256, 16 over 8, 709 us: registers for one wave of a
 // SIMD alone, and 64 KB written to LDS and 256 KB read for a tile, at some 80 bytes a
 // cycle.
 

@@ -10,8 +10,9 @@
 // for K and V apart: the rows of up to 16 tokens in registers, their largest
 // value over the wave, the scale, the codes. So a value is read once and a code
 // written once, whatever the order of the tokens, in one launch and without an
-// atomic in memory. Rows that the block holds already are touched only if its
-// scale grows.
+// atomic in memory. Rows that the block holds already are read with them, before it
+// is known whether the scale grows, and written only if it does; not where the call
+// begins the block.
 //
 // Bound: its bytes, behind the reading of slot_mapping (8 heads of 128, bf16, cold:
 // 16,384 tokens, 101 MB, 23.0 us); latency for a decode step, whose tokens lie in blocks
