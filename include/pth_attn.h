@@ -553,8 +553,9 @@ int32_t pth_attn_gather_f8(const PthAttnGatherF8Args* args, void* stream);
 int32_t pth_attn_gather_f8_args_bytes(void);
 
 /* Attention over a paged 8-bit cache: see PthAttnPagedF8Args. At most four kernels on
- * `stream` (two where the batch is not one of prompts and decodes), no allocation, no sync. The workspace holds nothing between calls;
- * calls that overlap in time need one each. */
+ * `stream` (two where the batch is not one of prompts and decodes), no allocation, no
+ * sync. The workspace holds nothing between calls; calls that overlap in time need one
+ * each. */
 int32_t pth_attn_paged_f8(const PthAttnPagedF8Args* args, void* stream);
 int32_t pth_attn_paged_f8_args_bytes(void);
 /* Floats of its workspace at this head size on the current device, whatever

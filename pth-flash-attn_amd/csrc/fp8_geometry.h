@@ -64,14 +64,15 @@ PA_HD int32_t f8_tiles_before(const F8Steps& s, int32_t m, int32_t group, const 
                                     : static_cast<uint32_t>(sum / static_cast<uint32_t>(group));
   return static_cast<int32_t>(f) + (m > s.linear ? m - s.linear : 0) * s.cap;
 }
+
 // Whether every unit of 128 rows is left whole (one "tile"): where all are short, or as
 // many as the longest has a share in the whole. Whole ones end unevenly, cut ones write
-// and read their sums. Prompts, 8 heads of 128, whole and cut: 1
-// prompt of 2,048 tokens 63 and 74 us, of 8,192 549 and 611; 4 of 2,048 175 and 216; 4 of
-// 1,900 behind 5,900 keys 855 and 905; 12 of 100 to 2,000 behind up to 7,000 642 and 723; one
-// head, 1 of 2,048 54 and 40, 1 of 8,192 208 and 191. Heads of 256, 4 of them: 1 of 1,024 58
-// and 52, of 4,096 208 and 280; 5 of 500 to 2,500 behind 100 to 6,200 440 and 542.
-// Many short units are better walked by work-groups that stay: 64 of 256 140 and 122.
+// and read their sums. Prompts, 8 heads of 128, whole and cut: 1 of 2,048 tokens 63 and 74
+// us, of 8,192 549 and 611; 4 of 2,048 175 and 216; 4 of 1,900 behind 5,900 keys 855 and
+// 905; 12 of 100 to 2,000 behind up to 7,000 642 and 723; one head, 1 of 2,048 54 and 40, 1
+// of 8,192 208 and 191. Heads of 256, 4 of them: 1 of 1,024 58 and 52, of 4,096 208 and
+// 280; 5 of 500 to 2,500 behind 100 to 6,200 440 and 542. Many short units are better
+// walked by work-groups that stay: 64 of 256 140 and 122.
 inline bool f8_whole_wide(int32_t head_size, int64_t span, int64_t units, int32_t cus) {
   if (span > int64_t{1} << 30) return false;  // such a tile's keys are added to a length
   if (units > 5 * p16_resident(head_size) * cus && span < 1024) return false;

@@ -32,9 +32,9 @@
 // so less (sixteen products, then 64 additions: 51 cycles a product, 40 with two waves),
 // and a tile is batches, of scores, softmax and PV, that a barrier starts together in
 // all waves. So codes are converted once for four waves, and nothing else is asked of a
-// tile than its softmax needs. Heads of 64 339 us. Heads of 256, 16 over 8, 709 us: registers for one wave of a
-// SIMD alone, and 64 KB written to LDS and 256 KB read for a tile, at some 80 bytes a
-// cycle.
+// tile than its softmax needs. Heads of 64 339 us. Heads of 256, 16 over 8, 709 us:
+// registers for one wave of a SIMD alone, and 64 KB written to LDS and 256 KB read for a
+// tile, at some 80 bytes a cycle.
 
 #include "fp8_device.h"
 
