@@ -391,7 +391,7 @@ typedef struct PthAttnPagedF8Args {
   const int32_t* kv_lens;         /* [num_reqs] */
   const int32_t* query_start_loc; /* [num_reqs + 1] or NULL */
   int32_t block_table_width;
-  int32_t max_kv_len; /* no request has more keys */
+  int32_t max_kv_len; /* no request has more keys (nor more than 2^31 - 8,193) */
   int32_t dtype;      /* of q and out: PTH_ATTN_F16 or PTH_ATTN_BF16 */
   int32_t num_reqs;
   int32_t num_tokens;

@@ -210,10 +210,8 @@ int32_t launch_paged_f8(const PthAttnPagedF8Args& a, hipStream_t stream) {
   p.g_div = Div32::make(static_cast<uint32_t>(p.group));
   p.num_blocks = c.num_blocks;
   const int64_t reach = static_cast<int64_t>(a.block_table_width) * c.block_size;
-  // Key positions stay below 2^31 with what the kernels add to them to spare: the rest of
-  // a tile, the next chunks of the 16-row kernel's waves (less than 600).
-  const int64_t most = INT32_MAX - 1024;
-  p.max_keys = static_cast<int32_t>(std::min({static_cast<int64_t>(a.max_kv_len), reach, most}));
+  p.max_keys = static_cast<int32_t>(
+      std::min({static_cast<int64_t>(a.max_kv_len), reach, int64_t{kF8MostKeys}}));
   p.num_reqs = a.num_reqs;
   p.num_tokens = a.num_tokens;
   p.num_kv_heads = c.num_kv_heads;

@@ -247,8 +247,7 @@ __global__ __launch_bounds__(64 * kP16Waves, WideOf<D>::kPerSimd) void f8_wide(
     int window = t0;
     const auto refill = [&](int t) {
       window = t;
-      const F8Block b =
-          f8_block(p, table, u.head, f8_tile_block(base, t + lane, t1 - 1, wave, len));
+      const F8Block b = f8_block(p, table, u.head, f8_tile_block(base, t + lane, wave, len));
       s_window[wave].address[lane] =
           (u32x4){static_cast<uint32_t>(b.k), static_cast<uint32_t>(b.k >> 32),
                   static_cast<uint32_t>(b.v), static_cast<uint32_t>(b.v >> 32)};

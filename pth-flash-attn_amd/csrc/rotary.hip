@@ -21,7 +21,7 @@
 // large call do not fit them.
 //
 // Bound: its bytes (16,384 tokens, 32 + 8 heads of 128, bf16, cold: 335 MB, 64.5 us, 5.2 TB/s);
-// latency for a decode step (64 tokens 2.5 us).
+// latency for a decode step (64 tokens 2.7 us).
 
 #include <hip/hip_runtime.h>
 

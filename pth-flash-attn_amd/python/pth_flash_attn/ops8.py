@@ -266,8 +266,8 @@ def paged_attn_fp8_fwd(
     (in V, its column).
 
     ``max_query_len`` chooses kernel and split (any value is correct);
-    ``max_seq_len`` bounds the lengths (longer ones are cut there, and at the
-    block table's reach); a page number outside the cache reads page 0. ``ws`` is
+    ``max_seq_len`` bounds the lengths (longer ones are cut there, at the block
+    table's reach and at 2^31 - 8,193 keys); a page number outside the cache reads page 0. ``ws`` is
     workspace of ``planner.fp8_workspace_floats`` floats; it holds nothing between
     calls, and calls that can run at the same time need one each. ``out`` may be
     ``q`` itself; other than that they share no memory.

@@ -22,7 +22,7 @@ using namespace pa;
     }                                                           \
   } while (0)
 
-constexpr int64_t kMostKeys = INT32_MAX - 1024;  // of a request, as the launcher bounds it
+constexpr int64_t kMostKeys = kF8MostKeys;
 
 // Blocks of the 64 tiles whose addresses a wave makes at once, up to the longest
 // request: within its keys, and those of the unit's own tiles as they are.
@@ -39,16 +39,14 @@ static void tile_blocks() {
         for (int lane = 0; lane < 64; ++lane)
           for (int wave = 0; wave < kP16Waves; ++wave) {
             const int32_t got = f8_tile_block(static_cast<int32_t>(base),
-                                              static_cast<int32_t>(t + lane),
-                                              static_cast<int32_t>(last), wave,
+                                              static_cast<int32_t>(t + lane), wave,
                                               static_cast<int32_t>(len));
             const int64_t end = (len - 1) & ~int64_t{15};
             CHECK(got >= base && got <= end, "key block %d of [%lld, %lld]", got,
                   (long long)base, (long long)end);
-            if (t + lane <= last)
-              CHECK(got == std::min(base + kP16WideKeys * (t + lane) + 16 * wave, end),
-                    "tile %lld of %lld keys from %lld on: block %d", (long long)(t + lane),
-                    (long long)len, (long long)base, got);
+            CHECK(got == std::min(base + kP16WideKeys * (t + lane) + 16 * wave, end),
+                  "tile %lld of %lld keys from %lld on: block %d", (long long)(t + lane),
+                  (long long)len, (long long)base, got);
           }
     }
   std::printf("tile blocks ok\n");
